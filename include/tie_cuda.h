@@ -249,6 +249,85 @@ int tie_cuda_moe_ffn_ep(tie_cuda_ctx *c, int layer, const float *x, float *out, 
  * experts spread over the ranks (the layer's ffn_norm_w must have been uploaded). */
 int tie_cuda_moe_block_inplace_ep(tie_cuda_ctx *c, int layer, float *hidden_dev, int n_tokens, unsigned flags);
 
+/* ---- attention over a paged cache: the other half of a layer, between its projections ----
+ * engine.c:263-862 keeps one conversation's keys and values in host memory and works on them token by token.  Here they
+ * stay on the device in pages that any number of sequences share out among themselves, in 16 or 8 bits, and a step's
+ * tokens - single tokens, trees of drafted tokens, pieces of prompts, several sequences at once - are one launch each for
+ * writing and for attention.
+ *
+ * The cache is the caller's: two arrays of device memory, [n_pages][n_head_kv][page_size][head_dim] elements each, 16-byte
+ * aligned, and for TIE_CUDA_KV_Q8 two of fp32 factors, [n_pages][n_head_kv][page_size].  An element of Q8 is a whole number
+ * of -127 .. 127 that stands for itself times its row's factor; rows are written as rint(x / s), s = max|x| / 127 (IEEE
+ * divisions).  A row with an infinity or NaN in it reads back as NaN throughout, one whose s would be below 2^-126 as
+ * zeros.  F16 rounds to nearest and holds infinities beyond +-65504. */
+#define TIE_CUDA_KV_F32 0 /* rows that tie_cuda_kv_read puts out; no cache has this type */
+#define TIE_CUDA_KV_F16 1
+#define TIE_CUDA_KV_BF16 2 /* KV_CACHE_TYPE, config.h */
+#define TIE_CUDA_KV_Q8 3
+typedef struct {
+	int type;	/* TIE_CUDA_KV_F16, _BF16 or _Q8 */
+	int n_head_kv;	/* 1 .. 256 */
+	int head_dim;	/* 64 or 128 (else TIE_CUDA_ENOTSUP) */
+	int page_size;	/* slots of a page: a power of two, 16 .. 65536 */
+	int n_pages;
+	void *k, *v;
+	float *k_scale, *v_scale; /* Q8 only, else NULL */
+} tie_cuda_kv_cache;
+
+/* The tokens of a step.  Sequence s has rows tok_start[s] .. tok_start[s+1] - 1 of the step's arrays (none, if they are
+ * equal); its row i belongs to its slot kv_len[s] + i, and slot j lies in page page_table[s][j / page_size] at place
+ * j % page_size.  Rows that no sequence has (a padded batch: n_tokens above tok_start[n_seq]) are neither read nor written.
+ * The arrays are device memory, read by the kernels: a captured step follows them when it is replayed.
+ * What does not fit - a page number outside the cache, rows outside [0, n_tokens), negative lengths, slots behind the row
+ * of the page table, more than 64 tokens of a sequence with a tree - is left out by the kernels and makes the call (with
+ * TIE_CUDA_NO_SYNC: the next synchronising one) return TIE_CUDA_EKERNEL.  No slot may belong to two rows of one step. */
+typedef struct {
+	int n_seq;		/* 1 .. 1024 */
+	int n_tokens;		/* rows of the step's arrays, 0 included */
+	const int *tok_start;	/* [n_seq + 1], ascending */
+	const int *kv_len;	/* [n_seq] slots in front of this step's tokens */
+	const int *page_table;	/* [n_seq][max_pages] */
+	int max_pages;		/* max_pages * page_size at most 2^30 */
+	const uint64_t *tree;	/* tie_cuda_attn: [n_tokens], bit j: the token sees its sequence's token j of this step (itself
+				 * only if its own bit is set; what lies in front of the step it sees in any case).  NULL: a token
+				 * sees the step's tokens up to itself */
+	const int *pos;		/* tie_cuda_qk_norm_rope: [n_tokens] positions of the rotation (the depth of a drafted token is not
+				 * its slot); NULL: the slot */
+} tie_cuda_kv_step;
+
+/* q, k and v of a step as they leave their projections, fp32 in device memory.  Strides are the floats from one token's
+ * row to the next (a multiple of 4, at least heads * head_dim): the three may be parts of one array. */
+typedef struct {
+	int n_head; /* query heads, a multiple of the cache's n_head_kv */
+	const float *q, *k, *v;
+	int64_t q_stride, k_stride, v_stride;
+	const float *q_norm_w, *k_norm_w; /* [head_dim] device, or NULL: no norm */
+	float norm_eps;
+	float rope_base;      /* pair i turns by position * rope_base^(-2 i / head_dim); 0: no rotation */
+	int rope_interleaved; /* 0: pairs (i, i + head_dim / 2); 1: pairs (2 i, 2 i + 1) */
+	float *q_out;	      /* [n_tokens][n_head][head_dim]; may be q itself if q's rows lie as closely */
+} tie_cuda_attn_qkv;
+
+/* q_out = rotate(norm(q)); the cache's slots of the step's tokens = rotate(norm(k)), v (model_qwen3.c:312-380: the norms of
+ * queries and keys for each head, the rotation and the store into the cache).  norm(x) = x * w / sqrt(mean(x^2) + eps) over
+ * a head.  Angles are formed in 64 bits.  The entry points from here to tie_cuda_attn take device pointers (TIE_CUDA_DEVICE, with or
+ * without TIE_CUDA_NO_SYNC), arrays of floats and of rows 16-byte aligned (else TIE_CUDA_EINVAL), and allocate nothing: a
+ * caller may capture them into a graph of its own (TIE_CUDA_GRAPH is ignored).  Calls of one
+ * context share its scratch and follow one another on its stream; so have replays of graphs that were captured from it. */
+int tie_cuda_qk_norm_rope(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step,
+			  const tie_cuda_attn_qkv *in, unsigned flags);
+/* k_out, v_out [n_tokens][n_head_kv][head_dim] of out_type (TIE_CUDA_KV_F32, _F16 or _BF16) = what the cache holds in the
+ * slots of the step's tokens; kv_len all 0 and tok_start from the sequences' lengths read everything back. */
+int tie_cuda_kv_read(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, void *k_out, void *v_out,
+		     int out_type, unsigned flags);
+/* out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q[t][h] . k_j), over the slots that token t sees, from the cache
+ * as it is (the step's own tokens must have been written); q, out [n_tokens][n_head][head_dim], n_head a multiple of the
+ * cache's n_head_kv, query head h with key/value head h / (n_head / n_head_kv).  A token that sees nothing gets zeros; what
+ * stands in slots that a token does not see, NaN included, is nothing to it.  fp32 results: queries and probabilities
+ * meet the cache's elements in parts that keep 22 bits (BF16: 24).  out may be q. */
+int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const float *q, int n_head,
+		  float scale, float *out, unsigned flags);
+
 /* ---- math_dispatch.c rows (accel = 2) ----
  * Same argument meaning as the reference's kernels are CALLED with (math_dispatch.c:224,254):
  * (X, W_data, O, in_dim, start_row, end_row); X, O host fp32.  W must point into (or at) a

@@ -1,5 +1,7 @@
 // C ABI of the library (include/tie_cuda.h): context, weight residency, the MoE feed-forward
 // call and the math_dispatch rows.  Host logic only; kernels live in the other translation units.
+#include <float.h>
+#include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -14,6 +16,7 @@
 
 #include "common.cuh"
 #include "ep_dev.cuh"
+#include "kv_cache.cuh"
 #include "kernels.cuh"
 #include "copy_pool.h"
 
@@ -82,6 +85,9 @@ int alloc_scratch(tie_cuda_ctx *c)
 	TRY(dev_alloc(c, &s.hq, s.rows_pad * XF));
 	TRY(dev_alloc(c, &s.route_counter, (T + 3) / 4));
 	TIE_CUDA_TRY(c, cudaMemset(s.route_counter, 0, (T + 3) / 4 * sizeof(int)));
+	TRY(dev_alloc(c, &s.attn_part, attn_part_floats(c)));
+	TRY(dev_alloc(c, &s.attn_count, c->sm_count));
+	TIE_CUDA_TRY(c, cudaMemset(s.attn_count, 0, c->sm_count * sizeof(unsigned)));
 	TRY(dev_alloc(c, &s.dec_sync, 2));
 	TIE_CUDA_TRY(c, cudaMemset(s.dec_sync, 0, 2 * sizeof(unsigned)));
 	TRY(dev_alloc(c, &s.row_expert, R));
@@ -233,9 +239,10 @@ int check_status_pinned(tie_cuda_ctx *c)
 int report_status(tie_cuda_ctx *c, unsigned st)
 {
 	if (st) {
-		snprintf(c->cuda_err, sizeof(c->cuda_err), "device status word 0x%x (%s%s%s)", st,
+		snprintf(c->cuda_err, sizeof(c->cuda_err), "device status word 0x%x (%s%s%s%s%s)", st,
 			 (st & ST_BAD_EXPERT) ? "expert id out of range " : "", (st & ST_WAIT_TIMEOUT) ? "barrier wait timed out " : "",
-			 (st & ST_BAD_TILE) ? "tile bookkeeping " : "");
+			 (st & ST_BAD_TILE) ? "tile bookkeeping " : "", (st & ST_BAD_PAGE) ? "page outside the cache " : "",
+			 (st & ST_BAD_STEP) ? "rows or slots of a step out of range " : "");
 		cudaMemsetAsync(c->s.status, 0, sizeof(unsigned), c->stream);
 		if (st & ST_WAIT_TIMEOUT)  // a grid barrier of the one-kernel decode step may have been left half-counted
 			cudaMemsetAsync(c->s.dec_sync, 0, 2 * sizeof(unsigned), c->stream);
@@ -399,6 +406,40 @@ int moe_block_device(tie_cuda_ctx *c, Layer &L, float *hidden, int n_tokens, uns
 		return moe_ffn_device(c, L, hidden, hidden, n_tokens, nullptr, hidden, flags, nullptr, c->s.x);
 	TRY(launch_rms_norm(c, hidden, L.norm_w, c->s.x, n_tokens));
 	return moe_ffn_device(c, L, c->s.x, hidden, n_tokens, nullptr, hidden, flags);
+}
+
+bool aligned16(const void *p)
+{
+	return ((uintptr_t)p & 15) == 0;
+}
+
+// What the host can see of a cache and a step.  *idle: a step without rows.
+int kv_views(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, unsigned flags, KvView &kv, StepView &st, bool &idle)
+{
+	if (!cache || !step || !(flags & TIE_CUDA_DEVICE))
+		return TIE_CUDA_EINVAL;
+	const bool q8 = cache->type == TIE_CUDA_KV_Q8;
+	if (!q8 && cache->type != TIE_CUDA_KV_F16 && cache->type != TIE_CUDA_KV_BF16)
+		return TIE_CUDA_ENOTSUP;
+	if (cache->head_dim != 64 && cache->head_dim != 128)
+		return TIE_CUDA_ENOTSUP;
+	if (cache->n_head_kv < 1 || cache->n_head_kv > 256 || cache->page_size < 16 || cache->page_size > 65536 ||
+	    (cache->page_size & (cache->page_size - 1)) || cache->n_pages < 1 || !cache->k || !cache->v || !aligned16(cache->k) ||
+	    !aligned16(cache->v))
+		return TIE_CUDA_EINVAL;
+	if (q8 && (!cache->k_scale || !cache->v_scale || ((uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & 3))
+		return TIE_CUDA_EINVAL;
+	if (step->n_seq < 1 || step->n_seq > KV_MAX_SEQ || step->n_tokens < 0 || !step->tok_start || !step->kv_len || !step->page_table ||
+	    step->max_pages < 1 || (long long)step->max_pages * cache->page_size > 1 << 30 ||
+	    ((uintptr_t)step->tok_start | (uintptr_t)step->kv_len | (uintptr_t)step->page_table | (uintptr_t)step->pos) & 3 ||
+	    (uintptr_t)step->tree & 7 || !c)
+		return TIE_CUDA_EINVAL;
+	kv = {static_cast<uint8_t *>(cache->k), static_cast<uint8_t *>(cache->v), cache->k_scale, cache->v_scale, cache->n_head_kv,
+	      __builtin_ctz(cache->page_size), cache->n_pages};
+	st = {step->tok_start, step->kv_len, step->page_table, reinterpret_cast<const unsigned long long *>(step->tree), step->pos,
+	      step->n_seq, step->n_tokens, step->max_pages, c->s.status};
+	idle = step->n_tokens == 0;
+	return TIE_CUDA_OK;
 }
 
 struct GraphKey {
@@ -793,6 +834,8 @@ int tie_cuda_init(tie_cuda_ctx **out, const tie_cuda_config *cfg)
 		return fail(rc);
 	if ((rc = decode_group_setup(c)) != TIE_CUDA_OK)
 		return fail(rc);
+	if ((rc = attn_setup(c)) != TIE_CUDA_OK)
+		return fail(rc);
 	*out = c;
 	return TIE_CUDA_OK;
 }
@@ -826,7 +869,7 @@ void tie_cuda_destroy(tie_cuda_ctx *c)
 	void *dev_ptrs[] = {s.x,     s.out_base, s.logits, s.bias,  s.topk_idx, s.topk_w, s.counts, s.offsets, s.tile_start, s.active, s.n_active,
 			    s.perm,  s.h,     s.y,	s.xs_hi, s.hs_hi,  s.row_expert, c->silu,  c->row_x,
 			    c->row_o, s.ep_counts, s.ep_offsets, s.ep_tile_start, s.ep_active, s.ep_n_active, s.ep_perm, s.ep_inv, s.inv,
-			    s.tile_info, s.xq, s.hq, s.dec_sync, c->df_table, s.sort_hist, s.route_counter};
+			    s.tile_info, s.xq, s.hq, s.dec_sync, c->df_table, s.sort_hist, s.route_counter, s.attn_part, s.attn_count};
 	for (void *p : dev_ptrs)
 		if (p)
 			cudaFree(p);
@@ -1632,6 +1675,87 @@ int tie_cuda_moe_block_inplace_ep(tie_cuda_ctx *c, int layer, float *hidden_dev,
 		}
 		return rc;
 	}));
+	if (flags & TIE_CUDA_NO_SYNC)
+		return TIE_CUDA_OK;
+	return check_status(c);
+}
+
+// ---- attention over a paged cache ----
+
+static int attn_heads(const tie_cuda_kv_cache *cache, int n_head)
+{
+	return n_head >= 1 && n_head <= 1024 && n_head % cache->n_head_kv == 0 ? TIE_CUDA_OK : TIE_CUDA_EINVAL;
+}
+
+int tie_cuda_qk_norm_rope(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const tie_cuda_attn_qkv *in,
+			  unsigned flags)
+{
+	KvView kv;
+	StepView st;
+	bool idle;
+	TRY(kv_views(c, cache, step, flags, kv, st, idle));
+	if (!in)
+		return TIE_CUDA_EINVAL;
+	TRY(attn_heads(cache, in->n_head));
+	if (idle)
+		return TIE_CUDA_OK;
+	const int64_t d = cache->head_dim;
+	const void *const rows[] = {in->q, in->k, in->v, in->q_out};
+	for (const void *p : rows)
+		if (!p || !aligned16(p))
+			return TIE_CUDA_EINVAL;
+	const int64_t strides[] = {in->q_stride, in->k_stride, in->v_stride}, least[] = {in->n_head * d, cache->n_head_kv * d, cache->n_head_kv * d};
+	for (int i = 0; i < 3; i++)
+		if (strides[i] < least[i] || strides[i] % 4)
+			return TIE_CUDA_EINVAL;
+	// a token's row of q_out must not be another token's row of q
+	if (in->q_out == in->q && in->q_stride != in->n_head * d)
+		return TIE_CUDA_EINVAL;
+	if (((uintptr_t)in->q_norm_w | (uintptr_t)in->k_norm_w) & 3 || !(in->norm_eps >= 0.0f) || !(in->rope_base >= 0.0f) || in->rope_base > FLT_MAX)
+		return TIE_CUDA_EINVAL;
+	TIE_CUDA_TRY(c, cudaSetDevice(c->device));
+	TRY(launch_qk_norm_rope(c, kv, st, cache->type, cache->head_dim, *in));
+	if (flags & TIE_CUDA_NO_SYNC)
+		return TIE_CUDA_OK;
+	return check_status(c);
+}
+
+int tie_cuda_kv_read(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, void *k_out, void *v_out, int out_type,
+		     unsigned flags)
+{
+	KvView kv;
+	StepView st;
+	bool idle;
+	TRY(kv_views(c, cache, step, flags, kv, st, idle));
+	if (out_type != TIE_CUDA_KV_F32 && out_type != TIE_CUDA_KV_F16 && out_type != TIE_CUDA_KV_BF16)
+		return TIE_CUDA_ENOTSUP;
+	if (idle)
+		return TIE_CUDA_OK;
+	if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+		return TIE_CUDA_EINVAL;
+	TIE_CUDA_TRY(c, cudaSetDevice(c->device));
+	TRY(launch_kv_read(c, kv, st, cache->type, cache->head_dim, k_out, v_out, out_type));
+	if (flags & TIE_CUDA_NO_SYNC)
+		return TIE_CUDA_OK;
+	return check_status(c);
+}
+
+int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const float *q, int n_head, float scale,
+		  float *out, unsigned flags)
+{
+	KvView kv;
+	StepView st;
+	bool idle;
+	TRY(kv_views(c, cache, step, flags, kv, st, idle));
+	TRY(attn_heads(cache, n_head));
+	if (!(fabsf(scale) <= FLT_MAX))
+		return TIE_CUDA_EINVAL;
+	if (idle)
+		return TIE_CUDA_OK;
+	if (!q || !out || !aligned16(q) || !aligned16(out))
+		return TIE_CUDA_EINVAL;
+	TIE_CUDA_TRY(c, cudaSetDevice(c->device));
+	TRY(launch_attn(c, kv, st, cache->type, cache->head_dim, q, out, n_head, scale));
 	if (flags & TIE_CUDA_NO_SYNC)
 		return TIE_CUDA_OK;
 	return check_status(c);

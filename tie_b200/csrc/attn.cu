@@ -1,0 +1,769 @@
+// Attention of a step's tokens over the paged cache (engine.c:794-862 does it per head and token on the host):
+//
+//   out[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q[t][h].k_j - max),
+//
+// j over the slots in front of the step and the step's own tokens that t sees (its tree mask, or those up to itself); a
+// token that sees nothing gets zeros.  One pass over keys and values with a running maximum and sum.
+#include <float.h>
+
+#include "kernels.cuh"
+#include "kv_cache.cuh"
+#include "mma_dot.cuh"
+#include "tc_ptx.cuh"
+
+namespace tie {
+namespace {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int GROUP = 16;	       // keys a warp takes at a time
+constexpr int UNIT = GROUP * WARPS;    // keys of one round of a CTA: what work is shared out in
+constexpr int MAX_ROWS = 16;	       // query rows of a CTA's tile
+constexpr float P_SHIFT = 14.0f;       // p is held as p * 2^14: fp16 parts of it reach down to 2^-38 of the largest
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+	const float *q;
+	float *out;
+	int n_head, group;  // group: query heads per key/value head
+	float scale_log2e;
+	float *part;
+	unsigned *count;
+};
+
+template <int KIND, int D>
+struct Cfg {
+	static constexpr int ROW = KIND == TIE_CUDA_KV_Q8 ? D : 2 * D;	// bytes of a head row of the cache
+	static constexpr int CHUNKS = ROW / 16;
+	static constexpr int STAGE = 2 * GROUP * ROW + (KIND == TIE_CUDA_KV_Q8 ? 2 * GROUP * 4 : 0);
+	static constexpr int STAGES = STAGE > 4352 ? 3 : 4;
+	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	// parts of an fp32 operand: 3 x 8 or 2 x 11 bits
+	// a 16-byte chunk's place in its row: eight consecutive keys' chunks of a column lie in eight different bank groups
+	__device__ static __forceinline__ int place(int row, int ch)
+	{
+		return row * ROW + ((ch ^ (CHUNKS == 4 ? (row >> 1) & 3 : row & 7)) << 4);
+	}
+};
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool there)
+{
+	const int n = there ? 16 : 0;
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void *src, bool there)
+{
+	const int n = there ? 4 : 0;
+	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
+{
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+		     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+		     : "r"(addr)
+		     : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
+{
+	uint32_t r;
+	asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+	return r;
+}
+__device__ __forceinline__ void mma_16816_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+	    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+	    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int KIND>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+	if constexpr (KIND == TIE_CUDA_KV_BF16)
+		mma_16816_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+	else
+		mma_16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// Two of the four signed bytes of x as halves, exactly: byte + 128 becomes the mantissa of 1024 + byte + 128.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t int8_pair(uint32_t x_biased)
+{
+	const uint32_t h = __byte_perm(x_biased, 0x64646464u, SEL);
+	const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&h), __half2half2(__ushort_as_half(0x6480)));  // 1152
+	return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// (a, b) as PARTS pairs of 16-bit parts, the largest first, that add up to them (to 22 bits in fp16, all 24 in bf16).
+template <int KIND, int PARTS>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PARTS])
+{
+#pragma unroll
+	for (int p = 0; p < PARTS; p++) {
+		if constexpr (KIND == TIE_CUDA_KV_BF16) {
+			const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+			part[p] = *reinterpret_cast<const uint32_t *>(&h);
+			a -= __bfloat162float(h.x);
+			b -= __bfloat162float(h.y);
+		} else {
+			const __half2 h = __floats2half2_rn(a, b);
+			part[p] = *reinterpret_cast<const uint32_t *>(&h);
+			a -= __half2float(h.x);
+			b -= __half2float(h.y);
+		}
+	}
+}
+
+__device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exponent)
+{
+	return (w & exponent) == exponent || (w >> 16 & exponent) == exponent;
+}
+
+// The work of a launch: items = (sequence, key/value head, tile of query rows), each of as many units as its keys take;
+// CTA b of G does units [U b / G, U (b + 1) / G), whatever items these belong to.  An item within one CTA is finished there;
+// the CTAs that share one leave (maximum, sum, rows) behind, and the last to be done adds them up in the order of the
+// CTAs, so that the result does not depend on which was last.
+struct Work {
+	long long start[KV_MAX_SEQ + 1];  // units in front of a sequence
+	long long warp_sum[WARPS];
+	int last;
+};
+
+template <int NB>
+__device__ __forceinline__ long long seq_units(const KvView &kv, const AttnArgs &a, const SeqView &q)
+{
+	const long long tiles = ((long long)q.n_tok * a.group + 8 * NB - 1) / (8 * NB);
+	return tiles * kv.n_head_kv * (((long long)q.kv_len + q.n_tok + UNIT - 1) / UNIT);
+}
+
+template <int NB>
+__device__ void share_work(Work &w, const KvView &kv, const StepView &st, const AttnArgs &a)
+{
+	constexpr int PER = KV_MAX_SEQ / THREADS;
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	long long mine[PER], sum = 0;
+#pragma unroll
+	for (int i = 0; i < PER; i++) {
+		const int s = threadIdx.x * PER + i;
+		mine[i] = s < st.n_seq ? seq_units<NB>(kv, a, kv_sequence(st, kv.page_shift, s)) : 0;
+		sum += mine[i];
+	}
+	long long incl = sum;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1) {
+		const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+		if (lane >= o)
+			incl += v;
+	}
+	if (lane == 31)
+		w.warp_sum[warp] = incl;
+	__syncthreads();
+	long long at = incl - sum;
+	for (int i = 0; i < warp; i++)
+		at += w.warp_sum[i];
+#pragma unroll
+	for (int i = 0; i < PER; i++) {
+		const int s = threadIdx.x * PER + i;
+		if (s <= st.n_seq)
+			w.start[s] = at;
+		at += mine[i];
+	}
+	if (threadIdx.x == THREADS - 1)
+		w.start[st.n_seq] = at;	 // (n_seq = KV_MAX_SEQ)
+	__syncthreads();
+}
+
+// One warp's state over the groups of keys it takes: S^T = K Q^T and O^T = V^T P^T on m16n8k16, keys (then dims) on the
+// 16-row side, query rows on the 8-column side, so that a single token's 8 heads fill the columns.  A lane holds rows
+// 2c and 2c + 1 (c = lane % 4) of each block of 8.
+template <int KIND, int D, int NB>
+struct Warp {
+	using C = Cfg<KIND, D>;
+	static constexpr int KS = D / 16, MB = D / 16;
+	uint32_t q[NB][C::PARTS][KS][2];
+	float row_scale[NB][2];	 // scale * log2 e, and what the row's parts were divided by
+	float acc[NB][MB][4];
+	float m[NB][2], l[NB][2];  // running maximum (of the whole column), sum (of this lane's keys)
+
+	__device__ __forceinline__ void begin(const AttnArgs &a, const SeqView &seq, int head_kv, int row0, int lane)
+	{
+		const int g = lane >> 2, c = lane & 3;
+		const int n_rows = seq.n_tok * a.group;
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++) {
+			const int r = row0 + nb * 8 + g;
+			const bool there = r < n_rows;
+			const int tok = there ? r / a.group : 0;
+			const float *src = a.q + ((long long)(seq.tok0 + tok) * a.n_head + head_kv * a.group + (there ? r - tok * a.group : 0)) * D;
+			float2 v[KS][2];
+			float top = 0.0f;
+#pragma unroll
+			for (int j = 0; j < KS; j++) {
+				// the order of a step's 16 dims is free as long as keys have the same: that of packed bytes for Q8
+				if constexpr (KIND == TIE_CUDA_KV_Q8) {
+					const float4 f = there ? *reinterpret_cast<const float4 *>(src + 16 * j + 4 * c) : make_float4(0, 0, 0, 0);
+					v[j][0] = make_float2(f.x, f.y);
+					v[j][1] = make_float2(f.z, f.w);
+				} else {
+					v[j][0] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 2 * c) : make_float2(0, 0);
+					v[j][1] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 8 + 2 * c) : make_float2(0, 0);
+				}
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+					top = fmaxf(top, fmaxf(fabsf(v[j][h].x), fabsf(v[j][h].y)));
+			}
+			// fp16 parts: the row is brought to 1 .. 2 by a power of two (any fp32 row then keeps its 22 bits)
+			float down = 1.0f, up = 1.0f;
+			if constexpr (KIND != TIE_CUDA_KV_BF16) {
+				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+				const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+				if (top > 0.0f) {
+					down = __uint_as_float((unsigned)(254 - e) << 23);
+					up = __uint_as_float((unsigned)e << 23);
+				}
+			}
+#pragma unroll
+			for (int j = 0; j < KS; j++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					uint32_t part[C::PARTS];
+					split_pair<KIND>(v[j][h].x * down, v[j][h].y * down, part);
+#pragma unroll
+					for (int p = 0; p < C::PARTS; p++)
+						q[nb][p][j][h] = part[p];
+				}
+#pragma unroll
+			for (int i = 0; i < 2; i++) {
+				row_scale[nb][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4) * a.scale_log2e;
+				m[nb][i] = -INFINITY;
+				l[nb][i] = 0.0f;
+			}
+#pragma unroll
+			for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					acc[nb][mb][i] = 0.0f;
+		}
+	}
+
+	// 16 keys from key0 on, in shared memory at `stage`; keys at or behind key_end, and all of them unless `there`, are nobody's.
+	__device__ __forceinline__ void group(const AttnArgs &a, const StepView &st, const SeqView &seq, uint32_t stage, int key0, int key_end, bool there, int row0, int lane)
+	{
+		const int g = lane >> 2, c = lane & 3;
+		const uint32_t ks = stage, vs = stage + GROUP * C::ROW;
+		float s[NB][4];
+		{
+			float part[NB][C::PARTS][4];  // a chain each: the tensor cores cut every sum off
+#pragma unroll
+			for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+				for (int p = 0; p < C::PARTS; p++)
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						part[nb][p][i] = 0.0f;
+			const int krow = lane & 15, kch = lane >> 4;
+#pragma unroll
+			for (int j = 0; j < (KIND == TIE_CUDA_KV_Q8 ? KS / 2 : KS); j++) {
+				uint32_t r[4];
+				ldsm4(r, ks + C::place(krow, 2 * j + kch));
+				if constexpr (KIND == TIE_CUDA_KV_Q8) {
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						r[i] ^= 0x80808080u;
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						const uint32_t f[4] = {int8_pair<0x4140>(r[2 * h]), int8_pair<0x4140>(r[2 * h + 1]), int8_pair<0x4342>(r[2 * h]),
+								       int8_pair<0x4342>(r[2 * h + 1])};
+#pragma unroll
+						for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+							for (int p = 0; p < C::PARTS; p++)
+								mma<KIND>(part[nb][p], f, q[nb][p][2 * j + h][0], q[nb][p][2 * j + h][1]);
+					}
+				} else {
+#pragma unroll
+					for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+						for (int p = 0; p < C::PARTS; p++)
+							mma<KIND>(part[nb][p], r, q[nb][p][j][0], q[nb][p][j][1]);
+				}
+			}
+#pragma unroll
+			for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					float v = part[nb][C::PARTS - 1][i];
+#pragma unroll
+					for (int p = C::PARTS - 2; p >= 0; p--)
+						v += part[nb][p][i];
+					s[nb][i] = v * row_scale[nb][i & 1];
+				}
+		}
+		float v_top = 1.0f, v_rel[2] = {1.0f, 1.0f};
+		if constexpr (KIND == TIE_CUDA_KV_Q8) {
+			float f[4];
+#pragma unroll
+			for (int i = 0; i < 2; i++) {
+				const uint32_t at = stage + 2 * GROUP * C::ROW + 4 * (g + 8 * i);
+				asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[i]) : "r"(at) : "memory");
+				asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[2 + i]) : "r"(at + 4 * GROUP) : "memory");
+				// (an infinite factor is as little a number as NaN, and NaN does not reach the group's largest)
+				f[2 + i] = fabsf(f[2 + i]) <= FLT_MAX ? f[2 + i] : __int_as_float(0x7fc00000);
+			}
+#pragma unroll
+			for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					s[nb][i] *= f[i >> 1];
+			v_top = fmaxf(fabsf(f[2]), fabsf(f[3]));
+			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 4));
+			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 8));
+			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 16));
+			v_top = v_top > 0.0f ? v_top : 1.0f;
+			v_rel[0] = f[2] / v_top;
+			v_rel[1] = f[3] / v_top;
+		}
+		const bool masked = !there || key0 + GROUP > min(seq.kv_len, key_end);
+		if (masked) {
+#pragma unroll
+			for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+				for (int i = 0; i < 2; i++) {
+					const int r = row0 + nb * 8 + 2 * c + i, tok = min(r / a.group, seq.n_tok - 1);
+					unsigned long long bits = 0;
+					if (st.tree)
+						bits = st.tree[seq.tok0 + tok];
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						const int key = key0 + g + 8 * h, j = key - seq.kv_len;
+						const bool sees = there && key < key_end && (j < 0 || (st.tree ? j < KV_MAX_TREE && (bits >> j & 1) : j <= tok));
+						if (!sees)
+							s[nb][2 * h + i] = -INFINITY;
+					}
+				}
+		}
+		uint32_t b[NB][C::PARTS][2];  // P^T as the second operand
+		float alpha[NB][2];
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++) {
+			float base[2];
+#pragma unroll
+			for (int i = 0; i < 2; i++) {
+				float top = fmaxf(s[nb][i], s[nb][2 + i]);
+				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+				top = fmaxf(top, m[nb][i]);
+				base[i] = (top == -INFINITY ? 0.0f : top) - P_SHIFT;
+				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2f(m[nb][i] - top);
+				m[nb][i] = top;
+			}
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				s[nb][i] = exp2f(s[nb][i] - base[i & 1]);
+#pragma unroll
+			for (int i = 0; i < 2; i++)
+				l[nb][i] = fmaf(l[nb][i], alpha[nb][i], s[nb][i] + s[nb][2 + i]);
+			if constexpr (KIND == TIE_CUDA_KV_Q8) {
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					s[nb][i] = s[nb][i] == 0.0f ? 0.0f : s[nb][i] * v_rel[i >> 1];
+			}
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				uint32_t part[C::PARTS];
+				split_pair<KIND>(s[nb][2 * h], s[nb][2 * h + 1], part);
+#pragma unroll
+				for (int p = 0; p < C::PARTS; p++)
+					b[nb][p][h] = transpose8x8(part[p]);
+			}
+		}
+		if constexpr (KIND != TIE_CUDA_KV_Q8) {
+			// 0 * infinity is not nothing: where a group that not every row sees holds a value that is no number, its products
+			// are made one by one
+			bool odd = false;
+			if (masked) {
+				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
+				for (int i = lane; i < GROUP * C::ROW / 4; i += 32) {
+					uint32_t w;
+					asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vs + 4 * i) : "memory");
+					odd = odd || nonfinite16(w, EXPONENT);
+				}
+				odd = __any_sync(0xffffffffu, odd);
+			}
+			if (odd) {
+				one_by_one(vs, s, alpha, lane);
+				return;
+			}
+		}
+#pragma unroll
+		for (int mb = 0; mb < MB; mb++) {
+			uint32_t f[4];
+			if constexpr (KIND == TIE_CUDA_KV_Q8) {
+				if (mb & 1)
+					continue;
+				uint32_t r[4];	// (keys 0-7, 8-15) of 16 dims, then of the next 16; a unit of 16 bits is two neighbouring dims
+				ldsm4_trans(r, vs + C::place(lane & 15, mb + (lane >> 4)));
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					r[i] ^= 0x80808080u;
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const uint32_t e[4] = {int8_pair<0x4240>(r[2 * h]), int8_pair<0x4341>(r[2 * h]), int8_pair<0x4240>(r[2 * h + 1]),
+							       int8_pair<0x4341>(r[2 * h + 1])};
+					fold(mb + h, e, b, alpha, v_top);
+				}
+			} else {
+				ldsm4_trans(f, vs + C::place((lane & 7) + 8 * (lane >> 4), 2 * mb + (lane >> 3 & 1)));
+				fold(mb, f, b, alpha, v_top);
+			}
+		}
+	}
+
+	// acc = acc * alpha + (the 16 keys' products, summed up from zero: lo parts first, one cut-off sum a part)
+	__device__ __forceinline__ void fold(int mb, const uint32_t (&f)[4], const uint32_t (&b)[NB][C::PARTS][2], const float (&alpha)[NB][2], float v_top)
+	{
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++) {
+			float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+			for (int p = C::PARTS - 1; p >= 0; p--)
+				mma<KIND>(d, f, b[nb][p][0], b[nb][p][1]);
+#pragma unroll
+			for (int i = 0; i < 4; i++) {
+				if constexpr (KIND == TIE_CUDA_KV_Q8)
+					acc[nb][mb][i] = fmaf(d[i], v_top, acc[nb][mb][i] * alpha[nb][i & 1]);
+				else
+					acc[nb][mb][i] = fmaf(acc[nb][mb][i], alpha[nb][i & 1], d[i]);
+			}
+		}
+	}
+
+	// dim of acc[..][mb][i]
+	__device__ static __forceinline__ int dim(int mb, int i, int lane)
+	{
+		return KIND == TIE_CUDA_KV_Q8 ? 16 * mb + 2 * (lane >> 2) + (i >> 1) : 16 * mb + (lane >> 2) + 8 * (i >> 1);
+	}
+
+	__device__ __forceinline__ void one_by_one(uint32_t vs, const float (&p)[NB][4], const float (&alpha)[NB][2], int lane)
+	{
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+			for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					acc[nb][mb][i] *= alpha[nb][i & 1];
+#pragma unroll 1
+		for (int k = 0; k < GROUP; k++) {
+			float pk[NB][2];
+#pragma unroll
+			for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+					pk[nb][i] = __shfl_sync(0xffffffffu, k < 8 ? p[nb][i] : p[nb][2 + i], (k & 7) * 4 + (lane & 3));
+#pragma unroll
+			for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const int d = dim(mb, 2 * h, lane);
+					uint16_t raw;
+					asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw) : "r"(vs + C::place(k, d >> 3) + 2 * (d & 7)) : "memory");
+					const float v = KIND == TIE_CUDA_KV_F16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float((uint32_t)raw << 16);
+#pragma unroll
+					for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+						for (int i = 0; i < 2; i++)
+							if (pk[nb][i] != 0.0f)
+								acc[nb][mb][2 * h + i] = fmaf(pk[nb][i], v, acc[nb][mb][2 * h + i]);
+				}
+		}
+	}
+};
+
+template <int KIND, int D, int NB>
+constexpr size_t smem_bytes()
+{
+	using C = Cfg<KIND, D>;
+	constexpr size_t stages = (size_t)WARPS * C::STAGES * C::STAGE, rows = (size_t)WARPS * 8 * NB * D * 4;
+	return (stages > rows ? stages : rows) + 1024;
+}
+
+// floats that a CTA leaves for a shared item: rows, then per row maximum and sum
+constexpr int PART_FLOATS = MAX_ROWS * (128 + 2);
+
+template <int KIND, int D, int NB>
+__global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const StepView st, const AttnArgs a)
+{
+	using C = Cfg<KIND, D>;
+	constexpr int ROWS = 8 * NB;
+	extern __shared__ uint8_t smem_raw[];
+	__shared__ Work work;
+	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS];
+	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+	share_work<NB>(work, kv, st, a);
+	const long long total = work.start[st.n_seq];
+	const int n_cta = (int)min((long long)gridDim.x, total);  // (each of them has a unit at least)
+	if (cta >= n_cta)
+		return;
+	const long long u_begin = total * cta / n_cta, u_end = total * (cta + 1) / n_cta;
+	const uint32_t stages = ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE;
+	Warp<KIND, D, NB> w;
+	for (long long u = u_begin; u < u_end;) {
+		int lo = 0, hi = st.n_seq - 1;	// the sequence of unit u: the last that starts at or in front of it and has any
+		while (lo < hi) {
+			const int mid = (lo + hi + 1) >> 1;
+			if (work.start[mid] <= u)
+				lo = mid;
+			else
+				hi = mid - 1;
+		}
+		const int s = lo;
+		const SeqView seq = kv_sequence(st, kv.page_shift, s);
+		const int n_keys = seq.kv_len + seq.n_tok, item_units = (n_keys + UNIT - 1) / UNIT;
+		const int tiles = (seq.n_tok * a.group + ROWS - 1) / ROWS;
+		const long long in_seq = u - work.start[s], item = in_seq / item_units;
+		const int unit0 = (int)(in_seq - item * item_units);
+		const int unit1 = (int)min((long long)item_units, unit0 + (u_end - u));
+		const int head = (int)(item / tiles), row0 = (int)(item % tiles) * ROWS;
+		// a tile's last row sees the furthest unless a tree says otherwise
+		const int last_tok = min((row0 + ROWS - 1) / a.group, seq.n_tok - 1);
+		const int key_end = st.tree ? n_keys : seq.kv_len + last_tok + 1;
+		if (st.tree && seq.n_tok > KV_MAX_TREE && threadIdx.x == 0)
+			kv_report(st, ST_BAD_STEP);
+		const int g_first = unit0 * WARPS + warp, g_end = min(unit1 * WARPS, (key_end + GROUP - 1) / GROUP);
+		w.begin(a, seq, head, row0, lane);
+		const int *pages = st.page_table + (long long)s * st.max_pages;
+		const int page_mask = (1 << kv.page_shift) - 1;
+		unsigned there = 0;  // a bit per group in flight, the oldest highest
+		auto fetch = [&](int g, int page, int slot) {
+			const int key0 = g * GROUP;
+			const long long first = g < g_end ? kv_page_row(kv, st, page, head) : -1;
+			there = there << 1 | (first >= 0);
+			if (g < g_end) {
+				const uint32_t dst = stages + slot * C::STAGE;
+				const long long row0 = max(first, 0ll) + (key0 & page_mask);
+#pragma unroll
+				for (int i = 0; i < GROUP * C::CHUNKS / 32; i++) {
+					const int r = (lane + 32 * i) / C::CHUNKS, ch = (lane + 32 * i) % C::CHUNKS;
+					const bool in = first >= 0 && key0 + r < key_end;
+					const long long at = in ? (row0 + r) * C::ROW + ch * 16 : 0;
+					cp_async16_or_zero(dst + C::place(r, ch), kv.k + at, in);
+					cp_async16_or_zero(dst + GROUP * C::ROW + C::place(r, ch), kv.v + at, in);
+				}
+				if constexpr (KIND == TIE_CUDA_KV_Q8) {
+					const bool in = first >= 0 && key0 + (lane & 15) < key_end;
+					cp_async4_or_zero(dst + 2 * GROUP * C::ROW + 4 * lane, (lane < 16 ? kv.k_scale : kv.v_scale) + (in ? row0 + (lane & 15) : 0), in);
+				}
+			}
+			ptx::cp_async_commit();
+		};
+		auto page_of = [&](int g) { return g < g_end ? pages[g * GROUP >> kv.page_shift] : 0; };
+		int ahead[C::STAGES];
+#pragma unroll
+		for (int i = 0; i < C::STAGES; i++)
+			ahead[i] = page_of(g_first + i * WARPS);
+#pragma unroll
+		for (int i = 0; i < C::STAGES - 1; i++)
+			fetch(g_first + i * WARPS, ahead[i], i);
+		int next_page = ahead[C::STAGES - 1], slot = 0;
+		for (int g = g_first; g < g_end; g += WARPS) {
+			const int behind = g + (C::STAGES - 1) * WARPS;
+			const int page = next_page;
+			next_page = page_of(behind + WARPS);
+			fetch(behind, page, slot == 0 ? C::STAGES - 1 : slot - 1);
+			ptx::cp_async_wait<C::STAGES - 1>();
+			__syncwarp();
+			w.group(a, st, seq, stages + slot * C::STAGE, g * GROUP, key_end, there >> (C::STAGES - 1) & 1, row0, lane);
+			__syncwarp();
+			slot = slot + 1 == C::STAGES ? 0 : slot + 1;
+		}
+		ptx::cp_async_wait<0>();
+
+		// the warps' keys together
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+			for (int i = 0; i < 2; i++) {
+				float sum = w.l[nb][i];
+				sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+				sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+				sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+				if (lane < 4) {
+					s_m[warp][nb * 8 + 2 * lane + i] = w.m[nb][i];
+					s_l[warp][nb * 8 + 2 * lane + i] = sum;
+				}
+			}
+		__syncthreads();  // (and nobody reads keys any more)
+		if (threadIdx.x < ROWS) {
+			const int r = threadIdx.x;
+			float top = -INFINITY, sum = 0.0f;
+			for (int i = 0; i < WARPS; i++)
+				top = fmaxf(top, s_m[i][r]);
+			for (int i = 0; i < WARPS; i++) {
+				const float f = s_m[i][r] == -INFINITY ? 0.0f : exp2f(s_m[i][r] - top);
+				s_w[r][i] = f;
+				sum = fmaf(s_l[i][r], f, sum);
+			}
+			s_top[r] = top;
+			s_sum[r] = sum;
+		}
+		float *rows = reinterpret_cast<float *>(smem);	// [warp][row][D]
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+			for (int mb = 0; mb < D / 16; mb++)
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					rows[(warp * ROWS + nb * 8 + 2 * (lane & 3) + (i & 1)) * D + w.dim(mb, i, lane)] = w.acc[nb][mb][i];
+		__syncthreads();
+		const bool whole = unit0 == 0 && unit1 == item_units;
+		const int n_rows = seq.n_tok * a.group;
+		auto out_row = [&](int r) {
+			const int tok = r / a.group;
+			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + head * a.group + (r - tok * a.group)) * D;
+		};
+		float *part = a.part + (size_t)(2 * cta + (unit0 == 0 ? 1 : 0)) * PART_FLOATS;
+		for (int i = threadIdx.x; i < ROWS * D / 4; i += THREADS) {
+			const int r = i / (D / 4), col = i % (D / 4) * 4;
+			float4 sum = make_float4(0, 0, 0, 0);
+			for (int k = 0; k < WARPS; k++) {
+				const float f = s_w[r][k];
+				const float4 v = *reinterpret_cast<const float4 *>(rows + (k * ROWS + r) * D + col);
+				if (f != 0.0f) {  // (a warp whose keys the row does not see has nothing to give)
+					sum.x = fmaf(v.x, f, sum.x);
+					sum.y = fmaf(v.y, f, sum.y);
+					sum.z = fmaf(v.z, f, sum.z);
+					sum.w = fmaf(v.w, f, sum.w);
+				}
+			}
+			if (whole) {
+				if (row0 + r < n_rows) {
+					const float inv = s_sum[r] == 0.0f ? 0.0f : 1.0f / s_sum[r];
+					*reinterpret_cast<float4 *>(out_row(row0 + r) + col) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+				}
+			} else {
+				*reinterpret_cast<float4 *>(part + r * D + col) = sum;
+			}
+		}
+		if (!whole) {
+			if (threadIdx.x < ROWS) {
+				part[MAX_ROWS * 128 + threadIdx.x] = s_top[threadIdx.x];
+				part[MAX_ROWS * 128 + MAX_ROWS + threadIdx.x] = s_sum[threadIdx.x];
+			}
+			// the CTAs of the item: those of its first and last unit, and all between
+			const long long i0 = work.start[s] + item * item_units, i1 = i0 + item_units - 1;
+			const int c0 = (int)(((i0 + 1) * n_cta - 1) / total), c1 = (int)(((i1 + 1) * n_cta - 1) / total);
+			__threadfence();
+			__syncthreads();
+			if (threadIdx.x == 0)
+				work.last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
+			__syncthreads();
+			if (work.last) {
+				__threadfence();
+				const float *first = a.part + (size_t)(2 * c0 + 1) * PART_FLOATS;
+				const float *others = a.part + (size_t)2 * (c0 + 1) * PART_FLOATS;  // + 2 i PART_FLOATS
+				auto at = [&](int i) { return i == 0 ? first : others + (size_t)2 * (i - 1) * PART_FLOATS; };
+				const int n = c1 - c0 + 1;
+				for (int r = warp; r < ROWS && row0 + r < n_rows; r += WARPS) {
+					float top = -INFINITY, sum = 0.0f;
+					for (int i = lane; i < n; i += 32)
+						top = fmaxf(top, __ldcg(at(i) + MAX_ROWS * 128 + r));
+#pragma unroll
+					for (int o = 16; o; o >>= 1)
+						top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+					float acc[D / 32];
+#pragma unroll
+					for (int j = 0; j < D / 32; j++)
+						acc[j] = 0.0f;
+					for (int b = 0; b < n; b += 32) {
+						float f = 0.0f, li = 0.0f;
+						if (b + lane < n) {
+							const float mi = __ldcg(at(b + lane) + MAX_ROWS * 128 + r);
+							f = mi == -INFINITY ? 0.0f : exp2f(mi - top);
+							li = __ldcg(at(b + lane) + MAX_ROWS * 128 + MAX_ROWS + r) * f;
+						}
+						for (int i = 0; i < min(32, n - b); i++) {
+							const float fi = __shfl_sync(0xffffffffu, f, i);
+							sum += __shfl_sync(0xffffffffu, li, i);
+							if (fi != 0.0f) {
+								const float *src = at(b + i) + r * D + lane;
+#pragma unroll
+								for (int j = 0; j < D / 32; j++)
+									acc[j] = fmaf(__ldcg(src + 32 * j), fi, acc[j]);
+							}
+						}
+					}
+					const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+					float *dst = out_row(row0 + r) + lane;
+#pragma unroll
+					for (int j = 0; j < D / 32; j++)
+						dst[32 * j] = acc[j] * inv;
+				}
+				if (threadIdx.x == 0)
+					a.count[c0] = 0;  // at rest again
+			}
+		}
+		__syncthreads();  // shared memory is the next item's
+		u += unit1 - unit0;
+	}
+}
+
+template <int KIND, int D, int NB>
+int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
+{
+	attn_rows<KIND, D, NB><<<c->sm_count, THREADS, smem_bytes<KIND, D, NB>(), c->stream>>>(kv, st, a);
+	TIE_CUDA_LAUNCHED(c);
+	return TIE_CUDA_OK;
+}
+template <int KIND, int D, int NB>
+int allow_smem(tie_cuda_ctx *c)
+{
+	TIE_CUDA_TRY(c, cudaFuncSetAttribute(attn_rows<KIND, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<KIND, D, NB>()));
+	return TIE_CUDA_OK;
+}
+template <int KIND>
+int allow_smem_all(tie_cuda_ctx *c)
+{
+	int rc = allow_smem<KIND, 128, 1>(c);
+	rc = rc ? rc : allow_smem<KIND, 128, 2>(c);
+	rc = rc ? rc : allow_smem<KIND, 64, 1>(c);
+	return rc ? rc : allow_smem<KIND, 64, 2>(c);
+}
+template <int KIND>
+int go_kind(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int head_dim, bool two, const AttnArgs &a)
+{
+	if (head_dim == 128)
+		return two ? go<KIND, 128, 2>(c, kv, st, a) : go<KIND, 128, 1>(c, kv, st, a);
+	return two ? go<KIND, 64, 2>(c, kv, st, a) : go<KIND, 64, 1>(c, kv, st, a);
+}
+
+}  // namespace
+
+size_t attn_part_floats(const tie_cuda_ctx *c)
+{
+	return (size_t)2 * c->sm_count * PART_FLOATS;
+}
+
+int attn_setup(tie_cuda_ctx *c)
+{
+	int rc = allow_smem_all<TIE_CUDA_KV_F16>(c);
+	rc = rc ? rc : allow_smem_all<TIE_CUDA_KV_BF16>(c);
+	return rc ? rc : allow_smem_all<TIE_CUDA_KV_Q8>(c);
+}
+
+int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale)
+{
+	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * LOG2E, c->s.attn_part, c->s.attn_count};
+	const bool two = (long long)st.n_tokens * a.group > 8ll * st.n_seq;  // tiles of 16 rows where sequences have more than 8
+	if (kind == TIE_CUDA_KV_F16)
+		return go_kind<TIE_CUDA_KV_F16>(c, kv, st, head_dim, two, a);
+	if (kind == TIE_CUDA_KV_BF16)
+		return go_kind<TIE_CUDA_KV_BF16>(c, kv, st, head_dim, two, a);
+	return go_kind<TIE_CUDA_KV_Q8>(c, kv, st, head_dim, two, a);
+}
+
+}  // namespace tie

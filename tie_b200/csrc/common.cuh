@@ -30,6 +30,8 @@ class CopyPool;	 // copy_pool.h
 constexpr unsigned ST_BAD_EXPERT = 1u;	  // expert id outside this context's range
 constexpr unsigned ST_WAIT_TIMEOUT = 2u;  // a bounded mbarrier wait gave up
 constexpr unsigned ST_BAD_TILE = 4u;	  // tile bookkeeping out of range
+constexpr unsigned ST_BAD_PAGE = 8u;	  // a page table names a page that the cache does not have
+constexpr unsigned ST_BAD_STEP = 16u;	  // a step's token rows, lengths or trees are not what tie_cuda_kv_step says
 
 // Weight storage kinds on the device.
 //  Q4_K is kept byte-for-byte as in the GGUF (144-byte blocks are 16-byte aligned).
@@ -103,6 +105,9 @@ struct Scratch {
 	__half *hq = nullptr;  // [Rpad][xq_cols(F)]
 	unsigned *status = nullptr;		    // [1], the word in front of out
 	int *route_counter = nullptr;		    // [(T + 3) / 4] CTAs done per token tile of the batched router (zero at rest)
+	// attention over the cache (attn.cu): what CTAs that share a row tile leave for the last of them
+	float *attn_part = nullptr;		    // [2 x CTAs][AttnPart::FLOATS]
+	unsigned *attn_count = nullptr;		    // [CTAs] of them that are done (zero at rest)
 	unsigned *dec_sync = nullptr;		    // [2] arrivals and epoch of the one-kernel decode step's grid barriers
 	int *row_expert = nullptr;		    // [R] staging for expert_rows
 	// expert-parallel dispatch state (sort of this rank's rows over ALL experts)

@@ -70,6 +70,14 @@ bool tc_supported(const tie_cuda_ctx *c, const Layer &L);
 int launch_tc_gate_up(tie_cuda_ctx *c, const Layer &L, int n_tile);
 int launch_tc_down(tie_cuda_ctx *c, const Layer &L, int n_tile, float *y, bool sorted);
 int launch_tc_down_peer(tie_cuda_ctx *c, const Layer &L, const EpDst &dst);
+// kv_cache.cu, attn.cu (kind, out_type: TIE_CUDA_KV_*)
+struct KvView;
+struct StepView;
+int launch_qk_norm_rope(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const tie_cuda_attn_qkv &in);
+int launch_kv_read(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, void *k_out, void *v_out, int out_type);
+size_t attn_part_floats(const tie_cuda_ctx *c);
+int attn_setup(tie_cuda_ctx *c);
+int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale);
 // ep.cu
 int launch_ep_signal(tie_cuda_ctx *c, int which);
 int launch_ep_push_tokens(tie_cuda_ctx *c, const float *x, int n_tokens);

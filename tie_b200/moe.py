@@ -36,10 +36,11 @@ EXPORTS = [
     "tie_cuda_moe_ep_combine", "tie_cuda_route_noalloc", "tie_cuda_ep_region", "tie_cuda_ep_ipc_handle",
     "tie_cuda_ep_attach", "tie_cuda_ep_detach", "tie_cuda_ep_set_timeout_ms", "tie_cuda_ep_publish", "tie_cuda_ep_compute",
     "tie_cuda_ep_gather", "tie_cuda_moe_ffn_ep", "tie_cuda_mat_mat",
-    "tie_cuda_moe_block_inplace_ep",
+    "tie_cuda_moe_block_inplace_ep", "tie_cuda_qk_norm_rope", "tie_cuda_kv_read", "tie_cuda_attn",
 ]
 EP_HANDLE_BYTES = 64
 EP_PEER_POINTERS, EP_PEER_IPC_HANDLES = 0, 1
+KV_F32, KV_F16, KV_BF16, KV_Q8 = 0, 1, 2, 3  # types of a cache (F32: of rows read back only)
 PHASES = ["router", "sort", "split", "gate_up", "swiglu", "down", "combine"]  # swiglu: 0, gate_up makes it (tie_cuda_get_profile)
 
 
@@ -156,6 +157,12 @@ def load_library() -> ctypes.CDLL:
     L.tie_cuda_moe_block_inplace_ep.argtypes = [vp, i32, vp, i32, u32]
     L.tie_cuda_mat_mat.restype = i32
     L.tie_cuda_mat_mat.argtypes = [vp, vp, vp, vp, i32, i32, i32, u32]
+    L.tie_cuda_qk_norm_rope.restype = i32
+    L.tie_cuda_qk_norm_rope.argtypes = [vp, vp, vp, vp, u32]
+    L.tie_cuda_kv_read.restype = i32
+    L.tie_cuda_kv_read.argtypes = [vp, vp, vp, vp, vp, i32, u32]
+    L.tie_cuda_attn.restype = i32
+    L.tie_cuda_attn.argtypes = [vp, vp, vp, vp, i32, f32, vp, u32]
     _lib = L
     return L
 
@@ -179,6 +186,60 @@ def _ptr(a):
         assert a.is_contiguous()
         return a.data_ptr()
     raise TypeError(type(a))
+
+
+class KvCache(ctypes.Structure):
+    """tie_cuda_kv_cache over the caller's tensors: k, v [n_pages][n_head_kv][page_size][head_dim] of the type that `kind`
+    names (KV_Q8: int8, with fp32 k_scale, v_scale [n_pages][n_head_kv][page_size])."""
+    _fields_ = [
+        ("type", ctypes.c_int), ("n_head_kv", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
+        ("n_pages", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+    ]
+
+    def __init__(self, kind: int, k, v, k_scale=None, v_scale=None):
+        n_pages, n_head_kv, page_size, head_dim = k.shape
+        assert tuple(v.shape) == tuple(k.shape)
+        for x in (k_scale, v_scale):
+            assert x is None or tuple(x.shape) == tuple(k.shape[:3])
+        super().__init__(kind, n_head_kv, head_dim, page_size, n_pages, _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale))
+        self.keep = (k, v, k_scale, v_scale)
+
+
+class KvStep(ctypes.Structure):
+    """tie_cuda_kv_step over the caller's device tensors: tok_start [n_seq + 1], kv_len [n_seq], page_table [n_seq][max_pages]
+    and pos [n_tokens] int32, tree [n_tokens] 64-bit."""
+    _fields_ = [
+        ("n_seq", ctypes.c_int), ("n_tokens", ctypes.c_int), ("tok_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p), ("max_pages", ctypes.c_int), ("tree", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+    ]
+
+    def __init__(self, tok_start, kv_len, page_table, n_tokens: int, tree=None, pos=None):
+        n_seq, max_pages = page_table.shape
+        assert tok_start.shape[0] == n_seq + 1 and kv_len.shape[0] == n_seq
+        super().__init__(n_seq, n_tokens, _ptr(tok_start), _ptr(kv_len), _ptr(page_table), max_pages, _ptr(tree), _ptr(pos))
+        self.keep = (tok_start, kv_len, page_table, tree, pos)
+
+
+class AttnQkv(ctypes.Structure):
+    _fields_ = [
+        ("n_head", ctypes.c_int), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+        ("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p), ("norm_eps", ctypes.c_float),
+        ("rope_base", ctypes.c_float), ("rope_interleaved", ctypes.c_int), ("q_out", ctypes.c_void_p),
+    ]
+
+
+def _rows_ptr(a, width: int):
+    """Address and row stride (in elements) of a tensor of rows, each `width` contiguous elements; an int address has them one behind the other."""
+    if isinstance(a, int):
+        return a, width
+    inner = a.stride()[1:]
+    want = 1
+    for n, s in zip(reversed(a.shape[1:]), reversed(inner)):
+        assert n == 1 or s == want, "the values of a token's row must be contiguous"
+        want *= n
+    return a.data_ptr(), a.stride(0) if a.shape[0] > 1 else max(width, a.stride(0))
 
 
 class MoeBackend:
@@ -380,6 +441,24 @@ class MoeBackend:
     def moe_block_inplace_ep_ptr(self, layer_idx: int, hidden, n_tokens: int, flags: int = DEVICE):
         rc = self.L.tie_cuda_moe_block_inplace_ep(self.h, layer_idx, _ptr(hidden), n_tokens, flags)
         self._check(rc, "tie_cuda_moe_block_inplace_ep")
+
+    # -- attention over a paged cache (device tensors) --
+    def qk_norm_rope_ptr(self, cache: KvCache, step: KvStep, q, k, v, q_out, n_head: int, q_norm_w=None, k_norm_w=None,
+                         norm_eps: float = 1e-6, rope_base: float = 1e6, rope_interleaved: bool = False, flags: int = DEVICE):
+        """q, k, v: [n_tokens][..] rows, which may be slices of one array (the row stride is taken from the tensor)."""
+        kv_width = cache.n_head_kv * cache.head_dim
+        (qp, qs), (kp, ks), (vp, vs) = _rows_ptr(q, n_head * cache.head_dim), _rows_ptr(k, kv_width), _rows_ptr(v, kv_width)
+        qkv = AttnQkv(n_head, qp, kp, vp, qs, ks, vs, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, rope_base, int(rope_interleaved), _ptr(q_out))
+        rc = self.L.tie_cuda_qk_norm_rope(self.h, ctypes.byref(cache), ctypes.byref(step), ctypes.byref(qkv), flags)
+        self._check(rc, "tie_cuda_qk_norm_rope")
+
+    def kv_read_ptr(self, cache: KvCache, step: KvStep, k_out, v_out, out_type: int = KV_F32, flags: int = DEVICE):
+        rc = self.L.tie_cuda_kv_read(self.h, ctypes.byref(cache), ctypes.byref(step), _ptr(k_out), _ptr(v_out), out_type, flags)
+        self._check(rc, "tie_cuda_kv_read")
+
+    def attn_ptr(self, cache: KvCache, step: KvStep, q, out, n_head: int, scale: float, flags: int = DEVICE):
+        rc = self.L.tie_cuda_attn(self.h, ctypes.byref(cache), ctypes.byref(step), _ptr(q), n_head, scale, _ptr(out), flags)
+        self._check(rc, "tie_cuda_attn")
 
     # -- math_dispatch rows --
     def make_current(self):
