@@ -320,6 +320,30 @@ def test_attention_of_prompt_pieces(be, kind, toks, lens):
     w.check_attn(q, out, scale)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim, heads, kv_heads, toks, lens, drafted", [
+    (128, 32, 4, [512], [1500], False), (128, 16, 4, [2100], [100], False), (64, 32, 8, [2000], [0], False), (128, 32, 4, [13], [9001], True),
+    (128, 32, 4, [64, 40, 0, 64], [3500, 700, 5, 1201], True), (64, 24, 8, [64, 64], [128, 4000], True), (128, 24, 2, [700, 300], [64, 900], False),
+])
+def test_long_caches_and_many_rows(be, kind, dim, heads, kv_heads, toks, lens, drafted):
+    """Many tiles of keys a row and many tiles of rows a CTA, a head at a time on the device in 64 bits."""
+    tree = trees(np.random.default_rng(9), toks) if drafted else None
+    w = World(30, kind, toks, lens, heads, kv_heads, dim, 64, tree=tree)
+    q, out, scale = w.attn(be)
+    row = 0
+    for s, t in enumerate(toks):
+        if t == 0:
+            continue
+        k, v, m = (torch.tensor(x).cuda() for x in (w.sequence("k", s), w.sequence("v", s), w.sees(s, row)))
+        for h in range(heads):
+            x, kk, vv = q[row:row + t, h].double(), k[:, h // (heads // kv_heads)], v[:, h // (heads // kv_heads)]
+            want = torch.softmax((x @ kk.T * scale).masked_fill(~m, -math.inf), 1) @ vv
+            big = 1.0 + scale * (x.abs() @ kk.abs().T).max(1, keepdim=True).values
+            off = (out[row:row + t, h].double() - want).abs()
+            assert (off <= big * 2.0 ** -17 * vv.abs().max()).all(), (s, h, off.max())
+        row += t
+
+
 def test_many_sequences_of_all_lengths(be):
     rng = np.random.default_rng(1)
     toks = rng.integers(0, 3, 333).tolist()

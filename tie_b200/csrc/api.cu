@@ -85,7 +85,7 @@ int alloc_scratch(tie_cuda_ctx *c)
 	TRY(dev_alloc(c, &s.hq, s.rows_pad * XF));
 	TRY(dev_alloc(c, &s.route_counter, (T + 3) / 4));
 	TIE_CUDA_TRY(c, cudaMemset(s.route_counter, 0, (T + 3) / 4 * sizeof(int)));
-	TRY(dev_alloc(c, &s.attn_part, attn_part_floats(c)));
+	TRY(dev_alloc(c, &s.attn_part, attn_scratch_floats(c)));
 	TRY(dev_alloc(c, &s.attn_count, c->sm_count));
 	TIE_CUDA_TRY(c, cudaMemset(s.attn_count, 0, c->sm_count * sizeof(unsigned)));
 	TRY(dev_alloc(c, &s.dec_sync, 2));

@@ -6,8 +6,8 @@
 // token that sees nothing gets zeros.  One pass over keys and values with a running maximum and sum.
 #include <float.h>
 
+#include "attn.cuh"
 #include "kernels.cuh"
-#include "kv_cache.cuh"
 #include "mma_dot.cuh"
 #include "tc_ptx.cuh"
 
@@ -16,19 +16,9 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int GROUP = 16;	       // keys a warp takes at a time
-constexpr int UNIT = GROUP * WARPS;    // keys of one round of a CTA: what work is shared out in
+constexpr int UNIT = ATTN_UNIT;	       // one round of a CTA's warps
 constexpr int MAX_ROWS = 16;	       // query rows of a CTA's tile
-constexpr float P_SHIFT = 14.0f;       // p is held as p * 2^14: fp16 parts of it reach down to 2^-38 of the largest
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttnArgs {
-	const float *q;
-	float *out;
-	int n_head, group;  // group: query heads per key/value head
-	float scale_log2e;
-	float *part;
-	unsigned *count;
-};
+static_assert(UNIT == GROUP * WARPS, "a unit is a group of keys for each warp");
 
 template <int KIND, int D>
 struct Cfg {
@@ -44,16 +34,6 @@ struct Cfg {
 	}
 };
 
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool there)
-{
-	const int n = there ? 16 : 0;
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void *src, bool there)
-{
-	const int n = there ? 4 : 0;
-	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
 {
 	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -86,15 +66,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 		mma_16816(c, a[0], a[1], a[2], a[3], b0, b1);
 }
 
-// Two of the four signed bytes of x as halves, exactly: byte + 128 becomes the mantissa of 1024 + byte + 128.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t int8_pair(uint32_t x_biased)
-{
-	const uint32_t h = __byte_perm(x_biased, 0x64646464u, SEL);
-	const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&h), __half2half2(__ushort_as_half(0x6480)));  // 1152
-	return *reinterpret_cast<const uint32_t *>(&v);
-}
-
 // (a, b) as PARTS pairs of 16-bit parts, the largest first, that add up to them (to 22 bits in fp16, all 24 in bf16).
 template <int KIND, int PARTS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PARTS])
@@ -113,65 +84,6 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PA
 			b -= __half2float(h.y);
 		}
 	}
-}
-
-__device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exponent)
-{
-	return (w & exponent) == exponent || (w >> 16 & exponent) == exponent;
-}
-
-// The work of a launch: items = (sequence, key/value head, tile of query rows), each of as many units as its keys take;
-// CTA b of G does units [U b / G, U (b + 1) / G), whatever items these belong to.  An item within one CTA is finished there;
-// the CTAs that share one leave (maximum, sum, rows) behind, and the last to be done adds them up in the order of the
-// CTAs, so that the result does not depend on which was last.
-struct Work {
-	long long start[KV_MAX_SEQ + 1];  // units in front of a sequence
-	long long warp_sum[WARPS];
-	int last;
-};
-
-template <int NB>
-__device__ __forceinline__ long long seq_units(const KvView &kv, const AttnArgs &a, const SeqView &q)
-{
-	const long long tiles = ((long long)q.n_tok * a.group + 8 * NB - 1) / (8 * NB);
-	return tiles * kv.n_head_kv * (((long long)q.kv_len + q.n_tok + UNIT - 1) / UNIT);
-}
-
-template <int NB>
-__device__ void share_work(Work &w, const KvView &kv, const StepView &st, const AttnArgs &a)
-{
-	constexpr int PER = KV_MAX_SEQ / THREADS;
-	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	long long mine[PER], sum = 0;
-#pragma unroll
-	for (int i = 0; i < PER; i++) {
-		const int s = threadIdx.x * PER + i;
-		mine[i] = s < st.n_seq ? seq_units<NB>(kv, a, kv_sequence(st, kv.page_shift, s)) : 0;
-		sum += mine[i];
-	}
-	long long incl = sum;
-#pragma unroll
-	for (int o = 1; o < 32; o <<= 1) {
-		const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-		if (lane >= o)
-			incl += v;
-	}
-	if (lane == 31)
-		w.warp_sum[warp] = incl;
-	__syncthreads();
-	long long at = incl - sum;
-	for (int i = 0; i < warp; i++)
-		at += w.warp_sum[i];
-#pragma unroll
-	for (int i = 0; i < PER; i++) {
-		const int s = threadIdx.x * PER + i;
-		if (s <= st.n_seq)
-			w.start[s] = at;
-		at += mine[i];
-	}
-	if (threadIdx.x == THREADS - 1)
-		w.start[st.n_seq] = at;	 // (n_seq = KV_MAX_SEQ)
-	__syncthreads();
 }
 
 // One warp's state over the groups of keys it takes: S^T = K Q^T and O^T = V^T P^T on m16n8k16, keys (then dims) on the
@@ -356,7 +268,7 @@ struct Warp {
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
 				top = fmaxf(top, m[nb][i]);
-				base[i] = (top == -INFINITY ? 0.0f : top) - P_SHIFT;
+				base[i] = (top == -INFINITY ? 0.0f : top) - ATTN_P_SHIFT;
 				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2f(m[nb][i] - top);
 				m[nb][i] = top;
 			}
@@ -491,20 +403,17 @@ constexpr size_t smem_bytes()
 	return (stages > rows ? stages : rows) + 1024;
 }
 
-// floats that a CTA leaves for a shared item: rows, then per row maximum and sum
-constexpr int PART_FLOATS = MAX_ROWS * (128 + 2);
-
 template <int KIND, int D, int NB>
 __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const StepView st, const AttnArgs a)
 {
 	using C = Cfg<KIND, D>;
 	constexpr int ROWS = 8 * NB;
 	extern __shared__ uint8_t smem_raw[];
-	__shared__ Work work;
+	__shared__ AttnWork work;
 	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS];
 	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
-	share_work<NB>(work, kv, st, a);
+	attn_share_work<THREADS>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
 	const long long total = work.start[st.n_seq];
 	const int n_cta = (int)min((long long)gridDim.x, total);  // (each of them has a unit at least)
 	if (cta >= n_cta)
@@ -513,17 +422,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 	const uint32_t stages = ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE;
 	Warp<KIND, D, NB> w;
 	for (long long u = u_begin; u < u_end;) {
-		int lo = 0, hi = st.n_seq - 1;	// the sequence of unit u: the last that starts at or in front of it and has any
-		while (lo < hi) {
-			const int mid = (lo + hi + 1) >> 1;
-			if (work.start[mid] <= u)
-				lo = mid;
-			else
-				hi = mid - 1;
-		}
-		const int s = lo;
+		const int s = attn_sequence_of(work, st.n_seq, u);
 		const SeqView seq = kv_sequence(st, kv.page_shift, s);
-		const int n_keys = seq.kv_len + seq.n_tok, item_units = (n_keys + UNIT - 1) / UNIT;
+		const int n_keys = seq.kv_len + seq.n_tok, item_units = attn_units(seq);
 		const int tiles = (seq.n_tok * a.group + ROWS - 1) / ROWS;
 		const long long in_seq = u - work.start[s], item = in_seq / item_units;
 		const int unit0 = (int)(in_seq - item * item_units);
@@ -626,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			const int tok = r / a.group;
 			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + head * a.group + (r - tok * a.group)) * D;
 		};
-		float *part = a.part + (size_t)(2 * cta + (unit0 == 0 ? 1 : 0)) * PART_FLOATS;
+		float *part = a.part + (2 * cta + (unit0 == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS);
 		for (int i = threadIdx.x; i < ROWS * D / 4; i += THREADS) {
 			const int r = i / (D / 4), col = i % (D / 4) * 4;
 			float4 sum = make_float4(0, 0, 0, 0);
@@ -656,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			}
 			// the CTAs of the item: those of its first and last unit, and all between
 			const long long i0 = work.start[s] + item * item_units, i1 = i0 + item_units - 1;
-			const int c0 = (int)(((i0 + 1) * n_cta - 1) / total), c1 = (int)(((i1 + 1) * n_cta - 1) / total);
+			const int c0 = attn_cta_of(i0, total, n_cta), c1 = attn_cta_of(i1, total, n_cta);
 			__threadfence();
 			__syncthreads();
 			if (threadIdx.x == 0)
@@ -664,45 +565,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			__syncthreads();
 			if (work.last) {
 				__threadfence();
-				const float *first = a.part + (size_t)(2 * c0 + 1) * PART_FLOATS;
-				const float *others = a.part + (size_t)2 * (c0 + 1) * PART_FLOATS;  // + 2 i PART_FLOATS
-				auto at = [&](int i) { return i == 0 ? first : others + (size_t)2 * (i - 1) * PART_FLOATS; };
-				const int n = c1 - c0 + 1;
-				for (int r = warp; r < ROWS && row0 + r < n_rows; r += WARPS) {
-					float top = -INFINITY, sum = 0.0f;
-					for (int i = lane; i < n; i += 32)
-						top = fmaxf(top, __ldcg(at(i) + MAX_ROWS * 128 + r));
-#pragma unroll
-					for (int o = 16; o; o >>= 1)
-						top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-					float acc[D / 32];
-#pragma unroll
-					for (int j = 0; j < D / 32; j++)
-						acc[j] = 0.0f;
-					for (int b = 0; b < n; b += 32) {
-						float f = 0.0f, li = 0.0f;
-						if (b + lane < n) {
-							const float mi = __ldcg(at(b + lane) + MAX_ROWS * 128 + r);
-							f = mi == -INFINITY ? 0.0f : exp2f(mi - top);
-							li = __ldcg(at(b + lane) + MAX_ROWS * 128 + MAX_ROWS + r) * f;
-						}
-						for (int i = 0; i < min(32, n - b); i++) {
-							const float fi = __shfl_sync(0xffffffffu, f, i);
-							sum += __shfl_sync(0xffffffffu, li, i);
-							if (fi != 0.0f) {
-								const float *src = at(b + i) + r * D + lane;
-#pragma unroll
-								for (int j = 0; j < D / 32; j++)
-									acc[j] = fmaf(__ldcg(src + 32 * j), fi, acc[j]);
-							}
-						}
-					}
-					const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-					float *dst = out_row(row0 + r) + lane;
-#pragma unroll
-					for (int j = 0; j < D / 32; j++)
-						dst[32 * j] = acc[j] * inv;
-				}
+				for (int r = warp; r < ROWS && row0 + r < n_rows; r += WARPS)
+					attn_join_row<D, MAX_ROWS>(a.part, c0, c1, r, lane, out_row(row0 + r));
 				if (threadIdx.x == 0)
 					a.count[c0] = 0;  // at rest again
 			}
@@ -743,22 +607,27 @@ int go_kind(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int head_dim,
 
 }  // namespace
 
-size_t attn_part_floats(const tie_cuda_ctx *c)
+size_t attn_scratch_floats(const tie_cuda_ctx *c)
 {
-	return (size_t)2 * c->sm_count * PART_FLOATS;
+	return 2 * c->sm_count * attn_part_floats(ATTN_MAX_ROWS);
 }
 
 int attn_setup(tie_cuda_ctx *c)
 {
 	int rc = allow_smem_all<TIE_CUDA_KV_F16>(c);
 	rc = rc ? rc : allow_smem_all<TIE_CUDA_KV_BF16>(c);
-	return rc ? rc : allow_smem_all<TIE_CUDA_KV_Q8>(c);
+	rc = rc ? rc : allow_smem_all<TIE_CUDA_KV_Q8>(c);
+	return rc ? rc : attn_tc_setup(c);
 }
 
 int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale)
 {
-	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * LOG2E, c->s.attn_part, c->s.attn_count};
-	const bool two = (long long)st.n_tokens * a.group > 8ll * st.n_seq;  // tiles of 16 rows where sequences have more than 8
+	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * ATTN_LOG2E, c->s.attn_part, c->s.attn_count};
+	// rows of a sequence and key/value head, on average: up to 8 and up to 16 in tiles of that, more in tiles of 128
+	const long long rows = ((long long)st.n_tokens * a.group + st.n_seq - 1) / st.n_seq;
+	if (rows > 16)
+		return launch_attn_tc(c, kv, st, kind, head_dim, a);
+	const bool two = rows > 8;
 	if (kind == TIE_CUDA_KV_F16)
 		return go_kind<TIE_CUDA_KV_F16>(c, kv, st, head_dim, two, a);
 	if (kind == TIE_CUDA_KV_BF16)

@@ -1,0 +1,182 @@
+// What the two attention kernels (attn.cu, attn_tc.cu) share: their arguments, and how work is shared out among CTAs.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace tie {
+
+constexpr float ATTN_P_SHIFT = 14.0f;  // p is held as p * 2^14: fp16 parts of it reach down to 2^-38 of the largest
+constexpr float ATTN_LOG2E = 1.4426950408889634f;
+constexpr int ATTN_UNIT = 128;	       // keys: what an item's work is counted in
+constexpr int ATTN_MAX_ROWS = 128;     // query rows of a tile, at most
+
+struct AttnArgs {
+	const float *q;
+	float *out;
+	int n_head, group;  // group: query heads per key/value head
+	float scale_log2e;
+	float *part;
+	unsigned *count;
+};
+
+// What a CTA leaves for a shared item of ROWS rows: [row][D] sums, then [row] maxima, then [row] sums of p.
+__host__ __device__ constexpr size_t attn_part_floats(int rows)
+{
+	return (size_t)rows * (128 + 2);
+}
+
+// The work of a launch: items = (sequence, key/value head, tile of query rows), each of as many units as its keys take;
+// CTA b of G does units [U b / G, U (b + 1) / G), whatever items these belong to.  An item within one CTA is finished there;
+// the CTAs that share one leave (maximum, sum, rows) behind, and the last to be done adds them up in the order of the
+// CTAs, so that the result does not depend on which was last.
+struct AttnWork {
+	long long start[KV_MAX_SEQ + 1];  // units (or items) in front of a sequence
+	long long warp_sum[16];
+	int last;
+};
+
+__device__ __forceinline__ long long attn_items(const KvView &kv, const AttnArgs &a, const SeqView &q, int rows)
+{
+	return ((long long)q.n_tok * a.group + rows - 1) / rows * kv.n_head_kv;
+}
+__device__ __forceinline__ int attn_units(const SeqView &q)
+{
+	return (q.kv_len + q.n_tok + ATTN_UNIT - 1) / ATTN_UNIT;
+}
+
+// Fills w.start with the running sums of `of(sequence)`, by all threads of the CTA.
+template <int THREADS, class F>
+__device__ __forceinline__ void attn_share_work(AttnWork &w, const KvView &kv, const StepView &st, F of)
+{
+	constexpr int PER = KV_MAX_SEQ / THREADS;
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	if (st.n_seq == 1) {
+		if (threadIdx.x == 0) {
+			w.start[0] = 0;
+			w.start[1] = of(kv_sequence(st, kv.page_shift, 0));
+		}
+		__syncthreads();
+		return;
+	}
+	long long mine[PER], sum = 0;
+#pragma unroll
+	for (int i = 0; i < PER; i++) {
+		const int s = threadIdx.x * PER + i;
+		mine[i] = s < st.n_seq ? of(kv_sequence(st, kv.page_shift, s)) : 0;
+		sum += mine[i];
+	}
+	long long incl = sum;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1) {
+		const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+		if (lane >= o)
+			incl += v;
+	}
+	if (lane == 31)
+		w.warp_sum[warp] = incl;
+	__syncthreads();
+	long long at = incl - sum;
+	for (int i = 0; i < warp; i++)
+		at += w.warp_sum[i];
+#pragma unroll
+	for (int i = 0; i < PER; i++) {
+		const int s = threadIdx.x * PER + i;
+		if (s <= st.n_seq)
+			w.start[s] = at;
+		at += mine[i];
+	}
+	if (threadIdx.x == THREADS - 1 && st.n_seq == KV_MAX_SEQ)
+		w.start[st.n_seq] = at;
+	__syncthreads();
+}
+
+// The sequence of unit (or item) u: the last that starts at or in front of it.
+__device__ __forceinline__ int attn_sequence_of(const AttnWork &w, int n_seq, long long u)
+{
+	int lo = 0, hi = n_seq - 1;
+	while (lo < hi) {
+		const int mid = (lo + hi + 1) >> 1;
+		if (w.start[mid] <= u)
+			lo = mid;
+		else
+			hi = mid - 1;
+	}
+	return lo;
+}
+
+// The CTA that has unit u of `total`.
+__device__ __forceinline__ int attn_cta_of(long long u, long long total, int n_cta)
+{
+	return (int)(((u + 1) * n_cta - 1) / total);
+}
+
+// Row r of what the CTAs c0 .. c1 left of an item, joined by a warp: lane l gets values l, l + 32 .. of the finished row.
+template <int D, int ROWS>
+__device__ __forceinline__ void attn_join_row(const float *parts, int c0, int c1, int r, int lane, float *dst)
+{
+	constexpr size_t PART = attn_part_floats(ROWS);
+	auto at = [&](int i) { return parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART; };
+	const int n = c1 - c0 + 1;
+	float top = -INFINITY, sum = 0.0f;
+	for (int i = lane; i < n; i += 32)
+		top = fmaxf(top, __ldcg(at(i) + ROWS * 128 + r));
+#pragma unroll
+	for (int o = 16; o; o >>= 1)
+		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+	float acc[D / 32];
+#pragma unroll
+	for (int j = 0; j < D / 32; j++)
+		acc[j] = 0.0f;
+	for (int b = 0; b < n; b += 32) {
+		float f = 0.0f, li = 0.0f;
+		if (b + lane < n) {
+			const float mi = __ldcg(at(b + lane) + ROWS * 128 + r);
+			f = mi == -INFINITY ? 0.0f : exp2f(mi - top);
+			li = __ldcg(at(b + lane) + ROWS * 128 + ROWS + r) * f;
+		}
+		for (int i = 0; i < min(32, n - b); i++) {
+			const float fi = __shfl_sync(0xffffffffu, f, i);
+			sum += __shfl_sync(0xffffffffu, li, i);
+			if (fi != 0.0f) {
+				const float *src = at(b + i) + r * D + lane;
+#pragma unroll
+				for (int j = 0; j < D / 32; j++)
+					acc[j] = fmaf(__ldcg(src + 32 * j), fi, acc[j]);
+			}
+		}
+	}
+	const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+	for (int j = 0; j < D / 32; j++)
+		dst[lane + 32 * j] = acc[j] * inv;
+}
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool there)
+{
+	const int n = there ? 16 : 0;
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void *src, bool there)
+{
+	const int n = there ? 4 : 0;
+	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exponent)
+{
+	return (w & exponent) == exponent || (w >> 16 & exponent) == exponent;
+}
+// Two of the four signed bytes of a word whose bytes were XORed with 0x80 as halves, exactly: byte + 128 becomes the
+// mantissa of 1024 + byte + 128.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t int8_pair(uint32_t x_biased)
+{
+	const uint32_t h = __byte_perm(x_biased, 0x64646464u, SEL);
+	const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&h), __half2half2(__ushort_as_half(0x6480)));  // 1152
+	return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// attn_tc.cu: tiles of 128 rows on tcgen05
+int attn_tc_setup(tie_cuda_ctx *c);
+int launch_attn_tc(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const AttnArgs &a);
+
+}  // namespace tie

@@ -106,7 +106,7 @@ struct Scratch {
 	unsigned *status = nullptr;		    // [1], the word in front of out
 	int *route_counter = nullptr;		    // [(T + 3) / 4] CTAs done per token tile of the batched router (zero at rest)
 	// attention over the cache (attn.cu): what CTAs that share a row tile leave for the last of them
-	float *attn_part = nullptr;		    // [2 x CTAs][AttnPart::FLOATS]
+	float *attn_part = nullptr;		    // [2 x CTAs][attn_part_floats]
 	unsigned *attn_count = nullptr;		    // [CTAs] of them that are done (zero at rest)
 	unsigned *dec_sync = nullptr;		    // [2] arrivals and epoch of the one-kernel decode step's grid barriers
 	int *row_expert = nullptr;		    // [R] staging for expert_rows

@@ -75,7 +75,7 @@ struct KvView;
 struct StepView;
 int launch_qk_norm_rope(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const tie_cuda_attn_qkv &in);
 int launch_kv_read(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, void *k_out, void *v_out, int out_type);
-size_t attn_part_floats(const tie_cuda_ctx *c);
+size_t attn_scratch_floats(const tie_cuda_ctx *c);
 int attn_setup(tie_cuda_ctx *c);
 int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale);
 // ep.cu
