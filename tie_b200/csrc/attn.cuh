@@ -134,6 +134,7 @@ __device__ __forceinline__ void attn_join_row(const float *parts, int c0, int c1
 			f = mi == -INFINITY ? 0.0f : exp2f(mi - top);
 			li = __ldcg(at(b + lane) + ROWS * 128 + ROWS + r) * f;
 		}
+#pragma unroll 8
 		for (int i = 0; i < min(32, n - b); i++) {
 			const float fi = __shfl_sync(0xffffffffu, f, i);
 			sum += __shfl_sync(0xffffffffu, li, i);

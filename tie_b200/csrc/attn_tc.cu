@@ -13,7 +13,7 @@
 //     output row of its own (joined at the end), so that one's exponentials run under the other's MMAs;
 //   * two warps load keys, two values: cp.async into the swizzled operand layout (pages of 16 slots and more, zeros behind
 //     the last key), expanded to fp16 in place where the cache has another type;
-//   * one thread issues the MMAs.  Q and P are operands in tensor memory (a step of shared memory then feeds only the 128
+//   * one thread finds the CTA's pieces of work, one issues the MMAs.  Q and P are operands in tensor memory (a step of shared memory then feeds only the 128
 //     keys or dims of its other operand: half of what the memory delivers); P's parts of 16 keys take the columns of these keys' scores.
 // Tensor memory: Q 128 columns, two score tiles, O: all 512.  Every wait is bounded, as in tensor.cu; after a
 // time-out no wait waits any more and all roles run to their ends.
@@ -28,14 +28,27 @@ namespace {
 
 constexpr int ROWS = ATTN_MAX_ROWS, TILE = ATTN_UNIT;
 constexpr int THREADS = 512, SOFT_THREADS = 256, LOAD_THREADS = 64;
-constexpr int W_KEYS = 8, W_VALUES = 10, W_MMA = 12;  // first warps of the roles behind the softmax warps
+constexpr int W_KEYS = 8, W_VALUES = 10, W_MMA = 12, W_PIECES = 13;  // first warps of the roles behind the softmax warps
+constexpr int PIECE_READERS = 13;  // the warps of those who work on them
 constexpr int SOFT_REGS = 192, LOAD_REGS = 80, MMA_REGS = 48;
 static_assert(2 * SOFT_REGS + LOAD_REGS + MMA_REGS <= 512, "a launch of 512 threads holds 128 registers a thread");
 constexpr int COL_Q = 0, COL_S = 128, COL_O = 384;
 constexpr uint32_t PANEL = TILE * 128;	// bytes of 64 dims of a tile: 128 rows of 128 bytes
 constexpr long long WAIT_CYCLES = 1ll << 30;
 
+// A piece of work of a CTA: an item, or (few items: shared) some units of one.  No more of them: s < 0.
+struct Piece {
+	SeqView seq;
+	int s, head, row0;
+	int unit0, unit1, item_units;
+	int n_tiles;	// from unit0 on: tiles that some row of the item sees keys of
+	int key_end;	// first key that nobody sees
+	int all_see;	// keys in front of this one are seen by every row
+};
+constexpr int PIECES = 4;
 struct Shared {
+	uint64_t piece_full[PIECES], piece_free[PIECES];
+	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
 	uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
 	uint64_t s_full[2], p_full[2], o_full[2], o_free, q_full, fin;  // (o_full: a warpgroup's own, so that it waits for every phase)
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
@@ -52,15 +65,6 @@ struct Shared {
 	float2 ml[2][ROWS];
 };
 
-// The n-th piece of work of this CTA: an item, or (few items: shared) some units of one.
-struct Piece {
-	SeqView seq;
-	int s, head, row0;
-	int unit0, unit1, item_units;
-	int n_tiles;	// from unit0 on: tiles that some row of the item sees keys of
-	int key_end;	// first key that nobody sees
-	int all_see;	// keys in front of this one are seen by every row
-};
 struct Walk {
 	bool shared;
 	long long total, u, u_end;
@@ -75,7 +79,7 @@ __device__ __forceinline__ void finish_piece(Piece &p, const StepView &st, const
 	p.n_tiles = max(0, min(p.unit1, (p.key_end + TILE - 1) / TILE) - p.unit0);
 }
 
-__device__ bool next_piece(Walk &w, Piece &p, const AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a)
+__device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
 	if (w.shared) {
 		if (w.u >= w.u_end)
@@ -110,6 +114,28 @@ __device__ bool next_piece(Walk &w, Piece &p, const AttnWork &work, const KvView
 	}
 	finish_piece(p, st, a);
 	return true;
+}
+
+// Whole items where each CTA has several, else their units shared out evenly.
+template <int N>
+__device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a, int n_cta, int cta)
+{
+	Walk w = {};
+	attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS); });
+	w.total = work.start[st.n_seq];
+	w.n_cta = n_cta;
+	w.shared = w.total < 3ll * n_cta;
+	if (w.shared) {
+		__syncthreads();
+		attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
+		w.total = work.start[st.n_seq];
+		w.n_cta = (int)min((long long)n_cta, w.total);
+		if (cta < w.n_cta) {
+			w.u = w.total * cta / w.n_cta;
+			w.u_end = w.total * (cta + 1) / w.n_cta;
+		}
+	}
+	return w;
 }
 
 template <int KIND, int D>
@@ -147,16 +173,17 @@ __device__ __forceinline__ void bar_sync()
 struct Waiter {
 	volatile uint32_t *abort;
 	unsigned *status;
-	__device__ __forceinline__ bool operator()(uint64_t &bar, uint32_t parity) const
+	// always: also after another wait has given up (the pieces go on: whoever reads them does not wait for anything else then)
+	__device__ __forceinline__ bool operator()(uint64_t &bar, uint32_t parity, bool always = false) const
 	{
 		const uint32_t b = ptx::smem_u32(&bar);
 		if (ptx::mbar_try_wait(b, parity))
 			return true;
 		const long long t0 = clock64();
 		while (!ptx::mbar_try_wait_suspend(b, parity, 20000u)) {
-			if (*abort)
+			if (!always && *abort)
 				return false;
-			if (clock64() - t0 > WAIT_CYCLES) {
+			if (clock64() - t0 > (always ? 4 * WAIT_CYCLES : WAIT_CYCLES)) {
 				atomicOr(status, ST_WAIT_TIMEOUT);
 				*abort = 1;
 				return false;
@@ -166,14 +193,78 @@ struct Waiter {
 	}
 };
 
-// fp16 hi and lo of a pair
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo)
+// The n-th piece of work, for a warp (or the issuing thread): taken, and given back.
+__device__ __forceinline__ Piece take_piece(Shared *sh, const Waiter &wait, uint32_t n)
 {
-	const __half2 h = __floats2half2_rn(a, b);
-	const float2 f = __half22float2(h);
-	const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+	wait(sh->piece_full[n % PIECES], n / PIECES & 1u, true);
+	return sh->piece[n % PIECES];
+}
+__device__ __forceinline__ void drop_piece(Shared *sh, uint32_t n, int lane)
+{
+	__syncwarp();
+	if (lane == 0)
+		ptx::mbar_arrive(ptx::smem_u32(&sh->piece_free[n % PIECES]));
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+	return r;
+}
+// 2^x to 2^-22, results below 2^-126 zero
+__device__ __forceinline__ float exp2_ftz(float x)
+{
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+
+// fp16 hi and lo of a pair
+__device__ __forceinline__ void split2(float2 x, uint32_t &hi, uint32_t &lo)
+{
+	const __half2 h = __floats2half2_rn(x.x, x.y);
+	const float2 f = __half22float2(h), d = add2(x, make_float2(-f.x, -f.y));
+	const __half2 l = __floats2half2_rn(d.x, d.y);
 	hi = *reinterpret_cast<const uint32_t *>(&h);
 	lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Larger magnitudes of two pairs of bf16 (NaN where there is one)
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b)
+{
+	const __nv_bfloat162 r = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&b)));
+	return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t half2_of_bf16x2(uint32_t w, float f)
+{
+	const float2 x = mul2(make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), make_float2(f, f));
+	const __half2 h = __floats2half2_rn(x.x, x.y);
+	return *reinterpret_cast<const uint32_t *>(&h);
+}
+// All ones over those of a pair that are numbers.
+__device__ __forceinline__ uint32_t finite16(uint32_t w, uint32_t exponent)
+{
+	return ((w & exponent) == exponent ? 0u : 0xffffu) | ((w >> 16 & exponent) == exponent ? 0u : 0xffff0000u);
 }
 
 // The loading warps of keys (VALUES false) or values: 64 threads.
@@ -255,46 +346,61 @@ struct Loader {
 			}
 		} else {
 			constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
-			if (KIND == TIE_CUDA_KV_BF16 || (VALUES && masked)) {
-#pragma unroll 4
+			if (VALUES && masked) {
+#pragma unroll 1
 				for (int i = 0; i < PASSES; i++) {
-					const int r = r0 + i * AT_ONCE;
-					const uint4 v = lds128(at + T::raw(r, ch));
+					const uint32_t to = at + T::place(r0 + i * AT_ONCE, ch);
+					const uint4 v = lds128(to);
 					uint32_t w[4] = {v.x, v.y, v.z, v.w};
-					bool change = KIND == TIE_CUDA_KV_BF16;
-					if (VALUES && masked) {
+					bool change = false;
 #pragma unroll
-						for (int j = 0; j < 4; j++)
-							if (nonfinite16(w[j], EXPONENT)) {  // (its products are made by the rows that see it)
-								w[j] &= ((w[j] & EXPONENT) == EXPONENT ? 0u : 0xffffu) | ((w[j] >> 16 & EXPONENT) == EXPONENT ? 0u : 0xffff0000u);
-								odd = change = true;
-							}
-					}
-					if constexpr (KIND == TIE_CUDA_KV_BF16) {
-						uint32_t top = 0;  // largest magnitudes of even and odd values, infinities and NaN left out
-#pragma unroll
-						for (int j = 0; j < 4; j++) {
-							uint32_t m = w[j] & 0x7fff7fffu;
-							if (nonfinite16(w[j], EXPONENT))
-								m &= ((m & EXPONENT) == EXPONENT ? 0u : 0xffffu) | ((m >> 16 & EXPONENT) == EXPONENT ? 0u : 0xffff0000u);
-							top = __vmaxu2(top, m);
+					for (int j = 0; j < 4; j++)
+						if (nonfinite16(w[j], EXPONENT)) {  // (its products are made by the rows that see it)
+							w[j] &= finite16(w[j], EXPONENT);
+							odd = change = true;
 						}
+					if (change)
+						sts128(to, make_uint4(w[0], w[1], w[2], w[3]));
+				}
+			}
+			if constexpr (KIND == TIE_CUDA_KV_BF16) {
+				// a row's largest to 2^14 .. 2^15: its 8 bits are exact down to 2^-32 of it
+				constexpr int B = 8;  // rows at once, for their latencies
+#pragma unroll 1
+				for (int i0 = 0; i0 < PASSES; i0 += B) {
+					uint4 v[B];
+					uint32_t top[B];
 #pragma unroll
-						for (int o = T::CHUNKS / 2; o; o >>= 1)
-							top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-						// the largest to 2^14 .. 2^15: 8 bits are exact down to 2^-32 of it
-						const int e = max((int)(max(top & 0xffffu, top >> 16) >> 7), 15);
+					for (int i = 0; i < B; i++) {
+						v[i] = lds128(at + T::place(r0 + (i0 + i) * AT_ONCE, ch));
+						top[i] = max_bf16x2(max_bf16x2(v[i].x, v[i].y), max_bf16x2(v[i].z, v[i].w));
+					}
+#pragma unroll
+					for (int o = T::CHUNKS / 2; o; o >>= 1)
+#pragma unroll
+						for (int i = 0; i < B; i++)
+							top[i] = max_bf16x2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+					for (int i = 0; i < B; i++) {
+						const int r = r0 + (i0 + i) * AT_ONCE;
+						uint32_t largest = max(top[i] & 0x7fffu, top[i] >> 16 & 0x7fffu);
+						if (__any_sync(0xffffffffu, largest >= EXPONENT)) {  // the largest among the numbers, where some are none
+							const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+							largest = 0;
+							for (int j = 0; j < 4; j++) {
+								const uint32_t f = w[j] & 0x7fff7fffu & finite16(w[j], EXPONENT);
+								largest = max(largest, max(f & 0xffffu, f >> 16));
+							}
+							for (int o = T::CHUNKS / 2; o; o >>= 1)
+								largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+						}
+						const int e = max((int)(largest >> 7), 15);
 						const float f = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
 						if (ch == 0)
 							scale[r] = __uint_as_float((uint32_t)(127 - 141 + e) << 23);
-#pragma unroll
-						for (int j = 0; j < 4; j++) {
-							const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
-							w[j] = *reinterpret_cast<const uint32_t *>(&h);
-						}
+						sts128(at + T::place(r, ch), make_uint4(half2_of_bf16x2(v[i].x, f), half2_of_bf16x2(v[i].y, f), half2_of_bf16x2(v[i].z, f),
+											half2_of_bf16x2(v[i].w, f)));
 					}
-					if (change)
-						sts128(at + T::place(r, ch), make_uint4(w[0], w[1], w[2], w[3]));
 				}
 			}
 		}
@@ -333,15 +439,14 @@ struct Loader {
 		ptx::mbar_arrive(ptx::smem_u32(VALUES ? &sh->v_full[slot] : &sh->k_full[slot]));
 	}
 
-	__device__ __forceinline__ void run(Walk w, const AttnWork &work, const AttnArgs &a, const Waiter &wait)
+	__device__ __forceinline__ void run(const Waiter &wait)
 	{
 		uint64_t *free_bar = VALUES ? sh->v_free : sh->k_free;
-		Walk wp = w;
 		Piece p, q;  // of the tile to be finished next, and of the one to be requested next
 		int pi = 0, qi = 0;
-		uint32_t asked = 0, done = 0;
-		bool more = advance_to_tile(w, q, work, a);
-		advance_to_tile(wp, p, work, a);
+		uint32_t asked = 0, done = 0, pn = 0, qn = 0;
+		bool more = next_with_tiles(q, qn, wait, false);
+		next_with_tiles(p, pn, wait, true);
 		while (done < asked || more) {
 			// the next request goes out as soon as its slot is free; until then what has come in is made ready
 			bool can = more && asked - done < 2;
@@ -357,7 +462,8 @@ struct Loader {
 				asked++;
 				if (++qi == q.n_tiles) {
 					qi = 0;
-					more = advance_to_tile(w, q, work, a);
+					qn++;
+					more = next_with_tiles(q, qn, wait, false);
 				}
 				if (asked - done < 2 && more)
 					continue;
@@ -370,17 +476,23 @@ struct Loader {
 			done++;
 			if (++pi == p.n_tiles) {
 				pi = 0;
-				advance_to_tile(wp, p, work, a);
+				drop_piece(sh, pn++, lane);
+				next_with_tiles(p, pn, wait, true);
 			}
 		}
 	}
-	__device__ __forceinline__ bool advance_to_tile(Walk &w, Piece &p, const AttnWork &work, const AttnArgs &a)
+	// Piece n, or the next behind it that has tiles; drop: gives those without back.
+	__device__ __forceinline__ bool next_with_tiles(Piece &p, uint32_t &n, const Waiter &wait, bool drop)
 	{
-		do {
-			if (!next_piece(w, p, work, kv, st, a))
+		for (;; n++) {
+			p = take_piece(sh, wait, n);
+			if (p.s < 0)
 				return false;
-		} while (p.n_tiles == 0);
-		return true;
+			if (p.n_tiles > 0)
+				return true;
+			if (drop)
+				drop_piece(sh, n, lane);
+		}
 	}
 };
 
@@ -408,6 +520,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		}
 		for (int i = 0; i < 4; i++)
 			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), LOAD_THREADS);
+		for (int i = 0; i < PIECES; i++) {
+			ptx::mbar_init(ptx::smem_u32(&sh->piece_full[i]), 1);
+			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), PIECE_READERS);
+		}
 		ptx::mbar_init(ptx::smem_u32(&sh->o_free), SOFT_THREADS / 2);
 		ptx::mbar_init(ptx::smem_u32(&sh->q_full), SOFT_THREADS);
 		ptx::mbar_init(ptx::smem_u32(&sh->fin), 1);
@@ -419,22 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		ptx::tmem_alloc(ptx::smem_u32(&sh->tmem_base), 512);
 		ptx::tmem_relinquish();
 	}
-	// whole items where each CTA has several, else their units shared out evenly
-	Walk walk = {};
-	attn_share_work<THREADS>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS); });
-	walk.total = work.start[st.n_seq];
-	walk.n_cta = gridDim.x;
-	walk.shared = walk.total < 3ll * gridDim.x;
-	if (walk.shared) {
-		__syncthreads();
-		attn_share_work<THREADS>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
-		walk.total = work.start[st.n_seq];
-		walk.n_cta = (int)min((long long)gridDim.x, walk.total);
-		if ((int)blockIdx.x < walk.n_cta) {
-			walk.u = walk.total * blockIdx.x / walk.n_cta;
-			walk.u_end = walk.total * (blockIdx.x + 1) / walk.n_cta;
-		}
-	}
+	const Walk walk = start_walk<THREADS>(work, kv, st, a, gridDim.x, blockIdx.x);
 	ptx::tc_fence_before();
 	__syncthreads();
 	ptx::tc_fence_after();
@@ -448,7 +549,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
 		uint32_t tiles = 0;
 		Piece p;
-		while (next_piece(walk, p, work, kv, st, a)) {
+		for (uint32_t n = 0;; n++) {
+			p = take_piece(sh, wait, n);
+			drop_piece(sh, n, lane);
+			if (p.s < 0)
+				break;
 			const int n_rows = p.seq.n_tok * a.group, row = p.row0 + r;
 			const bool there = row < n_rows;
 			const int tok = there ? row / a.group : p.seq.n_tok - 1;
@@ -476,8 +581,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 #pragma unroll
 					for (int i = 0; i < 8; i++) {
 						const float4 x = v[8 * c + i];
-						split2(x.x * down, x.y * down, hi[2 * i], lo[2 * i]);
-						split2(x.z * down, x.w * down, hi[2 * i + 1], lo[2 * i + 1]);
+						split2(make_float2(x.x * down, x.y * down), hi[2 * i], lo[2 * i]);
+						split2(make_float2(x.z * down, x.w * down), hi[2 * i + 1], lo[2 * i + 1]);
 					}
 					ptx::tmem_st16(lanes + COL_Q + wg * (HALF / 2) + 16 * c, hi);
 					ptx::tmem_st16(lanes + COL_Q + HALF + wg * (HALF / 2) + 16 * c, lo);
@@ -495,10 +600,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					kv_report(st, ST_BAD_STEP);
 			}
 			const int sees_to = p.seq.kv_len + tok + 1;  // no tree
-			float acc[D], m = -INFINITY, l = 0.0f;
+			float2 acc[HALF];
+			float m = -INFINITY, l = 0.0f;
 #pragma unroll
-			for (int i = 0; i < D; i++)
-				acc[i] = 0.0f;
+			for (int i = 0; i < HALF; i++)
+				acc[i] = make_float2(0.0f, 0.0f);
 			for (int i = 0; i < p.n_tiles; i++, tiles++) {
 				if ((int)(tiles & 1) != wg)
 					continue;
@@ -508,62 +614,61 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				wait(sh->f_full[fslot], (tiles >> 2) & 1u);
 				wait(sh->s_full[wg], ph);
 				ptx::tc_fence_after();
-				// the keys of each 32 that this row sees
-				uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
 				const uint32_t bad = sh->bad[fslot];
 				const bool masked = key0 + TILE > p.all_see || bad != 0;
-				if (masked) {
-#pragma unroll
-					for (int c = 0; c < 4; c++) {
-						if (st.tree) {
-							const int j = key0 + 32 * c - p.seq.kv_len;
-							if (j >= 0)
-								vis[c] = j < 64 ? (uint32_t)(bits >> j) : 0u;
-							else if (j > -32)
-								vis[c] = ((1u << -j) - 1u) | (uint32_t)bits << -j;
-						} else {
-							const int n = sees_to - (key0 + 32 * c);
-							vis[c] = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-						}
-						if (bad >> (2 * c) & 1)
-							vis[c] &= 0xffff0000u;
-						if (bad >> (2 * c + 1) & 1)
-							vis[c] &= 0x0000ffffu;
+				// which of 32 keys this row sees
+				auto visible = [&](int c) {
+					const int key = key0 + 32 * c;
+					uint32_t vis = ~0u;
+					if (st.tree) {
+						const int j = key - p.seq.kv_len;
+						if (j >= 0)
+							vis = j < 64 ? (uint32_t)(bits >> j) : 0u;
+						else if (j > -32)
+							vis = ((1u << -j) - 1u) | (uint32_t)bits << -j;
+					} else {
+						const int n = sees_to - key;
+						vis = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
 					}
-				}
+					return vis & ~((bad >> (2 * c) & 1 ? 0x0000ffffu : 0u) | (bad >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
+				};
 				// scores of 32 keys, times their rows' factors; -infinity where the row does not see
-				auto scores = [&](int c, float (&x)[32]) {
+				auto scores = [&](int c, float2 (&x)[16]) {
 					uint32_t v[32];
 					ptx::tmem_ld32(S + 32 * c, v);
 					ptx::tmem_ld_wait();
 #pragma unroll
-					for (int k = 0; k < 32; k += 4) {
-						float4 f = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-						if constexpr (T::SCALED)
-							f = *reinterpret_cast<const float4 *>(&sh->k_scale[fslot][32 * c + k]);
-						x[k] = __uint_as_float(v[k]) * f.x;
-						x[k + 1] = __uint_as_float(v[k + 1]) * f.y;
-						x[k + 2] = __uint_as_float(v[k + 2]) * f.z;
-						x[k + 3] = __uint_as_float(v[k + 3]) * f.w;
+					for (int k = 0; k < 16; k++)
+						x[k] = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+					if constexpr (T::SCALED) {
+#pragma unroll
+						for (int k = 0; k < 16; k += 2) {
+							const float4 f = *reinterpret_cast<const float4 *>(&sh->k_scale[fslot][32 * c + 2 * k]);
+							x[k] = mul2(x[k], make_float2(f.x, f.y));
+							x[k + 1] = mul2(x[k + 1], make_float2(f.z, f.w));
+						}
 					}
 					if (masked) {
+						const uint32_t vis = visible(c);
 #pragma unroll
-						for (int k = 0; k < 32; k++)
-							x[k] = vis[c] >> k & 1 ? x[k] : -INFINITY;
+						for (int k = 0; k < 16; k++) {
+							x[k].x = vis >> (2 * k) & 1 ? x[k].x : -INFINITY;
+							x[k].y = vis >> (2 * k + 1) & 1 ? x[k].y : -INFINITY;
+						}
 					}
 				};
 				float top = -INFINITY;
-#pragma unroll
-				for (int c = 0; c < 4; c++) {
-					float x[32];
+#pragma unroll 1
+				for (int c = 0; c < TILE / 32; c++) {
+					float2 x[16];
 					scores(c, x);
 #pragma unroll
-					for (int k = 0; k < 32; k++)
-						top = fmaxf(top, x[k]);
+					for (int k = 0; k < 16; k++)
+						top = fmaxf(top, fmaxf(x[k].x, x[k].y));
 				}
 				top = fmaxf(m, top * row_scale);
-				const float base = (top == -INFINITY ? 0.0f : top) - ATTN_P_SHIFT;
-				const float alpha = m == -INFINITY ? 0.0f : exp2f(m - top);
+				const float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
+				const float alpha = m == -INFINITY ? 0.0f : exp2_ftz(m - top);
 				m = top;
 				// the values' factors, and whether all of them are numbers; read before P is handed over: when its products are
 				// made the slot is another tile's
@@ -575,31 +680,35 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					if constexpr (T::SCALED)
 						v_top = sh->v_top[slot];
 				}
-				float sum = 0.0f;
-#pragma unroll
-				for (int c = 0; c < 4; c++) {
-					float x[32];
+				float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+				for (int c = 0; c < TILE / 32; c++) {
+					float2 x[16];
 					scores(c, x);
 					// the parts of 16 keys take the columns of their scores: hi 8, lo 8
-					uint32_t out[2][16];
 #pragma unroll
-					for (int k = 0; k < 32; k += 2) {
-						float p0 = exp2f(fmaf(x[k], row_scale, -base)), p1 = exp2f(fmaf(x[k + 1], row_scale, -base));
-						sum += p0 + p1;
-						if constexpr (T::SCALED) {
-							const float2 f = *reinterpret_cast<const float2 *>(&sh->v_scale[slot][32 * c + k]);
-							p0 = p0 == 0.0f ? 0.0f : p0 * f.x;
-							p1 = p1 == 0.0f ? 0.0f : p1 * f.y;
+					for (int h = 0; h < 2; h++) {
+						uint32_t out[16];
+#pragma unroll
+						for (int k = 0; k < 8; k++) {
+							const float2 e = fma2(x[8 * h + k], make_float2(row_scale, row_scale), make_float2(base, base));
+							float2 pk = make_float2(exp2_ftz(e.x), exp2_ftz(e.y));
+							sum = add2(sum, pk);
+							if constexpr (T::SCALED) {
+								const float2 f = *reinterpret_cast<const float2 *>(&sh->v_scale[slot][32 * c + 16 * h + 2 * k]);
+								const float2 z = mul2(pk, f);
+								// (where a row does not see every key, a factor that is no number is nothing to it)
+								pk = masked ? make_float2(pk.x == 0.0f ? 0.0f : z.x, pk.y == 0.0f ? 0.0f : z.y) : z;
+							}
+							split2(pk, out[k], out[8 + k]);
 						}
-						split2(p0, p1, out[k >> 4][(k >> 1) & 7], out[k >> 4][8 + ((k >> 1) & 7)]);
+						ptx::tmem_st16(S + 32 * c + 16 * h, out);
 					}
-					ptx::tmem_st16(S + 32 * c, out[0]);
-					ptx::tmem_st16(S + 32 * c + 16, out[1]);
 				}
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
 				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[wg]));
-				l = fmaf(l, alpha, sum);
+				l = fmaf(l, alpha, sum.x + sum.y);
 				wait(sh->o_full[wg], ph);
 				ptx::tc_fence_after();
 #pragma unroll
@@ -608,11 +717,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					ptx::tmem_ld32(lanes + COL_O + 32 * c, v);
 					ptx::tmem_ld_wait();
 #pragma unroll
-					for (int k = 0; k < 32; k++) {
+					for (int k = 0; k < 16; k++) {
+						const float2 o = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f = make_float2(alpha, alpha);
 						if constexpr (T::SCALED)
-							acc[32 * c + k] = fmaf(__uint_as_float(v[k]), v_top, acc[32 * c + k] * alpha);
+							acc[16 * c + k] = fma2(o, make_float2(v_top, v_top), mul2(acc[16 * c + k], f));
 						else
-							acc[32 * c + k] = fmaf(acc[32 * c + k], alpha, __uint_as_float(v[k]));
+							acc[16 * c + k] = fma2(acc[16 * c + k], f, o);
 					}
 				}
 				ptx::tc_fence_before();
@@ -622,21 +732,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					for (int k = 0; k < TILE; k++) {
 						if (key0 + k >= p.key_end)
 							break;
-						const uint32_t w = k < 32 ? vis[0] : k < 64 ? vis[1] : k < 96 ? vis[2] : vis[3];
-						if (!(w >> (k & 31) & 1))
+						if (!(visible(k >> 5) >> (k & 31) & 1))
 							continue;
 						const int page = st.page_table[(long long)p.s * st.max_pages + ((key0 + k) >> kv.page_shift)];
 						const long long at = (((long long)page * kv.n_head_kv + p.head) << kv.page_shift) + ((key0 + k) & ((1 << kv.page_shift) - 1));
 						const uint32_t *src = reinterpret_cast<const uint32_t *>(kv.v + at * T::ROW);
 						constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-						for (int d = 0; d < D / 2; d++) {
+						for (int d = 0; d < HALF; d++) {
 							const uint32_t x = src[d];
 							if (nonfinite16(x, EXPONENT)) {
 								const float2 f = KIND == TIE_CUDA_KV_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&x))
 													 : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-								acc[2 * d] += (x & EXPONENT) == EXPONENT ? f.x : 0.0f;
-								acc[2 * d + 1] += (x >> 16 & EXPONENT) == EXPONENT ? f.y : 0.0f;
+								acc[d].x += (x & EXPONENT) == EXPONENT ? f.x : 0.0f;
+								acc[d].y += (x >> 16 & EXPONENT) == EXPONENT ? f.y : 0.0f;
 							}
 						}
 					}
@@ -648,11 +757,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const uint32_t give = hand + (uint32_t)(wg ^ 1) * (ROWS * HALF * 4) + r * 16, take = hand + (uint32_t)wg * (ROWS * HALF * 4) + r * 16;
 #pragma unroll
 			for (int j = 0; j < HALF / 4; j++) {
-				uint4 x;
-				x.x = __float_as_uint(wg ? acc[4 * j] : acc[HALF + 4 * j]);
-				x.y = __float_as_uint(wg ? acc[4 * j + 1] : acc[HALF + 4 * j + 1]);
-				x.z = __float_as_uint(wg ? acc[4 * j + 2] : acc[HALF + 4 * j + 2]);
-				x.w = __float_as_uint(wg ? acc[4 * j + 3] : acc[HALF + 4 * j + 3]);
+				const float2 x0 = wg ? acc[2 * j] : acc[HALF / 2 + 2 * j], x1 = wg ? acc[2 * j + 1] : acc[HALF / 2 + 2 * j + 1];
+				const uint4 x = make_uint4(__float_as_uint(x0.x), __float_as_uint(x0.y), __float_as_uint(x1.x), __float_as_uint(x1.y));
 				sts128(give + j * (ROWS * 16), x);
 			}
 			bar_sync<1, SOFT_THREADS>();
@@ -668,15 +774,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 #pragma unroll
 				for (int j = 0; j < HALF / 4; j++) {
 					const uint4 x = lds128(take + j * (ROWS * 16));
-					const uint32_t xo[4] = {x.x, x.y, x.z, x.w};
-					float y[4];
-#pragma unroll
-					for (int k = 0; k < 4; k++) {
-						const float mine = wg ? acc[HALF + 4 * j + k] : acc[4 * j + k];
-						// (a warpgroup whose keys the row does not see has nothing to give)
-						y[k] = ((f_own == 0.0f ? 0.0f : mine * f_own) + (f_other == 0.0f ? 0.0f : __uint_as_float(xo[k]) * f_other)) * inv;
-					}
-					*reinterpret_cast<float4 *>(dst + 4 * j) = make_float4(y[0], y[1], y[2], y[3]);
+					const float2 m0 = wg ? acc[HALF / 2 + 2 * j] : acc[2 * j], m1 = wg ? acc[HALF / 2 + 2 * j + 1] : acc[2 * j + 1];
+					// (a warpgroup whose keys the row does not see has nothing to give)
+					auto join = [&](float mine, uint32_t others) {
+						return ((f_own == 0.0f ? 0.0f : mine * f_own) + (f_other == 0.0f ? 0.0f : __uint_as_float(others) * f_other)) * inv;
+					};
+					*reinterpret_cast<float4 *>(dst + 4 * j) = make_float4(join(m0.x, x.x), join(m0.y, x.y), join(m1.x, x.z), join(m1.y, x.w));
 				}
 			}
 			if (!whole) {
@@ -684,33 +787,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					part[ROWS * 128 + r] = top;
 					part[ROWS * 128 + ROWS + r] = sum;
 				}
-				const long long i0 = walk.u - p.unit1, i1 = i0 + p.item_units - 1;  // (walk.u: behind this piece)
-				const int c0 = attn_cta_of(i0, walk.total, walk.n_cta), c1 = attn_cta_of(i1, walk.total, walk.n_cta);
-				__threadfence();
-				bar_sync<1, SOFT_THREADS>();
-				if (threadIdx.x == 0)
-					work.last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
-				bar_sync<1, SOFT_THREADS>();
-				if (work.last) {
-					__threadfence();
-					for (int i = warp; i < ROWS && p.row0 + i < n_rows; i += SOFT_THREADS / 32) {
-						const int t = (p.row0 + i) / a.group;
-						attn_join_row<D, ROWS>(a.part, c0, c1, i, lane,
-								       a.out + ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + (p.row0 + i - t * a.group)) * D);
-					}
-					if (threadIdx.x == 0)
-						a.count[c0] = 0;  // at rest again
-				}
 			}
 		}
 	} else if (warp < W_MMA) {
 		ptx::setmaxnreg_dec<LOAD_REGS>();
 		if (warp < W_VALUES) {
 			Loader<KIND, D, false> loader = {kv, st, sh, k_ring, (int)threadIdx.x - W_KEYS * 32, lane};
-			loader.run(walk, work, a, wait);
+			loader.run(wait);
 		} else {
 			Loader<KIND, D, true> loader = {kv, st, sh, v_ring, (int)threadIdx.x - W_VALUES * 32, lane};
-			loader.run(walk, work, a, wait);
+			loader.run(wait);
 		}
 	} else {
 		ptx::setmaxnreg_dec<MMA_REGS>();
@@ -739,7 +825,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					ptx::mma_commit(ptx::smem_u32(&sh->o_full[slot]));
 				};
 				Piece p;
-				while (next_piece(walk, p, work, kv, st, a)) {
+				for (uint32_t n = 0;; n++) {
+					p = take_piece(sh, wait, n);
+					ptx::mbar_arrive(ptx::smem_u32(&sh->piece_free[n % PIECES]));
+					if (p.s < 0)
+						break;
 					if (p.n_tiles == 0)
 						continue;
 					wait(sh->q_full, pieces & 1u);
@@ -768,13 +858,56 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			}
 			__syncwarp();
 			wait(sh->fin, 0);
+		} else if (warp == W_PIECES && lane == 0) {
+			Piece p;
+			Walk walk_on = walk;
+			for (uint32_t n = 0;; n++) {
+				const bool any = next_piece(walk_on, p, work, kv, st, a);
+				if (!any)
+					p.s = -1;
+				if (n >= PIECES)
+					wait(sh->piece_free[n % PIECES], (n / PIECES & 1u) ^ 1u, true);
+				sh->piece[n % PIECES] = p;
+				ptx::mbar_arrive(ptx::smem_u32(&sh->piece_full[n % PIECES]));
+				if (!any)
+					break;
+			}
 		}
 	}
 	ptx::tc_fence_before();
 	__syncthreads();
+	pdl_trigger();	// attn_join may set itself up
 	if (warp == W_MMA) {
 		ptx::tc_fence_after();
 		ptx::tmem_dealloc(tmem, 512);
+	}
+}
+
+// The parts that CTAs left of the items they shared, joined: CTA (c, i) takes 16 rows of the item that began in CTA c and
+// went on behind it, if there is one.  A launch of its own: an item of a few tiles of keys a CTA has tens of parts of
+// 66 KB, and one CTA, the last at the item, took 130 us to add them up (tree of 13 tokens over 9001 slots: 172 us).
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = 16;
+template <int D>
+__global__ void __launch_bounds__(JOIN_THREADS) attn_join(const KvView kv, const StepView st, const AttnArgs a, int n_cta)
+{
+	__shared__ AttnWork work;
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
+	const Walk w = start_walk<JOIN_THREADS>(work, kv, st, a, n_cta, c0);
+	if (!w.shared || w.u >= w.u_end)
+		return;
+	const long long u = w.u_end - 1;
+	const int s = attn_sequence_of(work, st.n_seq, u);
+	const SeqView seq = kv_sequence(st, kv.page_shift, s);
+	const int units = attn_units(seq), tiles = (int)(((long long)seq.n_tok * a.group + ROWS - 1) / ROWS);
+	const long long item = (u - work.start[s]) / units, i0 = work.start[s] + item * units, i1 = i0 + units - 1;
+	if (i0 < w.u || i1 == u)
+		return;
+	const int c1 = attn_cta_of(i1, w.total, w.n_cta), head = (int)(item / tiles), row0 = (int)(item % tiles) * ROWS;
+	pdl_wait();
+	for (int i = blockIdx.y * JOIN_ROWS + warp; i < (blockIdx.y + 1) * JOIN_ROWS && row0 + i < seq.n_tok * a.group; i += JOIN_THREADS / 32) {
+		const int t = (row0 + i) / a.group;
+		attn_join_row<D, ROWS>(a.part, c0, c1, i, lane,
+				       a.out + ((long long)(seq.tok0 + t) * a.n_head + head * a.group + (row0 + i - t * a.group)) * D);
 	}
 }
 
@@ -788,7 +921,7 @@ int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
 	attn_tiles<KIND, D><<<c->sm_count, THREADS, smem_bytes<KIND, D>(), c->stream>>>(kv, st, a);
 	TIE_CUDA_LAUNCHED(c);
-	return TIE_CUDA_OK;
+	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / JOIN_ROWS), JOIN_THREADS, 0, kv, st, a, c->sm_count);
 }
 template <int KIND>
 int allow_smem(tie_cuda_ctx *c)
