@@ -427,8 +427,10 @@ int kv_views(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_
 	    (cache->page_size & (cache->page_size - 1)) || cache->n_pages < 1 || !cache->k || !cache->v || !aligned16(cache->k) ||
 	    !aligned16(cache->v))
 		return TIE_CUDA_EINVAL;
-	if (q8 && (!cache->k_scale || !cache->v_scale || ((uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & 3))
+	if (q8 && (!cache->k_scale || !cache->v_scale || !aligned16(cache->k_scale) || !aligned16(cache->v_scale)))
 		return TIE_CUDA_EINVAL;
+	if (((long long)cache->n_pages * cache->n_head_kv) * cache->page_size > 0x7fffffff)
+		return TIE_CUDA_ENOTSUP;  // (rows are numbered in 32 bits where boxes of them are asked for)
 	if (step->n_seq < 1 || step->n_seq > KV_MAX_SEQ || step->n_tokens < 0 || !step->tok_start || !step->kv_len || !step->page_table ||
 	    step->max_pages < 1 || (long long)step->max_pages * cache->page_size > 1 << 30 ||
 	    ((uintptr_t)step->tok_start | (uintptr_t)step->kv_len | (uintptr_t)step->page_table | (uintptr_t)step->pos) & 3 ||

@@ -3,37 +3,37 @@
 //
 //   S = Q K^T, P = exp2(S - max), O = P V      rows (token, head of the group) on the 128 lanes of tensor memory
 //
-// fp32 results need more than one 16-bit operand per value: Q and P are fp16 hi + lo (22 bits), two MMAs each, against
-// keys and values that are exact in fp16 (F16; Q8's whole numbers; BF16 rows brought to fp16 by a power of two), the factors
-// of rows applied in fp32.  The products of a tile start from zero and are added to fp32 registers: the tensor cores cut
-// every sum off, which over a long cache would add up.
+// fp32 results need more than one 16-bit operand per value.  F16 and Q8: Q and P are fp16 hi + lo (22 bits) against keys and
+// values that are exact in fp16, the factors of Q8's rows applied in fp32; BF16: three bf16 parts (24 bits), tiles of 64
+// keys, since tensor memory holds no more.  The products of a tile start from zero and are added to fp32 registers: the
+// tensor cores cut every sum off, which over a long cache would add up.
 //
 // One CTA per SM, 512 threads:
 //   * two warpgroups of softmax threads, a thread per row, take key tiles in turn, each with a running maximum, sum and
 //     output row of its own (joined at the end), so that one's exponentials run under the other's MMAs;
-//   * two warps load keys, two values: cp.async into the swizzled operand layout (pages of 16 slots and more, zeros behind
-//     the last key), expanded to fp16 in place where the cache has another type;
-//   * one thread finds the CTA's pieces of work, one issues the MMAs.  Q and P are operands in tensor memory (a step of shared memory then feeds only the 128
-//     keys or dims of its other operand: half of what the memory delivers); P's parts of 16 keys take the columns of these keys' scores.
-// Tensor memory: Q 128 columns, two score tiles, O: all 512.  Every wait is bounded, as in tensor.cu; after a
-// time-out no wait waits any more and all roles run to their ends.
+//   * a warp requests keys, another values, by TMA straight into the swizzled operand layout, a box per page (as one
+//     cp.async per 16 bytes the address arithmetic alone took 5000 cycles a tile from two warps);
+//   * two warps each make operands of what came in where it is not one yet: Q8's bytes become fp16 in place, values behind
+//     the last key and values that are no numbers become zeros;
+//   * one thread finds the CTA's pieces of work, one issues the MMAs.  Q and P are operands in tensor memory (a step of
+//     shared memory then feeds only the keys or dims of the other operand: half of what the memory delivers); P's parts
+//     of 16 keys take the columns of these keys' scores.
+// Every wait is bounded, as in tensor.cu; after a time-out no wait waits any more and all roles run to their ends.
 #include <float.h>
 
 #include "attn.cuh"
+#include "decode_common.cuh"
 #include "kernels.cuh"
 #include "tc_ptx.cuh"
 
 namespace tie {
 namespace {
 
-constexpr int ROWS = ATTN_MAX_ROWS, TILE = ATTN_UNIT;
-constexpr int THREADS = 512, SOFT_THREADS = 256, LOAD_THREADS = 64;
-constexpr int W_KEYS = 8, W_VALUES = 10, W_MMA = 12, W_PIECES = 13;  // first warps of the roles behind the softmax warps
-constexpr int PIECE_READERS = 13;  // the warps of those who work on them
-constexpr int SOFT_REGS = 192, LOAD_REGS = 80, MMA_REGS = 48;
-static_assert(2 * SOFT_REGS + LOAD_REGS + MMA_REGS <= 512, "a launch of 512 threads holds 128 registers a thread");
-constexpr int COL_Q = 0, COL_S = 128, COL_O = 384;
-constexpr uint32_t PANEL = TILE * 128;	// bytes of 64 dims of a tile: 128 rows of 128 bytes
+constexpr int ROWS = ATTN_MAX_ROWS;
+constexpr int THREADS = 512, SOFT_THREADS = 256, MAKE_THREADS = 64;
+constexpr int W_KEYS = 8, W_VALUES = 10, W_MMA = 12, W_PIECES = 13, W_ASK = 14;  // first warps of the roles behind the softmax warps
+constexpr int SOFT_REGS = 192, MAKE_REGS = 80, REST_REGS = 48;
+static_assert(2 * SOFT_REGS + MAKE_REGS + REST_REGS <= 512, "a launch of 512 threads holds 128 registers a thread");
 constexpr long long WAIT_CYCLES = 1ll << 30;
 
 // A piece of work of a CTA: an item, or (few items: shared) some units of one.  No more of them: s < 0.
@@ -45,24 +45,24 @@ struct Piece {
 	int key_end;	// first key that nobody sees
 	int all_see;	// keys in front of this one are seen by every row
 };
-constexpr int PIECES = 4;
+constexpr int PIECES = 4, MAX_STAGES = 4, MAX_FACTS = 8, MAX_TILE = 128;
 struct Shared {
 	uint64_t piece_full[PIECES], piece_free[PIECES];
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
-	uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
-	uint64_t s_full[2], p_full[2], o_full[2], o_free, q_full, fin;  // (o_full: a warpgroup's own, so that it waits for every phase)
+	uint64_t k_raw[MAX_STAGES], k_full[MAX_STAGES], k_free[MAX_STAGES];  // keys have come in; are the operand; have been used
+	uint64_t v_raw[MAX_STAGES], v_full[MAX_STAGES], v_free[MAX_STAGES];
+	uint64_t s_full[2], p_full[2], o_full[2], o_free, q_full, fin;	// (a warpgroup's own where only it waits: it sees every phase)
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
-	// made.  Tile n + 4 is requested after the scores of n + 2, these after the products of n, whose P then has been made.
-	uint64_t f_full[4];
-	uint32_t bad[4];	  // groups of 16 keys of a tile whose page does not exist
-	alignas(16) float k_scale[4][TILE];
-	alignas(16) float v_raw[2][TILE], v_scale[2][TILE];
-	float v_top[2];
-	uint32_t odd[2][2];	  // a masked tile's values hold one that is no number (per loading warp)
-	uint32_t tmem_base, abort;
-	float load_max[2][2];
+	// made: tile n + FACTS is requested after the scores of tile n + 2 at the least, these after the products of n.
+	uint64_t f_full[MAX_FACTS];
+	uint32_t bad[MAX_FACTS], bad_values[MAX_STAGES];  // groups of 16 keys of a tile whose page does not exist
+	alignas(16) float k_scale[MAX_FACTS][MAX_TILE];
+	alignas(16) float v_got[2][MAX_TILE], v_scale[2][MAX_TILE];
+	float v_top[2], make_max[2][2];
+	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
 	float q_max[2][ROWS];
 	float2 ml[2][ROWS];
+	uint32_t tmem_base, abort;
 };
 
 struct Walk {
@@ -71,14 +71,16 @@ struct Walk {
 	int n_cta, round;
 };
 
+template <int TK>
 __device__ __forceinline__ void finish_piece(Piece &p, const StepView &st, const AttnArgs &a)
 {
 	const int first_tok = p.row0 / a.group, last_tok = min((p.row0 + ROWS - 1) / a.group, p.seq.n_tok - 1);
 	p.key_end = p.seq.kv_len + (st.tree ? p.seq.n_tok : last_tok + 1);
 	p.all_see = p.seq.kv_len + (st.tree ? 0 : first_tok + 1);
-	p.n_tiles = max(0, min(p.unit1, (p.key_end + TILE - 1) / TILE) - p.unit0);
+	p.n_tiles = max(0, (min(p.unit1 * ATTN_UNIT, p.key_end) - p.unit0 * ATTN_UNIT + TK - 1) / TK);
 }
 
+template <int TK>
 __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
 	if (w.shared) {
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &wo
 		p.unit0 = 0;
 		p.unit1 = p.item_units = attn_units(p.seq);
 	}
-	finish_piece(p, st, a);
+	finish_piece<TK>(p, st, a);
 	return true;
 }
 
@@ -140,17 +142,23 @@ __device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, con
 
 template <int KIND, int D>
 struct Tile {
-	static constexpr bool SCALED = KIND != TIE_CUDA_KV_F16;
-	static constexpr int ROW = KIND == TIE_CUDA_KV_Q8 ? D : 2 * D;	// bytes of a head row of the cache
-	static constexpr int CHUNKS = ROW / 16;
-	static constexpr uint32_t BYTES = TILE * D * 2;
-	// where a 16-byte chunk of row r's fp16 values lies in the operand tile
+	static constexpr bool SCALED = KIND == TIE_CUDA_KV_Q8;
+	static constexpr int TK = KIND == TIE_CUDA_KV_BF16 ? 64 : 128;	 // keys
+	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	 // of a value of Q and of P
+	static constexpr int STAGES = KIND == TIE_CUDA_KV_BF16 || (KIND == TIE_CUDA_KV_F16 && D == 64) ? 4 : 2;
+	static constexpr int FACTS = 2 * STAGES;
+	static_assert(FACTS >= STAGES + 2 && FACTS <= MAX_FACTS && STAGES <= MAX_STAGES && (!SCALED || STAGES == 2), "rings");
+	// tensor memory: parts of Q, two score tiles (and what P's parts need beyond their columns), O
+	static constexpr int SLOT = PARTS == 3 ? TK + TK / 2 : TK, COL_Q = 0, COL_S = PARTS * D / 2, COL_O = COL_S + 2 * SLOT;
+	static_assert(COL_O + D <= 512, "tensor memory");
+	static constexpr uint32_t PANEL = TK * 128;  // 64 dims of a tile: rows of 128 bytes
+	static constexpr uint32_t BYTES = TK * D * 2;
+	static constexpr int ROW = SCALED ? D : 2 * D;	 // bytes of a head row of the cache
+	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128, BOXES = ROW / BOX_BYTES;  // of a row, per TMA box
+	static constexpr uint32_t RAW = SCALED && D == 64 ? TK * ROW : 0;  // rows of 64 bytes come in beside the operand
+	static constexpr size_t SMEM = 2 * (size_t)STAGES * (BYTES + RAW) + (size_t)ROWS * D * 4 + 1024;
+	// where a 16-byte chunk of row r's 16-bit values lies in the operand tile
 	__device__ static __forceinline__ uint32_t place(int r, int ch) { return (ch >> 3) * PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
-	// ... and where it comes in: packed bytes lie in the last panel until they are expanded
-	__device__ static __forceinline__ uint32_t raw(int r, int ch)
-	{
-		return KIND == TIE_CUDA_KV_Q8 ? (D == 128 ? PANEL : 0u) + r * 128 + ((ch ^ (r & 7)) << 4) : place(r, ch);
-	}
 };
 
 __device__ __forceinline__ uint4 lds128(uint32_t at)
@@ -239,265 +247,199 @@ __device__ __forceinline__ float exp2_ftz(float x)
 	return r;
 }
 
-// fp16 hi and lo of a pair
-__device__ __forceinline__ void split2(float2 x, uint32_t &hi, uint32_t &lo)
+// The 16-bit parts of a pair, the largest first: fp16 hi and lo, or three of bf16.
+template <int KIND, int PARTS>
+__device__ __forceinline__ void split2(float2 x, uint32_t (&part)[PARTS])
 {
-	const __half2 h = __floats2half2_rn(x.x, x.y);
-	const float2 f = __half22float2(h), d = add2(x, make_float2(-f.x, -f.y));
-	const __half2 l = __floats2half2_rn(d.x, d.y);
-	hi = *reinterpret_cast<const uint32_t *>(&h);
-	lo = *reinterpret_cast<const uint32_t *>(&l);
+#pragma unroll
+	for (int p = 0; p < PARTS; p++) {
+		float2 f;
+		if constexpr (KIND == TIE_CUDA_KV_BF16) {
+			const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+			part[p] = *reinterpret_cast<const uint32_t *>(&h);
+			f = make_float2(-__uint_as_float(part[p] << 16), -__uint_as_float(part[p] & 0xffff0000u));
+		} else {
+			const __half2 h = __floats2half2_rn(x.x, x.y);
+			part[p] = *reinterpret_cast<const uint32_t *>(&h);
+			f = __half22float2(h);
+			f = make_float2(-f.x, -f.y);
+		}
+		if (p < PARTS - 1)
+			x = add2(x, f);
+	}
 }
 
-// Larger magnitudes of two pairs of bf16 (NaN where there is one)
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b)
-{
-	const __nv_bfloat162 r = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&b)));
-	return *reinterpret_cast<const uint32_t *>(&r);
-}
-__device__ __forceinline__ uint32_t half2_of_bf16x2(uint32_t w, float f)
-{
-	const float2 x = mul2(make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), make_float2(f, f));
-	const __half2 h = __floats2half2_rn(x.x, x.y);
-	return *reinterpret_cast<const uint32_t *>(&h);
-}
 // All ones over those of a pair that are numbers.
 __device__ __forceinline__ uint32_t finite16(uint32_t w, uint32_t exponent)
 {
 	return ((w & exponent) == exponent ? 0u : 0xffffu) | ((w >> 16 & exponent) == exponent ? 0u : 0xffff0000u);
 }
 
-// The loading warps of keys (VALUES false) or values: 64 threads.
+// Requests the tiles of keys (VALUES false) or values: a warp, a lane per page of a tile.
 template <int KIND, int D, bool VALUES>
-struct Loader {
+__device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared *sh, const CUtensorMap *map, uint32_t ring, uint32_t raw, const Waiter &wait,
+				    int lane)
+{
 	using T = Tile<KIND, D>;
-	const KvView &kv;
-	const StepView &st;
-	Shared *sh;
-	uint32_t ring;	// two operand tiles
-	int t, lane;
-
-	// Requests tile `unit` of piece p, this CTA's n-th.
-	__device__ __forceinline__ void issue(const Piece &p, int unit, uint32_t n)
-	{
-		const uint32_t slot = n & 1u;
-		const uint8_t *rows = VALUES ? kv.v : kv.k;
-		const int key0 = unit * TILE, page_mask = (1 << kv.page_shift) - 1, grp = lane & 7;
-		// a lane finds the row of one group of 16 keys
-		long long first = -1;
-		const int gkey = key0 + grp * 16;
-		if (gkey < p.key_end) {
-			first = kv_page_row(kv, st, st.page_table[(long long)p.s * st.max_pages + (gkey >> kv.page_shift)], p.head);
-			if (first >= 0)
-				first += gkey & page_mask;
-		}
-		const uint32_t bad = __ballot_sync(0xffffffffu, gkey < p.key_end && first < 0) & 0xffu;
-		if (!VALUES && t == 0)
-			sh->bad[n & 3u] = bad;
-		const uint32_t dst = ring + slot * T::BYTES;
-		constexpr int AT_ONCE = LOAD_THREADS / T::CHUNKS, PASSES = TILE / AT_ONCE, PER_GROUP = 16 / AT_ONCE;
-		const int ch = t % T::CHUNKS, r0 = t / T::CHUNKS;
+	const int run = min(1 << kv.page_shift, T::TK), n_runs = T::TK / run, page_mask = (1 << kv.page_shift) - 1;
+	uint64_t *free_bar = VALUES ? sh->v_free : sh->k_free, *raw_bar = VALUES ? sh->v_raw : sh->k_raw;
+	uint32_t n = 0;
+	for (uint32_t pn = 0;; pn++) {
+		const Piece p = take_piece(sh, wait, pn);
+		drop_piece(sh, pn, lane);
+		if (p.s < 0)
+			break;
+		const int *pages = st.page_table + (long long)p.s * st.max_pages;
+		auto page_of = [&](int i) {  // of this lane's keys of the piece's tile i
+			const int key = p.unit0 * ATTN_UNIT + i * T::TK + lane * run;
+			return lane < n_runs && i < p.n_tiles && key < p.key_end ? pages[key >> kv.page_shift] : -1;
+		};
+		int next = page_of(0);
+		for (int i = 0; i < p.n_tiles; i++, n++) {
+			const int key0 = p.unit0 * ATTN_UNIT + i * T::TK, key = key0 + lane * run, page = next;
+			const uint32_t slot = n % T::STAGES;
+			next = page_of(i + 1);
+			const bool wanted = lane < n_runs && key < p.key_end;
+			long long row = wanted ? kv_page_row(kv, st, page, p.head) : -1;
+			const bool in = row >= 0;
+			const uint32_t got = __ballot_sync(0xffffffffu, in), lost = __ballot_sync(0xffffffffu, wanted && !in);
+			row += key & page_mask;
+			if (n >= T::STAGES)
+				wait(free_bar[slot], (n / T::STAGES & 1u) ^ 1u);
+			__syncwarp();
+			if (lane == 0) {
+				uint32_t bad = 0;
+				if (lost)
+					for (int g = 0; g < T::TK / 16; g++)
+						bad |= (lost >> (g * 16 / run) & 1u) << g;
+				(VALUES ? sh->bad_values[slot] : sh->bad[n % T::FACTS]) = bad;
+				if (!VALUES && !T::SCALED)
+					ptx::mbar_arrive(ptx::smem_u32(&sh->f_full[n % T::FACTS]));
+				ptx::mbar_arrive_expect_tx(ptx::smem_u32(&raw_bar[slot]), __popc(got) * run * (T::ROW + (T::SCALED ? 4 : 0)));
+			}
+			__syncwarp();
+			if (in) {
+				const uint32_t bar = ptx::smem_u32(&raw_bar[slot]);
+				const uint32_t dst = T::RAW ? raw + slot * T::RAW + lane * run * T::ROW
+							    : ring + slot * T::BYTES + (T::SCALED ? T::PANEL : 0u) + lane * run * 128;
 #pragma unroll
-		for (int i = 0; i < PASSES; i++) {
-			const int r = r0 + i * AT_ONCE;
-			const long long row = __shfl_sync(0xffffffffu, first, AT_ONCE <= 16 ? i / (PER_GROUP ? PER_GROUP : 1) : r >> 4);
-			const bool in = row >= 0 && key0 + r < p.key_end;
-			cp_async16_or_zero(dst + T::raw(r, ch), rows + (in ? (row + (r & 15)) * T::ROW + ch * 16 : 0), in);
-		}
-		if constexpr (KIND == TIE_CUDA_KV_Q8) {
-			const float *scales = VALUES ? kv.v_scale : kv.k_scale;
-			const uint32_t to = ptx::smem_u32(VALUES ? sh->v_raw[slot] : sh->k_scale[n & 3u]);
-#pragma unroll
-			for (int i = 0; i < 2; i++) {
-				const int r = t + LOAD_THREADS * i;
-				const long long row = __shfl_sync(0xffffffffu, first, r >> 4);
-				const bool in = row >= 0 && key0 + r < p.key_end;
-				cp_async4_or_zero(to + 4 * r, scales + (in ? row + (r & 15) : 0), in);
+				for (int b = 0; b < T::BOXES; b++)
+					ptx::tma_load_2d(dst + b * T::PANEL, map, bar, b * 64, (int)row);
+				if constexpr (T::SCALED)
+					bulk_g2s(ptx::smem_u32(VALUES ? sh->v_got[slot] : sh->k_scale[n % T::FACTS]) + 4 * lane * run, (VALUES ? kv.v_scale : kv.k_scale) + row,
+						  run * 4, bar);
 			}
 		}
-		ptx::cp_async_commit();
 	}
+}
 
-	// The n-th tile has come in (this thread's part of it): makes it the operand and hands it over.
-	__device__ __forceinline__ void finish(const Piece &p, int unit, uint32_t n)
-	{
-		const uint32_t slot = n & 1u;
-		const uint32_t at = ring + slot * T::BYTES;
-		constexpr int AT_ONCE = LOAD_THREADS / T::CHUNKS, PASSES = TILE / AT_ONCE;
-		const int ch = t % T::CHUNKS, r0 = t / T::CHUNKS;
-		const bool masked = (unit + 1) * TILE > p.all_see;
-		float *scale = VALUES ? sh->v_raw[slot] : sh->k_scale[n & 3u];
-		bool odd = false;
-		if constexpr (KIND == TIE_CUDA_KV_Q8) {
-#pragma unroll
-			for (int i0 = 0; i0 < PASSES; i0 += 4) {
-				uint4 v[4];
-#pragma unroll
-				for (int i = 0; i < 4; i++)
-					v[i] = lds128(at + T::raw(r0 + (i0 + i) * AT_ONCE, ch));
-				__syncwarp();  // a row's bytes are all in registers before its values overwrite them
-#pragma unroll
-				for (int i = 0; i < 4; i++) {
-					const int r = r0 + (i0 + i) * AT_ONCE;
-					const uint32_t b[4] = {v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u};
-					sts128(at + T::place(r, 2 * ch), make_uint4(int8_pair<0x4140>(b[0]), int8_pair<0x4342>(b[0]), int8_pair<0x4140>(b[1]), int8_pair<0x4342>(b[1])));
-					sts128(at + T::place(r, 2 * ch + 1), make_uint4(int8_pair<0x4140>(b[2]), int8_pair<0x4342>(b[2]), int8_pair<0x4140>(b[3]), int8_pair<0x4342>(b[3])));
-				}
-			}
-		} else {
-			constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
-			if (VALUES && masked) {
+// Makes operands of what has come in: two warps for keys (Q8 only), two for values.
+template <int KIND, int D, bool VALUES>
+__device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, const Waiter &wait, int t, int lane)
+{
+	using T = Tile<KIND, D>;
+	uint32_t n = 0;
+	for (uint32_t pn = 0;; pn++) {
+		const Piece p = take_piece(sh, wait, pn);
+		drop_piece(sh, pn, lane);
+		if (p.s < 0)
+			break;
+		for (int i = 0; i < p.n_tiles; i++, n++) {
+			const int key0 = p.unit0 * ATTN_UNIT + i * T::TK;
+			const uint32_t slot = n % T::STAGES, at = ring + slot * T::BYTES;
+			wait(VALUES ? sh->v_raw[slot] : sh->k_raw[slot], n / T::STAGES & 1u);
+			const uint32_t bad = VALUES ? sh->bad_values[slot] : 0u;
+			const bool masked = VALUES && (key0 + T::TK > p.all_see || bad != 0);
+			bool odd = false;
+			// the keys that are somebody's: the others' values are zeros, whatever has come in
+			auto there = [&](int r) { return key0 + r < p.key_end && !(bad >> (r >> 4) & 1u); };
+			if constexpr (T::SCALED) {
+				constexpr int CHUNKS = T::ROW / 16, AT_ONCE = MAKE_THREADS / CHUNKS, PASSES = T::TK / AT_ONCE, B = 8;
+				const int ch = t % CHUNKS, r0 = t / CHUNKS;
 #pragma unroll 1
-				for (int i = 0; i < PASSES; i++) {
-					const uint32_t to = at + T::place(r0 + i * AT_ONCE, ch);
+				for (int j0 = 0; j0 < PASSES; j0 += B) {
+					uint4 v[B];
+#pragma unroll
+					for (int j = 0; j < B; j++) {
+						const int r = r0 + (j0 + j) * AT_ONCE;
+						v[j] = lds128(T::RAW ? raw + slot * T::RAW + r * T::ROW + ch * 16 : at + T::PANEL + r * 128 + ((ch ^ (r & 7)) << 4));
+					}
+					__syncwarp();  // a row's bytes are all in registers before its values overwrite them
+#pragma unroll
+					for (int j = 0; j < B; j++) {
+						const int r = r0 + (j0 + j) * AT_ONCE;
+						if (masked && !there(r))
+							v[j] = make_uint4(0, 0, 0, 0);
+						const uint32_t b[4] = {v[j].x ^ 0x80808080u, v[j].y ^ 0x80808080u, v[j].z ^ 0x80808080u, v[j].w ^ 0x80808080u};
+						sts128(at + T::place(r, 2 * ch), make_uint4(int8_pair<0x4140>(b[0]), int8_pair<0x4342>(b[0]), int8_pair<0x4140>(b[1]), int8_pair<0x4342>(b[1])));
+						sts128(at + T::place(r, 2 * ch + 1), make_uint4(int8_pair<0x4140>(b[2]), int8_pair<0x4342>(b[2]), int8_pair<0x4140>(b[3]), int8_pair<0x4342>(b[3])));
+					}
+				}
+				if constexpr (VALUES) {	 // factors relative to the tile's largest, which multiplies the tile's sums
+					float f[2];
+					float top = 0.0f;
+#pragma unroll
+					for (int j = 0; j < 2; j++) {
+						f[j] = there(t + MAKE_THREADS * j) ? sh->v_got[slot][t + MAKE_THREADS * j] : 0.0f;
+						// (an infinite factor is as little a number as NaN, and NaN does not reach the largest)
+						f[j] = fabsf(f[j]) <= FLT_MAX ? f[j] : __int_as_float(0x7fc00000);
+						top = fmaxf(top, fabsf(f[j]));
+					}
+#pragma unroll
+					for (int o = 16; o; o >>= 1)
+						top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+					if (lane == 0)
+						sh->make_max[slot][t >> 5] = top;
+					bar_sync<3, MAKE_THREADS>();
+					top = fmaxf(sh->make_max[slot][0], sh->make_max[slot][1]);
+					top = top > 0.0f ? top : 1.0f;
+					if (t == 0)
+						sh->v_top[slot] = top;
+					sh->v_scale[slot][t] = f[0] / top;
+					sh->v_scale[slot][t + MAKE_THREADS] = f[1] / top;
+				}
+			} else if (masked) {
+				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
+				constexpr int CHUNKS = T::ROW / 16, AT_ONCE = MAKE_THREADS / CHUNKS, PASSES = T::TK / AT_ONCE;
+				const int ch = t % CHUNKS, r0 = t / CHUNKS;
+#pragma unroll 4
+				for (int j = 0; j < PASSES; j++) {
+					const int r = r0 + j * AT_ONCE;
+					const uint32_t to = at + T::place(r, ch);
 					const uint4 v = lds128(to);
 					uint32_t w[4] = {v.x, v.y, v.z, v.w};
 					bool change = false;
+					if (!there(r)) {
+						w[0] = w[1] = w[2] = w[3] = 0;
+						change = true;
+					} else {
 #pragma unroll
-					for (int j = 0; j < 4; j++)
-						if (nonfinite16(w[j], EXPONENT)) {  // (its products are made by the rows that see it)
-							w[j] &= finite16(w[j], EXPONENT);
-							odd = change = true;
-						}
+						for (int k = 0; k < 4; k++)
+							if (nonfinite16(w[k], EXPONENT)) {  // (its products are made by the rows that see it)
+								w[k] &= finite16(w[k], EXPONENT);
+								odd = change = true;
+							}
+					}
 					if (change)
 						sts128(to, make_uint4(w[0], w[1], w[2], w[3]));
 				}
 			}
-			if constexpr (KIND == TIE_CUDA_KV_BF16) {
-				// a row's largest to 2^14 .. 2^15: its 8 bits are exact down to 2^-32 of it
-				constexpr int B = 8;  // rows at once, for their latencies
-#pragma unroll 1
-				for (int i0 = 0; i0 < PASSES; i0 += B) {
-					uint4 v[B];
-					uint32_t top[B];
-#pragma unroll
-					for (int i = 0; i < B; i++) {
-						v[i] = lds128(at + T::place(r0 + (i0 + i) * AT_ONCE, ch));
-						top[i] = max_bf16x2(max_bf16x2(v[i].x, v[i].y), max_bf16x2(v[i].z, v[i].w));
-					}
-#pragma unroll
-					for (int o = T::CHUNKS / 2; o; o >>= 1)
-#pragma unroll
-						for (int i = 0; i < B; i++)
-							top[i] = max_bf16x2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-#pragma unroll
-					for (int i = 0; i < B; i++) {
-						const int r = r0 + (i0 + i) * AT_ONCE;
-						uint32_t largest = max(top[i] & 0x7fffu, top[i] >> 16 & 0x7fffu);
-						if (__any_sync(0xffffffffu, largest >= EXPONENT)) {  // the largest among the numbers, where some are none
-							const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-							largest = 0;
-							for (int j = 0; j < 4; j++) {
-								const uint32_t f = w[j] & 0x7fff7fffu & finite16(w[j], EXPONENT);
-								largest = max(largest, max(f & 0xffffu, f >> 16));
-							}
-							for (int o = T::CHUNKS / 2; o; o >>= 1)
-								largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-						}
-						const int e = max((int)(largest >> 7), 15);
-						const float f = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
-						if (ch == 0)
-							scale[r] = __uint_as_float((uint32_t)(127 - 141 + e) << 23);
-						sts128(at + T::place(r, ch), make_uint4(half2_of_bf16x2(v[i].x, f), half2_of_bf16x2(v[i].y, f), half2_of_bf16x2(v[i].z, f),
-											half2_of_bf16x2(v[i].w, f)));
-					}
-				}
-			}
-		}
-		if constexpr (T::SCALED) {
-			// keys: the factors as they are; values: relative to the tile's largest, which multiplies the tile's sums
 			if (VALUES) {
-				if (KIND == TIE_CUDA_KV_BF16)
-					bar_sync<3, LOAD_THREADS>();
-				float f[2] = {scale[t], scale[t + LOAD_THREADS]};
-#pragma unroll
-				for (int i = 0; i < 2; i++)  // (an infinite factor is as little a number as NaN, and NaN does not reach the largest)
-					f[i] = fabsf(f[i]) <= FLT_MAX ? f[i] : __int_as_float(0x7fc00000);
-				float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), 0.0f);
-#pragma unroll
-				for (int o = 16; o; o >>= 1)
-					top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+				odd = __any_sync(0xffffffffu, odd);
 				if (lane == 0)
-					sh->load_max[slot][t >> 5] = top;
-				bar_sync<3, LOAD_THREADS>();
-				top = fmaxf(sh->load_max[slot][0], sh->load_max[slot][1]);
-				top = top > 0.0f ? top : 1.0f;
-				if (t == 0)
-					sh->v_top[slot] = top;
-				sh->v_scale[slot][t] = f[0] / top;
-				sh->v_scale[slot][t + LOAD_THREADS] = f[1] / top;
+					sh->odd[slot][t >> 5] = odd;
+			} else {
+				ptx::mbar_arrive(ptx::smem_u32(&sh->f_full[n % T::FACTS]));
 			}
-		}
-		if (VALUES) {
-			odd = __any_sync(0xffffffffu, odd);
-			if (lane == 0)
-				sh->odd[slot][t >> 5] = odd;
-		} else {
-			ptx::mbar_arrive(ptx::smem_u32(&sh->f_full[n & 3u]));
-		}
-		ptx::fence_proxy_async_smem();
-		ptx::mbar_arrive(ptx::smem_u32(VALUES ? &sh->v_full[slot] : &sh->k_full[slot]));
-	}
-
-	__device__ __forceinline__ void run(const Waiter &wait)
-	{
-		uint64_t *free_bar = VALUES ? sh->v_free : sh->k_free;
-		Piece p, q;  // of the tile to be finished next, and of the one to be requested next
-		int pi = 0, qi = 0;
-		uint32_t asked = 0, done = 0, pn = 0, qn = 0;
-		bool more = next_with_tiles(q, qn, wait, false);
-		next_with_tiles(p, pn, wait, true);
-		while (done < asked || more) {
-			// the next request goes out as soon as its slot is free; until then what has come in is made ready
-			bool can = more && asked - done < 2;
-			if (can && asked >= 2) {
-				if (done < asked)
-					can = __all_sync(0xffffffffu, ptx::mbar_try_wait(ptx::smem_u32(&free_bar[asked & 1]), ((asked >> 1) & 1u) ^ 1u));
-				else
-					wait(free_bar[asked & 1], ((asked >> 1) & 1u) ^ 1u);
-			}
-			if (can) {
-				__syncwarp();
-				issue(q, q.unit0 + qi, asked);
-				asked++;
-				if (++qi == q.n_tiles) {
-					qi = 0;
-					qn++;
-					more = next_with_tiles(q, qn, wait, false);
-				}
-				if (asked - done < 2 && more)
-					continue;
-			}
-			if (asked - done == 2)
-				ptx::cp_async_wait<1>();
-			else
-				ptx::cp_async_wait<0>();
-			finish(p, p.unit0 + pi, done);
-			done++;
-			if (++pi == p.n_tiles) {
-				pi = 0;
-				drop_piece(sh, pn++, lane);
-				next_with_tiles(p, pn, wait, true);
-			}
+			ptx::fence_proxy_async_smem();
+			ptx::mbar_arrive(ptx::smem_u32(VALUES ? &sh->v_full[slot] : &sh->k_full[slot]));
 		}
 	}
-	// Piece n, or the next behind it that has tiles; drop: gives those without back.
-	__device__ __forceinline__ bool next_with_tiles(Piece &p, uint32_t &n, const Waiter &wait, bool drop)
-	{
-		for (;; n++) {
-			p = take_piece(sh, wait, n);
-			if (p.s < 0)
-				return false;
-			if (p.n_tiles > 0)
-				return true;
-			if (drop)
-				drop_piece(sh, n, lane);
-		}
-	}
-};
+}
 
 template <int KIND, int D>
-__global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const StepView st, const AttnArgs a)
+__global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const StepView st, const AttnArgs a, const __grid_constant__ CUtensorMap k_map,
+						     const __grid_constant__ CUtensorMap v_map)
 {
 	using T = Tile<KIND, D>;
 	constexpr int HALF = D / 2;
@@ -506,23 +448,29 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	__shared__ AttnWork work;
 	Shared *sh = &shared;
 	const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
-	const uint32_t k_ring = smem, v_ring = smem + 2 * T::BYTES, hand = smem + 4 * T::BYTES;
+	constexpr int TK = T::TK;
+	const uint32_t k_ring = smem, v_ring = k_ring + T::STAGES * T::BYTES, k_raw = v_ring + T::STAGES * T::BYTES, v_raw = k_raw + T::STAGES * T::RAW;
+	const uint32_t hand = v_raw + T::STAGES * T::RAW;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	if (threadIdx.x == 0) {
-		for (int i = 0; i < 2; i++) {
-			ptx::mbar_init(ptx::smem_u32(&sh->k_full[i]), LOAD_THREADS);
+		for (int i = 0; i < T::STAGES; i++) {
+			ptx::mbar_init(ptx::smem_u32(&sh->k_raw[i]), 1);
+			ptx::mbar_init(ptx::smem_u32(&sh->k_full[i]), MAKE_THREADS);
 			ptx::mbar_init(ptx::smem_u32(&sh->k_free[i]), 1);
-			ptx::mbar_init(ptx::smem_u32(&sh->v_full[i]), LOAD_THREADS);
+			ptx::mbar_init(ptx::smem_u32(&sh->v_raw[i]), 1);
+			ptx::mbar_init(ptx::smem_u32(&sh->v_full[i]), MAKE_THREADS);
 			ptx::mbar_init(ptx::smem_u32(&sh->v_free[i]), 1);
+		}
+		for (int i = 0; i < 2; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->s_full[i]), 1);
 			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS / 2);
 			ptx::mbar_init(ptx::smem_u32(&sh->o_full[i]), 1);
 		}
-		for (int i = 0; i < 4; i++)
-			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), LOAD_THREADS);
+		for (int i = 0; i < T::FACTS; i++)
+			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), T::SCALED ? MAKE_THREADS : 1);
 		for (int i = 0; i < PIECES; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->piece_full[i]), 1);
-			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), PIECE_READERS);
+			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), SOFT_THREADS / 32 + 1 + 2 + (T::SCALED ? 4 : 2));  // softmax, MMA, ask, make
 		}
 		ptx::mbar_init(ptx::smem_u32(&sh->o_free), SOFT_THREADS / 2);
 		ptx::mbar_init(ptx::smem_u32(&sh->q_full), SOFT_THREADS);
@@ -577,15 +525,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				row_scale = fabsf(a.scale_log2e) * __uint_as_float((uint32_t)e << 23);
 #pragma unroll
 				for (int c = 0; c < HALF / 32; c++) {
-					uint32_t hi[16], lo[16];
+					uint32_t out[T::PARTS][16];
 #pragma unroll
 					for (int i = 0; i < 8; i++) {
 						const float4 x = v[8 * c + i];
-						split2(make_float2(x.x * down, x.y * down), hi[2 * i], lo[2 * i]);
-						split2(make_float2(x.z * down, x.w * down), hi[2 * i + 1], lo[2 * i + 1]);
+						uint32_t part[T::PARTS];
+						split2<KIND>(make_float2(x.x * down, x.y * down), part);
+#pragma unroll
+						for (int k = 0; k < T::PARTS; k++)
+							out[k][2 * i] = part[k];
+						split2<KIND>(make_float2(x.z * down, x.w * down), part);
+#pragma unroll
+						for (int k = 0; k < T::PARTS; k++)
+							out[k][2 * i + 1] = part[k];
 					}
-					ptx::tmem_st16(lanes + COL_Q + wg * (HALF / 2) + 16 * c, hi);
-					ptx::tmem_st16(lanes + COL_Q + HALF + wg * (HALF / 2) + 16 * c, lo);
+#pragma unroll
+					for (int k = 0; k < T::PARTS; k++)
+						ptx::tmem_st16(lanes + T::COL_Q + k * HALF + wg * (HALF / 2) + 16 * c, out[k]);
 				}
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
@@ -608,14 +564,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			for (int i = 0; i < p.n_tiles; i++, tiles++) {
 				if ((int)(tiles & 1) != wg)
 					continue;
-				const int key0 = (p.unit0 + i) * TILE, slot = wg;  // (tile n has operand slot and warpgroup n & 1)
-				const uint32_t ph = (tiles >> 1) & 1u, S = lanes + COL_S + wg * TILE;
-				const uint32_t fslot = tiles & 3u;
-				wait(sh->f_full[fslot], (tiles >> 2) & 1u);
+				const int key0 = p.unit0 * ATTN_UNIT + i * TK;
+				const uint32_t ph = (tiles >> 1) & 1u, slot = tiles % T::STAGES, S = lanes + T::COL_S + wg * T::SLOT;
+				const uint32_t fslot = tiles % T::FACTS;
+				wait(sh->f_full[fslot], tiles / T::FACTS & 1u);
 				wait(sh->s_full[wg], ph);
 				ptx::tc_fence_after();
 				const uint32_t bad = sh->bad[fslot];
-				const bool masked = key0 + TILE > p.all_see || bad != 0;
+				const bool masked = key0 + TK > p.all_see || bad != 0;
 				// which of 32 keys this row sees
 				auto visible = [&](int c) {
 					const int key = key0 + 32 * c;
@@ -659,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				};
 				float top = -INFINITY;
 #pragma unroll 1
-				for (int c = 0; c < TILE / 32; c++) {
+				for (int c = 0; c < TK / 32; c++) {
 					float2 x[16];
 					scores(c, x);
 #pragma unroll
@@ -675,20 +631,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				bool odd = false;
 				float v_top = 1.0f;
 				if (T::SCALED || masked) {
-					wait(sh->v_full[slot], ph);
+					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
 					odd = sh->odd[slot][0] | sh->odd[slot][1];
 					if constexpr (T::SCALED)
 						v_top = sh->v_top[slot];
 				}
 				float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-				for (int c = 0; c < TILE / 32; c++) {
+				for (int c = 0; c < TK / 32; c++) {
 					float2 x[16];
 					scores(c, x);
-					// the parts of 16 keys take the columns of their scores: hi 8, lo 8
+					// the first two parts of 16 keys take the columns of their scores, 8 each; a third comes behind all of them
 #pragma unroll
 					for (int h = 0; h < 2; h++) {
-						uint32_t out[16];
+						uint32_t out[16], third[8];
 #pragma unroll
 						for (int k = 0; k < 8; k++) {
 							const float2 e = fma2(x[8 * h + k], make_float2(row_scale, row_scale), make_float2(base, base));
@@ -700,9 +656,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 								// (where a row does not see every key, a factor that is no number is nothing to it)
 								pk = masked ? make_float2(pk.x == 0.0f ? 0.0f : z.x, pk.y == 0.0f ? 0.0f : z.y) : z;
 							}
-							split2(pk, out[k], out[8 + k]);
+							uint32_t part[T::PARTS];
+							split2<KIND>(pk, part);
+							out[k] = part[0];
+							out[8 + k] = part[1];
+							if constexpr (T::PARTS == 3)
+								third[k] = part[2];
 						}
 						ptx::tmem_st16(S + 32 * c + 16 * h, out);
+						if constexpr (T::PARTS == 3)
+							ptx::tmem_st8(S + TK + 16 * c + 8 * h, third);
 					}
 				}
 				ptx::tmem_st_wait();
@@ -714,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 #pragma unroll
 				for (int c = 0; c < D / 32; c++) {
 					uint32_t v[32];
-					ptx::tmem_ld32(lanes + COL_O + 32 * c, v);
+					ptx::tmem_ld32(lanes + T::COL_O + 32 * c, v);
 					ptx::tmem_ld_wait();
 #pragma unroll
 					for (int k = 0; k < 16; k++) {
@@ -729,7 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
 				if (KIND != TIE_CUDA_KV_Q8 && odd) {  // infinities and NaN among values that not every row sees: p > 0 times them is what they are
 #pragma unroll 1
-					for (int k = 0; k < TILE; k++) {
+					for (int k = 0; k < TK; k++) {
 						if (key0 + k >= p.key_end)
 							break;
 						if (!(visible(k >> 5) >> (k & 31) & 1))
@@ -790,39 +753,37 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			}
 		}
 	} else if (warp < W_MMA) {
-		ptx::setmaxnreg_dec<LOAD_REGS>();
-		if (warp < W_VALUES) {
-			Loader<KIND, D, false> loader = {kv, st, sh, k_ring, (int)threadIdx.x - W_KEYS * 32, lane};
-			loader.run(wait);
-		} else {
-			Loader<KIND, D, true> loader = {kv, st, sh, v_ring, (int)threadIdx.x - W_VALUES * 32, lane};
-			loader.run(wait);
-		}
+		ptx::setmaxnreg_dec<MAKE_REGS>();
+		if (warp >= W_VALUES)
+			make<KIND, D, true>(sh, v_ring, v_raw, wait, (int)threadIdx.x - W_VALUES * 32, lane);
+		else if (T::SCALED)
+			make<KIND, D, false>(sh, k_ring, k_raw, wait, (int)threadIdx.x - W_KEYS * 32, lane);
 	} else {
-		ptx::setmaxnreg_dec<MMA_REGS>();
+		ptx::setmaxnreg_dec<REST_REGS>();
 		if (warp == W_MMA) {
 			if (ptx::elect_one()) {
-				constexpr uint32_t idesc_qk = ptx::umma_idesc_f16(ROWS, TILE);
-				constexpr uint32_t idesc_pv = ptx::umma_idesc_f16(ROWS, D) | 1u << 16;	// V: dims contiguous
+				constexpr uint32_t types = KIND == TIE_CUDA_KV_BF16 ? 1u << 7 | 1u << 10 : 0u;
+				constexpr uint32_t idesc_qk = ptx::umma_idesc_f16(ROWS, TK) | types;
+				constexpr uint32_t idesc_pv = ptx::umma_idesc_f16(ROWS, D) | types | 1u << 16;	// V: dims contiguous
 				uint32_t tiles = 0, pieces = 0;
-				// P V of tile n
-				auto products = [&](uint32_t n) {
-					const uint32_t slot = n & 1u, ph = (n >> 1) & 1u;
-					wait(sh->v_full[slot], ph);
-					wait(sh->p_full[slot], ph);
+				auto products = [&](uint32_t n) {  // P V of tile n
+					const uint32_t slot = n % T::STAGES;
+					wait(sh->v_full[slot], n / T::STAGES & 1u);
+					wait(sh->p_full[n & 1u], (n >> 1) & 1u);
 					const bool ok = n == 0 || wait(sh->o_free, (n - 1) & 1u);
 					ptx::tc_fence_after();
 					if (ok && !*wait.abort) {
 						// MN-major: 8 keys 1024 bytes apart, 64 dims a panel apart
-						const uint32_t b = ptx::umma_desc_lo(v_ring + slot * T::BYTES) | (PANEL >> 4) << 16, P = tmem + COL_S + slot * TILE;
+						const uint32_t b = ptx::umma_desc_lo(v_ring + slot * T::BYTES) | (T::PANEL >> 4) << 16, P = tmem + T::COL_S + (n & 1u) * T::SLOT;
 #pragma unroll
-						for (int part = 1; part >= 0; part--)
+						for (int part = T::PARTS - 1; part >= 0; part--)
 #pragma unroll
-							for (int k = 0; k < TILE / 16; k++)
-								ptx::mma_f16_ts(tmem + COL_O, P + 16 * k + 8 * part, b + k * (2048 >> 4), idesc_pv, part == 0 || k > 0);
+							for (int k = 0; k < TK / 16; k++)
+								ptx::mma_f16_ts(tmem + T::COL_O, P + (part < 2 ? 16 * k + 8 * part : TK + 8 * k), b + k * (2048 >> 4), idesc_pv,
+										part < T::PARTS - 1 || k > 0);
 					}
 					ptx::mma_commit(ptx::smem_u32(&sh->v_free[slot]));
-					ptx::mma_commit(ptx::smem_u32(&sh->o_full[slot]));
+					ptx::mma_commit(ptx::smem_u32(&sh->o_full[n & 1u]));
 				};
 				Piece p;
 				for (uint32_t n = 0;; n++) {
@@ -834,20 +795,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 						continue;
 					wait(sh->q_full, pieces & 1u);
 					for (int i = 0; i < p.n_tiles; i++, tiles++) {
-						const uint32_t slot = tiles & 1u, ph = (tiles >> 1) & 1u;
-						wait(sh->k_full[slot], ph);
+						const uint32_t slot = tiles % T::STAGES;
+						wait(T::SCALED ? sh->k_full[slot] : sh->k_raw[slot], tiles / T::STAGES & 1u);
 						ptx::tc_fence_after();
 						if (!*wait.abort) {
 							const uint32_t b = ptx::umma_desc_lo(k_ring + slot * T::BYTES);
 #pragma unroll
-							for (int part = 1; part >= 0; part--)
+							for (int part = T::PARTS - 1; part >= 0; part--)
 #pragma unroll
 								for (int k = 0; k < D / 16; k++)
-									ptx::mma_f16_ts(tmem + COL_S + slot * TILE, tmem + COL_Q + part * HALF + 8 * k,
-											b + (k >> 2) * (PANEL >> 4) + 2 * (k & 3), idesc_qk, part == 0 || k > 0);
+									ptx::mma_f16_ts(tmem + T::COL_S + (tiles & 1u) * T::SLOT, tmem + T::COL_Q + part * HALF + 8 * k,
+											b + (k >> 2) * (T::PANEL >> 4) + 2 * (k & 3), idesc_qk, part < T::PARTS - 1 || k > 0);
 						}
 						ptx::mma_commit(ptx::smem_u32(&sh->k_free[slot]));
-						ptx::mma_commit(ptx::smem_u32(&sh->s_full[slot]));
+						ptx::mma_commit(ptx::smem_u32(&sh->s_full[tiles & 1u]));
 						if (i > 0)
 							products(tiles - 1);
 					}
@@ -858,11 +819,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			}
 			__syncwarp();
 			wait(sh->fin, 0);
-		} else if (warp == W_PIECES && lane == 0) {
+		} else if (warp >= W_ASK) {
+			if (warp == W_ASK)
+				ask<KIND, D, false>(kv, st, sh, &k_map, k_ring, k_raw, wait, lane);
+			else
+				ask<KIND, D, true>(kv, st, sh, &v_map, v_ring, v_raw, wait, lane);
+		} else if (lane == 0) {
 			Piece p;
 			Walk walk_on = walk;
 			for (uint32_t n = 0;; n++) {
-				const bool any = next_piece(walk_on, p, work, kv, st, a);
+				const bool any = next_piece<T::TK>(walk_on, p, work, kv, st, a);
 				if (!any)
 					p.s = -1;
 				if (n >= PIECES)
@@ -912,22 +878,30 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_join(const KvView kv, const
 }
 
 template <int KIND, int D>
-constexpr size_t smem_bytes()
-{
-	return 4 * (size_t)Tile<KIND, D>::BYTES + (size_t)ROWS * D * 4 + 1024;
-}
-template <int KIND, int D>
 int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
-	attn_tiles<KIND, D><<<c->sm_count, THREADS, smem_bytes<KIND, D>(), c->stream>>>(kv, st, a);
+	using T = Tile<KIND, D>;
+	// boxes: the rows of a page, up to a tile's, x 128 bytes of each
+	const size_t rows = ((size_t)kv.n_pages * kv.n_head_kv) << kv.page_shift;
+	const unsigned box_rows = 1 << kv.page_shift < T::TK ? 1u << kv.page_shift : T::TK;
+	const size_t elem = T::SCALED ? 1 : 2;
+	const CUtensorMapDataType type = T::SCALED ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+	CUtensorMap map[2];
+	for (int i = 0; i < 2; i++) {
+		const int rc = tc_encode_2d(c, &map[i], type, elem, i ? kv.v : kv.k, rows, D, T::BOX_BYTES / elem, box_rows,
+					    T::RAW ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+		if (rc)
+			return rc;
+	}
+	attn_tiles<KIND, D><<<c->sm_count, THREADS, T::SMEM, c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
 	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / JOIN_ROWS), JOIN_THREADS, 0, kv, st, a, c->sm_count);
 }
 template <int KIND>
 int allow_smem(tie_cuda_ctx *c)
 {
-	TIE_CUDA_TRY(c, cudaFuncSetAttribute(attn_tiles<KIND, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<KIND, 128>()));
-	TIE_CUDA_TRY(c, cudaFuncSetAttribute(attn_tiles<KIND, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<KIND, 64>()));
+	TIE_CUDA_TRY(c, cudaFuncSetAttribute(attn_tiles<KIND, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<KIND, 128>::SMEM));
+	TIE_CUDA_TRY(c, cudaFuncSetAttribute(attn_tiles<KIND, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile<KIND, 64>::SMEM));
 	return TIE_CUDA_OK;
 }
 

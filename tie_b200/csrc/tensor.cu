@@ -1038,8 +1038,8 @@ static PFN_encodeTiled get_encode_fn()
 	return fn;
 }
 
-static int encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols,
-		     unsigned box_cols, unsigned box_rows, CUtensorMapSwizzle swz)
+int tc_encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols,
+		 unsigned box_cols, unsigned box_rows, CUtensorMapSwizzle swz)
 {
 	PFN_encodeTiled enc = get_encode_fn();
 	if (!enc) {
@@ -1115,7 +1115,7 @@ int tc_make_weight_map(tie_cuda_ctx *c, DevTensor &t, bool half_tiles, int n_exp
 	const int nb = t.k / QK_K;
 	const unsigned box_rows = half_tiles ? TC_BM / 2 : TC_BM;
 	if (t.kind == W_Q4K) {
-		int rc = encode_2d(c, &t.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, t.ptr, (size_t)t.rows * n_experts, (size_t)nb * Q4K_BYTES,
+		int rc = tc_encode_2d(c, &t.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, t.ptr, (size_t)t.rows * n_experts, (size_t)nb * Q4K_BYTES,
 				   Q4K_BYTES, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 		if (rc)
 			return rc;
