@@ -15,8 +15,8 @@
 #include <new>
 
 #include "common.cuh"
+#include "attn.cuh"
 #include "ep_dev.cuh"
-#include "kv_cache.cuh"
 #include "kernels.cuh"
 #include "copy_pool.h"
 
@@ -87,6 +87,7 @@ int alloc_scratch(tie_cuda_ctx *c)
 	TIE_CUDA_TRY(c, cudaMemset(s.route_counter, 0, (T + 3) / 4 * sizeof(int)));
 	TRY(dev_alloc(c, &s.attn_part, attn_scratch_floats(c)));
 	TRY(dev_alloc(c, &s.attn_count, c->sm_count));
+	TRY(dev_alloc(c, &s.attn_join, c->sm_count));
 	TIE_CUDA_TRY(c, cudaMemset(s.attn_count, 0, c->sm_count * sizeof(unsigned)));
 	TRY(dev_alloc(c, &s.dec_sync, 2));
 	TIE_CUDA_TRY(c, cudaMemset(s.dec_sync, 0, 2 * sizeof(unsigned)));
@@ -871,7 +872,7 @@ void tie_cuda_destroy(tie_cuda_ctx *c)
 	void *dev_ptrs[] = {s.x,     s.out_base, s.logits, s.bias,  s.topk_idx, s.topk_w, s.counts, s.offsets, s.tile_start, s.active, s.n_active,
 			    s.perm,  s.h,     s.y,	s.xs_hi, s.hs_hi,  s.row_expert, c->silu,  c->row_x,
 			    c->row_o, s.ep_counts, s.ep_offsets, s.ep_tile_start, s.ep_active, s.ep_n_active, s.ep_perm, s.ep_inv, s.inv,
-			    s.tile_info, s.xq, s.hq, s.dec_sync, c->df_table, s.sort_hist, s.route_counter, s.attn_part, s.attn_count};
+			    s.tile_info, s.xq, s.hq, s.dec_sync, c->df_table, s.sort_hist, s.route_counter, s.attn_part, s.attn_count, s.attn_join};
 	for (void *p : dev_ptrs)
 		if (p)
 			cudaFree(p);

@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 	const int n_cta = (int)min((long long)gridDim.x, total);  // (each of them has a unit at least)
 	if (cta >= n_cta)
 		return;
-	const long long u_begin = total * cta / n_cta, u_end = total * (cta + 1) / n_cta;
+	const long long u_begin = attn_div(total * cta, n_cta), u_end = attn_div(total * (cta + 1), n_cta);
 	const uint32_t stages = ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE;
 	Warp<KIND, D, NB> w;
 	for (long long u = u_begin; u < u_end;) {
@@ -426,10 +426,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 		const SeqView seq = kv_sequence(st, kv.page_shift, s);
 		const int n_keys = seq.kv_len + seq.n_tok, item_units = attn_units(seq);
 		const int tiles = (seq.n_tok * a.group + ROWS - 1) / ROWS;
-		const long long in_seq = u - work.start[s], item = in_seq / item_units;
+		const long long in_seq = u - work.start[s], item = attn_div(in_seq, item_units);
 		const int unit0 = (int)(in_seq - item * item_units);
 		const int unit1 = (int)min((long long)item_units, unit0 + (u_end - u));
-		const int head = (int)(item / tiles), row0 = (int)(item % tiles) * ROWS;
+		const int head = (int)attn_div(item, tiles), row0 = (int)(item - (long long)head * tiles) * ROWS;
 		// a tile's last row sees the furthest unless a tree says otherwise
 		const int last_tok = min((row0 + ROWS - 1) / a.group, seq.n_tok - 1);
 		const int key_end = st.tree ? n_keys : seq.kv_len + last_tok + 1;
@@ -622,7 +622,7 @@ int attn_setup(tie_cuda_ctx *c)
 
 int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale)
 {
-	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * ATTN_LOG2E, c->s.attn_part, c->s.attn_count};
+	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * ATTN_LOG2E, c->s.attn_part, c->s.attn_count, c->s.attn_join};
 	// rows of a sequence and key/value head, on average: up to 8 and up to 16 in tiles of that, more in tiles of 128
 	const long long rows = ((long long)st.n_tokens * a.group + st.n_seq - 1) / st.n_seq;
 	if (rows > 16)

@@ -10,6 +10,11 @@ constexpr float ATTN_LOG2E = 1.4426950408889634f;
 constexpr int ATTN_UNIT = 128;	       // keys: what an item's work is counted in
 constexpr int ATTN_MAX_ROWS = 128;     // query rows of a tile, at most
 
+// An item that begins in a CTA and goes on in others: parts, and the rows they are of (n_rows: of the sequence and head; 0: none).
+struct AttnJoin {
+	int n, tok0, head, row0, n_rows;
+};
+
 struct AttnArgs {
 	const float *q;
 	float *out;
@@ -17,6 +22,7 @@ struct AttnArgs {
 	float scale_log2e;
 	float *part;
 	unsigned *count;
+	AttnJoin *join;
 };
 
 // What a CTA leaves for a shared item of ROWS rows: [row][D] sums, then [row] maxima, then [row] sums of p.
@@ -37,7 +43,7 @@ struct AttnWork {
 
 __device__ __forceinline__ long long attn_items(const KvView &kv, const AttnArgs &a, const SeqView &q, int rows)
 {
-	return ((long long)q.n_tok * a.group + rows - 1) / rows * kv.n_head_kv;
+	return ((long long)q.n_tok * a.group + rows - 1) / rows * kv.n_head_kv;  // (rows: a constant)
 }
 __device__ __forceinline__ int attn_units(const SeqView &q)
 {
@@ -104,10 +110,16 @@ __device__ __forceinline__ int attn_sequence_of(const AttnWork &w, int n_seq, lo
 	return lo;
 }
 
+// a / b for a, b > 0: mostly of numbers that 32 bits hold, where it is several times as fast
+__device__ __forceinline__ long long attn_div(long long a, long long b)
+{
+	return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
+
 // The CTA that has unit u of `total`.
 __device__ __forceinline__ int attn_cta_of(long long u, long long total, int n_cta)
 {
-	return (int)(((u + 1) * n_cta - 1) / total);
+	return (int)attn_div((u + 1) * n_cta - 1, total);
 }
 
 // Row r of what the CTAs c0 .. c1 left of an item, joined by a warp: lane l gets values l, l + 32 .. of the finished row.

@@ -61,7 +61,7 @@ struct Shared {
 	float v_top[2], make_max[2][2];
 	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
 	float q_max[2][ROWS];
-	float2 ml[2][ROWS];
+	float2 ml[ROWS];
 	uint32_t tmem_base, abort;
 };
 
@@ -90,11 +90,11 @@ __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &wo
 		p.seq = kv_sequence(st, kv.page_shift, p.s);
 		const int tiles = (int)(((long long)p.seq.n_tok * a.group + ROWS - 1) / ROWS);
 		p.item_units = attn_units(p.seq);
-		const long long in_seq = w.u - work.start[p.s], item = in_seq / p.item_units;
+		const long long in_seq = w.u - work.start[p.s], item = attn_div(in_seq, p.item_units);
 		p.unit0 = (int)(in_seq - item * p.item_units);
 		p.unit1 = (int)min((long long)p.item_units, p.unit0 + (w.u_end - w.u));
-		p.head = (int)(item / tiles);
-		p.row0 = (int)(item % tiles) * ROWS;
+		p.head = (int)attn_div(item, tiles);
+		p.row0 = (int)(item - (long long)p.head * tiles) * ROWS;
 		w.u += p.unit1 - p.unit0;
 	} else {
 		// whole items, a sequence's last rows (the ones that see most) first, there and back over the CTAs
@@ -133,8 +133,8 @@ __device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, con
 		w.total = work.start[st.n_seq];
 		w.n_cta = (int)min((long long)n_cta, w.total);
 		if (cta < w.n_cta) {
-			w.u = w.total * cta / w.n_cta;
-			w.u_end = w.total * (cta + 1) / w.n_cta;
+			w.u = attn_div(w.total * cta, w.n_cta);
+			w.u_end = attn_div(w.total * (cta + 1), w.n_cta);
 		}
 	}
 	return w;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 						     const __grid_constant__ CUtensorMap v_map)
 {
 	using T = Tile<KIND, D>;
-	constexpr int HALF = D / 2;
+	constexpr int HALF = D / 2, D4 = D / 4, PER = 32 / D4;  // PER: rows a warp moves at once
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ Shared shared;
 	__shared__ AttnWork work;
@@ -505,16 +505,34 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const int n_rows = p.seq.n_tok * a.group, row = p.row0 + r;
 			const bool there = row < n_rows;
 			const int tok = there ? row / a.group : p.seq.n_tok - 1;
-			const int head = p.head * a.group + (there ? row - tok * a.group : 0);
-			const long long q_row = ((long long)(p.seq.tok0 + tok) * a.n_head + head) * D;
+			// float offset of query row `line` of the sequence and head, in q and in out
+			auto row_at = [&](int line) {
+				const int t = line / a.group;
+				return ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + (line - t * a.group)) * D;
+			};
+			// 4 dims of a row of the tile, in shared memory: no conflicts, neither along a row nor across the rows
+			auto spot = [&](int d4, int line) { return hand + ((uint32_t)d4 * ROWS + (line ^ (d4 & 7))) * 16; };
 			float row_scale = 0.0f;
-			if (p.n_tiles > 0) {  // this thread's half of the row, hi and lo, into tensor memory
-				float4 v[HALF / 4];
+			bar_sync<1, SOFT_THREADS>();  // shared memory has nothing of the piece before any more
+			if (p.n_tiles > 0) {
+				// The rows as they lie, through shared memory (a thread's own row from global memory: 32 lines a load), and this
+				// thread's half of its row, in parts, into tensor memory.  Loops stay loops here and below: what runs once a
+				// piece is bound by the fetch of its instructions (unrolled, this took 6600 cycles a piece).
+#pragma unroll 1
+				for (int i = 0; i < ROWS / 8 / PER; i++) {
+					const int line = warp * (ROWS / 8) + i * PER + lane / D4;
+					const bool in = p.row0 + line < n_rows;
+					cp_async16_or_zero(spot(lane % D4, line), a.q + (in ? row_at(p.row0 + line) + lane % D4 * 4 : 0), in);
+				}
+				ptx::cp_async_commit();
+				ptx::cp_async_wait<0>();
+				bar_sync<1, SOFT_THREADS>();
 				float top = 0.0f;
-#pragma unroll
+#pragma unroll 4
 				for (int i = 0; i < HALF / 4; i++) {
-					v[i] = there ? *reinterpret_cast<const float4 *>(a.q + q_row + wg * HALF + 4 * i) : make_float4(0, 0, 0, 0);
-					top = fmaxf(fmaxf(fmaxf(top, fabsf(v[i].x)), fmaxf(fabsf(v[i].y), fabsf(v[i].z))), fabsf(v[i].w));
+					const uint4 x = lds128(spot(wg * (HALF / 4) + i, r));
+					top = fmaxf(fmaxf(fmaxf(top, fabsf(__uint_as_float(x.x))), fmaxf(fabsf(__uint_as_float(x.y)), fabsf(__uint_as_float(x.z)))),
+						    fabsf(__uint_as_float(x.w)));
 				}
 				sh->q_max[wg][r] = top;
 				bar_sync<1, SOFT_THREADS>();
@@ -523,25 +541,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				const int e = top > 0.0f ? min(max((int)(__float_as_uint(top) >> 23), 1), 253) : 127;
 				const float down = copysignf(__uint_as_float((uint32_t)(254 - e) << 23), a.scale_log2e);
 				row_scale = fabsf(a.scale_log2e) * __uint_as_float((uint32_t)e << 23);
+#pragma unroll 1
+				for (int c = 0; c < HALF / 16; c++) {
+					uint32_t out[T::PARTS][8];
 #pragma unroll
-				for (int c = 0; c < HALF / 32; c++) {
-					uint32_t out[T::PARTS][16];
+					for (int i = 0; i < 4; i++) {
+						const uint4 x = lds128(spot(wg * (HALF / 4) + 4 * c + i, r));
+						uint32_t part[2][T::PARTS];
+						split2<KIND>(make_float2(__uint_as_float(x.x) * down, __uint_as_float(x.y) * down), part[0]);
+						split2<KIND>(make_float2(__uint_as_float(x.z) * down, __uint_as_float(x.w) * down), part[1]);
 #pragma unroll
-					for (int i = 0; i < 8; i++) {
-						const float4 x = v[8 * c + i];
-						uint32_t part[T::PARTS];
-						split2<KIND>(make_float2(x.x * down, x.y * down), part);
-#pragma unroll
-						for (int k = 0; k < T::PARTS; k++)
-							out[k][2 * i] = part[k];
-						split2<KIND>(make_float2(x.z * down, x.w * down), part);
-#pragma unroll
-						for (int k = 0; k < T::PARTS; k++)
-							out[k][2 * i + 1] = part[k];
+						for (int k = 0; k < T::PARTS; k++) {
+							out[k][2 * i] = part[0][k];
+							out[k][2 * i + 1] = part[1][k];
+						}
 					}
 #pragma unroll
 					for (int k = 0; k < T::PARTS; k++)
-						ptx::tmem_st16(lanes + T::COL_Q + k * HALF + wg * (HALF / 2) + 16 * c, out[k]);
+						ptx::tmem_st8(lanes + T::COL_Q + k * HALF + wg * (HALF / 2) + 8 * c, out[k]);
 				}
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
@@ -589,14 +606,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					return vis & ~((bad >> (2 * c) & 1 ? 0x0000ffffu : 0u) | (bad >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
 				};
 				// scores of 32 keys, times their rows' factors; -infinity where the row does not see
-				auto scores = [&](int c, float2 (&x)[16]) {
+				auto scores = [&](int c, float2 (&x)[16], bool scaled) {
 					uint32_t v[32];
 					ptx::tmem_ld32(S + 32 * c, v);
 					ptx::tmem_ld_wait();
 #pragma unroll
 					for (int k = 0; k < 16; k++)
 						x[k] = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
-					if constexpr (T::SCALED) {
+					if (T::SCALED && !scaled) {
 #pragma unroll
 						for (int k = 0; k < 16; k += 2) {
 							const float4 f = *reinterpret_cast<const float4 *>(&sh->k_scale[fslot][32 * c + 2 * k]);
@@ -604,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 							x[k + 1] = mul2(x[k + 1], make_float2(f.z, f.w));
 						}
 					}
-					if (masked) {
+					if (masked && !(T::SCALED && scaled)) {
 						const uint32_t vis = visible(c);
 #pragma unroll
 						for (int k = 0; k < 16; k++) {
@@ -617,11 +634,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 #pragma unroll 1
 				for (int c = 0; c < TK / 32; c++) {
 					float2 x[16];
-					scores(c, x);
+					scores(c, x, false);
 #pragma unroll
 					for (int k = 0; k < 16; k++)
 						top = fmaxf(top, fmaxf(x[k].x, x[k].y));
+					if constexpr (T::SCALED) {
+						// back with the factors in them: each read of those by all lanes costs the shared memory 512 cycles a tile
+#pragma unroll
+						for (int h = 0; h < 2; h++) {
+							uint32_t v[16];
+#pragma unroll
+							for (int k = 0; k < 8; k++) {
+								v[2 * k] = __float_as_uint(x[8 * h + k].x);
+								v[2 * k + 1] = __float_as_uint(x[8 * h + k].y);
+							}
+							ptx::tmem_st16(S + 32 * c + 16 * h, v);
+						}
+					}
 				}
+				if constexpr (T::SCALED)
+					ptx::tmem_st_wait();
 				top = fmaxf(m, top * row_scale);
 				const float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
 				const float alpha = m == -INFINITY ? 0.0f : exp2_ftz(m - top);
@@ -640,19 +672,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 #pragma unroll 1
 				for (int c = 0; c < TK / 32; c++) {
 					float2 x[16];
-					scores(c, x);
+					scores(c, x, true);
 					// the first two parts of 16 keys take the columns of their scores, 8 each; a third comes behind all of them
 #pragma unroll
 					for (int h = 0; h < 2; h++) {
 						uint32_t out[16], third[8];
+						float4 vs;
 #pragma unroll
 						for (int k = 0; k < 8; k++) {
 							const float2 e = fma2(x[8 * h + k], make_float2(row_scale, row_scale), make_float2(base, base));
 							float2 pk = make_float2(exp2_ftz(e.x), exp2_ftz(e.y));
 							sum = add2(sum, pk);
 							if constexpr (T::SCALED) {
-								const float2 f = *reinterpret_cast<const float2 *>(&sh->v_scale[slot][32 * c + 16 * h + 2 * k]);
-								const float2 z = mul2(pk, f);
+								if ((k & 1) == 0)
+									vs = *reinterpret_cast<const float4 *>(&sh->v_scale[slot][32 * c + 16 * h + 2 * k]);
+								const float2 z = mul2(pk, k & 1 ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
 								// (where a row does not see every key, a factor that is no number is nothing to it)
 								pk = masked ? make_float2(pk.x == 0.0f ? 0.0f : z.x, pk.y == 0.0f ? 0.0f : z.y) : z;
 							}
@@ -715,40 +749,52 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				}
 			}
 
-			// the two warpgroups' keys together: each finishes half of the dims
-			sh->ml[wg][r] = make_float2(m, l);
-			const uint32_t give = hand + (uint32_t)(wg ^ 1) * (ROWS * HALF * 4) + r * 16, take = hand + (uint32_t)wg * (ROWS * HALF * 4) + r * 16;
+			// the two warpgroups' keys together: the second's through shared memory to the first
+			if (wg == 1) {
+				sh->ml[r] = make_float2(m, l);
 #pragma unroll
-			for (int j = 0; j < HALF / 4; j++) {
-				const float2 x0 = wg ? acc[2 * j] : acc[HALF / 2 + 2 * j], x1 = wg ? acc[2 * j + 1] : acc[HALF / 2 + 2 * j + 1];
-				const uint4 x = make_uint4(__float_as_uint(x0.x), __float_as_uint(x0.y), __float_as_uint(x1.x), __float_as_uint(x1.y));
-				sts128(give + j * (ROWS * 16), x);
+				for (int j = 0; j < D4; j++)
+					sts128(spot(j, r), make_uint4(__float_as_uint(acc[2 * j].x), __float_as_uint(acc[2 * j].y), __float_as_uint(acc[2 * j + 1].x),
+								      __float_as_uint(acc[2 * j + 1].y)));
 			}
 			bar_sync<1, SOFT_THREADS>();
-			const float2 other = sh->ml[wg ^ 1][r];
-			const float top = fmaxf(m, other.x);
-			const float f_own = m == -INFINITY ? 0.0f : exp2f(m - top), f_other = other.x == -INFINITY ? 0.0f : exp2f(other.x - top);
-			const float sum = l * f_own + other.y * f_other;
 			const bool whole = p.unit0 == 0 && p.unit1 == p.item_units;
-			const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 			float *part = a.part + (2 * blockIdx.x + (p.unit0 == 0 ? 1 : 0)) * attn_part_floats(ROWS);
-			float *dst = whole ? a.out + q_row + wg * HALF : part + r * D + wg * HALF;
-			if (!whole || there) {
-#pragma unroll
-				for (int j = 0; j < HALF / 4; j++) {
-					const uint4 x = lds128(take + j * (ROWS * 16));
-					const float2 m0 = wg ? acc[HALF / 2 + 2 * j] : acc[2 * j], m1 = wg ? acc[HALF / 2 + 2 * j + 1] : acc[2 * j + 1];
-					// (a warpgroup whose keys the row does not see has nothing to give)
-					auto join = [&](float mine, uint32_t others) {
-						return ((f_own == 0.0f ? 0.0f : mine * f_own) + (f_other == 0.0f ? 0.0f : __uint_as_float(others) * f_other)) * inv;
-					};
-					*reinterpret_cast<float4 *>(dst + 4 * j) = make_float4(join(m0.x, x.x), join(m0.y, x.y), join(m1.x, x.z), join(m1.y, x.w));
-				}
-			}
-			if (!whole) {
-				if (wg == 0) {
+			if (wg == 0) {
+				const float2 other = sh->ml[r];
+				const float top = fmaxf(m, other.x);
+				// (a warpgroup whose keys the row does not see has sums of zero)
+				float own = m == -INFINITY ? 0.0f : exp2_ftz(m - top), theirs = other.x == -INFINITY ? 0.0f : exp2_ftz(other.x - top);
+				const float sum = l * own + other.y * theirs;
+				if (whole) {
+					const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+					own *= inv;
+					theirs *= inv;
+				} else {
 					part[ROWS * 128 + r] = top;
 					part[ROWS * 128 + ROWS + r] = sum;
+				}
+				const float2 f = make_float2(own, own), g = make_float2(theirs, theirs);
+#pragma unroll
+				for (int j = 0; j < D4; j++) {
+					const uint4 x = lds128(spot(j, r));
+					const float2 y0 = fma2(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), g, mul2(acc[2 * j], f));
+					const float2 y1 = fma2(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), g, mul2(acc[2 * j + 1], f));
+					const uint4 y = make_uint4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y));
+					if (whole)
+						sts128(spot(j, r), y);
+					else
+						reinterpret_cast<uint4 *>(part)[j * ROWS + r] = y;  // [4 dims][row]
+				}
+			}
+			if (whole) {
+				bar_sync<1, SOFT_THREADS>();
+#pragma unroll 4
+				for (int i = 0; i < ROWS / 8 / PER; i++) {
+					const int line = warp * (ROWS / 8) + i * PER + lane / D4;
+					const uint4 y = lds128(spot(lane % D4, line));
+					if (p.row0 + line < n_rows)
+						reinterpret_cast<uint4 *>(a.out + row_at(p.row0 + line))[lane % D4] = y;
 				}
 			}
 		}
@@ -829,8 +875,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			Walk walk_on = walk;
 			for (uint32_t n = 0;; n++) {
 				const bool any = next_piece<T::TK>(walk_on, p, work, kv, st, a);
-				if (!any)
+				if (!any) {
+					// the last piece's item goes on in other CTAs: its join
+					AttnJoin join = {0, 0, 0, 0, 0};
+					if (n > 0 && walk.shared && p.unit0 == 0 && p.unit1 < p.item_units) {
+						const long long i0 = walk_on.u - p.unit1;
+						join = {attn_cta_of(i0 + p.item_units - 1, walk.total, walk.n_cta) - (int)blockIdx.x + 1, p.seq.tok0, p.head, p.row0, p.seq.n_tok * a.group};
+					}
+					a.join[blockIdx.x] = join;
 					p.s = -1;
+				}
 				if (n >= PIECES)
 					wait(sh->piece_free[n % PIECES], (n / PIECES & 1u) ^ 1u, true);
 				sh->piece[n % PIECES] = p;
@@ -849,32 +903,69 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	}
 }
 
-// The parts that CTAs left of the items they shared, joined: CTA (c, i) takes 16 rows of the item that began in CTA c and
-// went on behind it, if there is one.  A launch of its own: an item of a few tiles of keys a CTA has tens of parts of
-// 66 KB, and one CTA, the last at the item, took 130 us to add them up (tree of 13 tokens over 9001 slots: 172 us).
-constexpr int JOIN_THREADS = 256, JOIN_ROWS = 16;
+// The parts that CTAs left of the items they shared, joined: CTA (c, i) takes 32 rows x 32 dims of the item that began in CTA c
+// and went on behind it, if there is one; its warps take the parts in turn, a lane a row, and are joined in their order.  A
+// launch of its own: an item of a few tiles of keys a CTA has tens of parts of 66 KB, and one CTA, the last at the item,
+// took 130 us to add them up (tree of 13 tokens over 9001 slots: 172 us).
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
 template <int D>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_join(const KvView kv, const StepView st, const AttnArgs a, int n_cta)
+__global__ void __launch_bounds__(JOIN_THREADS) attn_join(const AttnArgs a)
 {
-	__shared__ AttnWork work;
+	__shared__ float s_m[JOIN_WARPS][32], s_l[JOIN_WARPS][32];
+	__shared__ float4 s_acc[JOIN_WARPS][8][32];
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
-	const Walk w = start_walk<JOIN_THREADS>(work, kv, st, a, n_cta, c0);
-	if (!w.shared || w.u >= w.u_end)
-		return;
-	const long long u = w.u_end - 1;
-	const int s = attn_sequence_of(work, st.n_seq, u);
-	const SeqView seq = kv_sequence(st, kv.page_shift, s);
-	const int units = attn_units(seq), tiles = (int)(((long long)seq.n_tok * a.group + ROWS - 1) / ROWS);
-	const long long item = (u - work.start[s]) / units, i0 = work.start[s] + item * units, i1 = i0 + units - 1;
-	if (i0 < w.u || i1 == u)
-		return;
-	const int c1 = attn_cta_of(i1, w.total, w.n_cta), head = (int)(item / tiles), row0 = (int)(item % tiles) * ROWS;
 	pdl_wait();
-	for (int i = blockIdx.y * JOIN_ROWS + warp; i < (blockIdx.y + 1) * JOIN_ROWS && row0 + i < seq.n_tok * a.group; i += JOIN_THREADS / 32) {
-		const int t = (row0 + i) / a.group;
-		attn_join_row<D, ROWS>(a.part, c0, c1, i, lane,
-				       a.out + ((long long)(seq.tok0 + t) * a.n_head + head * a.group + (row0 + i - t * a.group)) * D);
+	const AttnJoin it = a.join[c0];
+	const int n = it.n, first = (blockIdx.y & 3) * 32, r = first + lane, d40 = (blockIdx.y >> 2) * 8;
+	if (it.row0 + first >= it.n_rows)  // (none: no rows)
+		return;
+	constexpr size_t PART = attn_part_floats(ROWS);
+	float top = -INFINITY, sum = 0.0f;
+	float4 acc[8];
+#pragma unroll
+	for (int j = 0; j < 8; j++)
+		acc[j] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+	for (int i = warp; i < n; i += JOIN_WARPS) {
+		const float *part = a.part + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART;
+		float4 v[8];
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			v[j] = __ldcg(reinterpret_cast<const float4 *>(part) + (d40 + j) * ROWS + r);
+		const float m = __ldcg(part + ROWS * 128 + r), l = __ldcg(part + ROWS * 128 + ROWS + r), next = fmaxf(top, m);
+		const float f = m == -INFINITY ? 0.0f : exp2_ftz(m - next), g = top == -INFINITY ? 0.0f : exp2_ftz(top - next);
+		top = next;
+		sum = fmaf(l, f, sum * g);
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			acc[j] = make_float4(fmaf(v[j].x, f, acc[j].x * g), fmaf(v[j].y, f, acc[j].y * g), fmaf(v[j].z, f, acc[j].z * g), fmaf(v[j].w, f, acc[j].w * g));
 	}
+	s_m[warp][lane] = top;
+	s_l[warp][lane] = sum;
+#pragma unroll
+	for (int j = 0; j < 8; j++)
+		s_acc[warp][j][lane] = acc[j];
+	__syncthreads();
+	// a warp: 4 dims of the 32 rows
+	top = -INFINITY;
+#pragma unroll
+	for (int i = 0; i < JOIN_WARPS; i++)
+		top = fmaxf(top, s_m[i][lane]);
+	sum = 0.0f;
+	float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+	for (int i = 0; i < JOIN_WARPS; i++) {
+		const float f = s_m[i][lane] == -INFINITY ? 0.0f : exp2_ftz(s_m[i][lane] - top);
+		const float4 v = s_acc[i][warp][lane];
+		sum = fmaf(s_l[i][lane], f, sum);
+		y = make_float4(fmaf(v.x, f, y.x), fmaf(v.y, f, y.y), fmaf(v.z, f, y.z), fmaf(v.w, f, y.w));
+	}
+	if (it.row0 + r >= it.n_rows)
+		return;
+	const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+	const int t = (it.row0 + r) / a.group;
+	float *dst = a.out + ((long long)(it.tok0 + t) * a.n_head + it.head * a.group + (it.row0 + r - t * a.group)) * D;
+	reinterpret_cast<float4 *>(dst)[d40 + warp] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
 template <int KIND, int D>
@@ -895,7 +986,7 @@ int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 	}
 	attn_tiles<KIND, D><<<c->sm_count, THREADS, T::SMEM, c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
-	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / JOIN_ROWS), JOIN_THREADS, 0, kv, st, a, c->sm_count);
+	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / 32 * (D / 32)), JOIN_THREADS, 0, a);
 }
 template <int KIND>
 int allow_smem(tie_cuda_ctx *c)

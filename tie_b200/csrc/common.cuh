@@ -20,6 +20,7 @@ constexpr int MAX_TOP_K = 8;
 constexpr int TC_TOKEN_TILE = 64;  // rows of one expert per token tile of the tensor-core path (or 32: run_experts)
 constexpr int SILU_N = TIE_CUDA_SILU_TABLE_SIZE;
 constexpr int TC_MAX_PARTS = 8;	  // parts that a dense product's rows are split into, at most
+struct AttnJoin;
 constexpr int SORT_SLICE = 256;   // rows per CTA of the dispatch sort
 constexpr int OUT_PAD = 64;	  // floats in front of the output rows: the status word is the last of them
 constexpr int COPY_CHUNKS = 16;	  // pageable host batches are copied in at most this many chunks
@@ -108,6 +109,7 @@ struct Scratch {
 	// attention over the cache (attn.cu): what CTAs that share a row tile leave for the last of them
 	float *attn_part = nullptr;		    // [2 x CTAs][attn_part_floats]
 	unsigned *attn_count = nullptr;		    // [CTAs] of them that are done (zero at rest)
+	AttnJoin *attn_join = nullptr;	    // [CTAs] what attn_tc.cu's second launch has to join
 	unsigned *dec_sync = nullptr;		    // [2] arrivals and epoch of the one-kernel decode step's grid barriers
 	int *row_expert = nullptr;		    // [R] staging for expert_rows
 	// expert-parallel dispatch state (sort of this rank's rows over ALL experts)
