@@ -505,10 +505,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const int n_rows = p.seq.n_tok * a.group, row = p.row0 + r;
 			const bool there = row < n_rows;
 			const int tok = there ? row / a.group : p.seq.n_tok - 1;
-			// float offset of query row `line` of the sequence and head, in q and in out
-			auto row_at = [&](int line) {
-				const int t = line / a.group;
-				return ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + (line - t * a.group)) * D;
+			// This warp's rows of the tile (PER at once, D / 4 lanes a row): f(row of the tile, float offset in q and in out).
+			// The division by the group is done once: one per row made the loop over 16 rows take 6600 cycles.
+			auto my_rows = [&](auto f) {
+				int line = warp * (ROWS / 8) + lane / D4, t = (p.row0 + line) / a.group, g = p.row0 + line - t * a.group;
+#pragma unroll 4
+				for (int i = 0; i < ROWS / 8 / PER; i++, line += PER) {
+					f(line, ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + g) * D + lane % D4 * 4);
+#pragma unroll
+					for (int k = 0; k < PER; k++)
+						if (++g == a.group)
+							g = 0, t++;
+				}
 			};
 			// 4 dims of a row of the tile, in shared memory: no conflicts, neither along a row nor across the rows
 			auto spot = [&](int d4, int line) { return hand + ((uint32_t)d4 * ROWS + (line ^ (d4 & 7))) * 16; };
@@ -516,14 +524,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			bar_sync<1, SOFT_THREADS>();  // shared memory has nothing of the piece before any more
 			if (p.n_tiles > 0) {
 				// The rows as they lie, through shared memory (a thread's own row from global memory: 32 lines a load), and this
-				// thread's half of its row, in parts, into tensor memory.  Loops stay loops here and below: what runs once a
-				// piece is bound by the fetch of its instructions (unrolled, this took 6600 cycles a piece).
-#pragma unroll 1
-				for (int i = 0; i < ROWS / 8 / PER; i++) {
-					const int line = warp * (ROWS / 8) + i * PER + lane / D4;
+				// thread's half of its row, in parts, into tensor memory.
+				my_rows([&](int line, long long at) {
 					const bool in = p.row0 + line < n_rows;
-					cp_async16_or_zero(spot(lane % D4, line), a.q + (in ? row_at(p.row0 + line) + lane % D4 * 4 : 0), in);
-				}
+					cp_async16_or_zero(spot(lane % D4, line), a.q + (in ? at : 0), in);
+				});
 				ptx::cp_async_commit();
 				ptx::cp_async_wait<0>();
 				bar_sync<1, SOFT_THREADS>();
@@ -781,22 +786,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					const float2 y0 = fma2(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), g, mul2(acc[2 * j], f));
 					const float2 y1 = fma2(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), g, mul2(acc[2 * j + 1], f));
 					const uint4 y = make_uint4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y));
-					if (whole)
-						sts128(spot(j, r), y);
-					else
-						reinterpret_cast<uint4 *>(part)[j * ROWS + r] = y;  // [4 dims][row]
+					sts128(spot(j, r), y);
 				}
 			}
-			if (whole) {
-				bar_sync<1, SOFT_THREADS>();
-#pragma unroll 4
-				for (int i = 0; i < ROWS / 8 / PER; i++) {
-					const int line = warp * (ROWS / 8) + i * PER + lane / D4;
+			bar_sync<1, SOFT_THREADS>();
+			if (whole)
+				my_rows([&](int line, long long at) {
 					const uint4 y = lds128(spot(lane % D4, line));
 					if (p.row0 + line < n_rows)
-						reinterpret_cast<uint4 *>(a.out + row_at(p.row0 + line))[lane % D4] = y;
-				}
-			}
+						*reinterpret_cast<uint4 *>(a.out + at) = y;
+				});
+			else
+#pragma unroll 4
+				for (int j = wg; j < D4; j += 2)  // [4 dims][row]
+					reinterpret_cast<uint4 *>(part)[j * ROWS + r] = lds128(spot(j, r));
 		}
 	} else if (warp < W_MMA) {
 		ptx::setmaxnreg_dec<MAKE_REGS>();
