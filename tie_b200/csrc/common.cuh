@@ -227,6 +227,12 @@ struct tie_cuda_ctx {
 	// small per-call device buffers for the dispatch rows
 	float *row_x = nullptr, *row_o = nullptr;
 	size_t row_cap = 0;
+	// turns per position of a rotation's pairs, for the base and head size of the last call (kv_cache.cu)
+	struct RopeTurns {
+		float base = 0.0f;
+		int head_dim = 0;
+		double turns[64] = {0.0};
+	} rope;
 	std::mutex row_mutex;  // the dispatch rows may be called from several host threads at once
 	tie::EpState ep;
 };

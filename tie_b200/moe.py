@@ -177,14 +177,14 @@ def _ptr(a):
     """Address of a numpy array / torch tensor / int / None."""
     if a is None:
         return None
+    if hasattr(a, "data_ptr"):
+        assert a.is_contiguous()
+        return a.data_ptr()
     if isinstance(a, int):
         return a
     if isinstance(a, np.ndarray):
         assert a.flags["C_CONTIGUOUS"]
         return a.ctypes.data
-    if hasattr(a, "data_ptr"):
-        assert a.is_contiguous()
-        return a.data_ptr()
     raise TypeError(type(a))
 
 
@@ -234,9 +234,10 @@ def _rows_ptr(a, width: int):
     """Address and row stride (in elements) of a tensor of rows, each `width` contiguous elements; an int address has them one behind the other."""
     if isinstance(a, int):
         return a, width
-    inner = a.stride()[1:]
+    if a.is_contiguous():
+        return a.data_ptr(), width
     want = 1
-    for n, s in zip(reversed(a.shape[1:]), reversed(inner)):
+    for n, s in zip(reversed(a.shape[1:]), reversed(a.stride()[1:])):
         assert n == 1 or s == want, "the values of a token's row must be contiguous"
         want *= n
     return a.data_ptr(), a.stride(0) if a.shape[0] > 1 else max(width, a.stride(0))
