@@ -7,6 +7,7 @@
 #include <float.h>
 
 #include "attn.cuh"
+#include "decode_common.cuh"
 #include "kernels.cuh"
 #include "mma_dot.cuh"
 #include "tc_ptx.cuh"
@@ -15,22 +16,26 @@ namespace tie {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int GROUP = 16;	       // keys a warp takes at a time
-constexpr int UNIT = ATTN_UNIT;	       // one round of a CTA's warps
-constexpr int MAX_ROWS = 16;	       // query rows of a CTA's tile
-static_assert(UNIT == GROUP * WARPS, "a unit is a group of keys for each warp");
+constexpr int MAX_ROWS = 16;  // query rows of a CTA's tile
 
 template <int KIND, int D>
 struct Cfg {
-	static constexpr int ROW = KIND == TIE_CUDA_KV_Q8 ? D : 2 * D;	// bytes of a head row of the cache
-	static constexpr int CHUNKS = ROW / 16;
-	static constexpr int STAGE = 2 * GROUP * ROW + (KIND == TIE_CUDA_KV_Q8 ? 2 * GROUP * 4 : 0);
-	static constexpr int STAGES = STAGE > 4352 ? 3 : 4;
+	static constexpr bool Q8 = KIND == TIE_CUDA_KV_Q8;
+	static constexpr int ROW = Q8 ? D : 2 * D;  // bytes of a head row of the cache
+	static constexpr int GROUP = ROW == 256 ? 16 : 32;  // keys a warp takes at a time
+	static constexpr int HALVES = GROUP / 16;
+	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128, BOXES = ROW / BOX_BYTES;  // of a row, per TMA box
+	static constexpr int PANEL = GROUP * 128;	 // a box's bytes, where rows are wider than one
+	static constexpr int STAGE = 2 * GROUP * ROW, STAGES = STAGE > 4096 ? 3 : 6;
+	static constexpr int FACTORS = Q8 ? 2 * GROUP * 4 : 0;	// of a stage's keys, then of its values: behind all warps' stages
+	static_assert(STAGE % 1024 == 0, "the swizzle is by address");
 	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	// parts of an fp32 operand: 3 x 8 or 2 x 11 bits
-	// a 16-byte chunk's place in its row: eight consecutive keys' chunks of a column lie in eight different bank groups
+	// where TMA puts a 16-byte chunk of a row: eight consecutive keys' chunks of a column lie in eight different bank groups
 	__device__ static __forceinline__ int place(int row, int ch)
 	{
-		return row * ROW + ((ch ^ (CHUNKS == 4 ? (row >> 1) & 3 : row & 7)) << 4);
+		if (ROW == 64)
+			return row * 64 + ((ch ^ (row >> 1 & 3)) << 4);
+		return (ch >> 3) * PANEL + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
 	}
 };
 
@@ -86,17 +91,70 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PA
 	}
 }
 
+// What the warps of a CTA request from: TMA boxes of a group's rows in one page, and the factors of Q8's rows.
+template <int KIND, int D>
+struct Ring {
+	using C = Cfg<KIND, D>;
+	uint32_t stages, factors, bars;	 // this warp's, in shared memory
+	uint32_t asked = 0, taken = 0;
+	unsigned there = 0;  // per group in flight 2 bits, the oldest highest: which 16 keys have a page
+
+	__device__ __forceinline__ uint32_t slot(uint32_t n) const { return stages + n % C::STAGES * C::STAGE; }
+	__device__ __forceinline__ uint32_t factor(uint32_t n) const { return factors + n % C::STAGES * C::FACTORS; }
+	__device__ __forceinline__ uint32_t bar(uint32_t n) const { return bars + n % C::STAGES * 8; }
+
+	// The group whose first key is key0; page[h]: of its 16-key halves (the same where a page holds the group).
+	__device__ __forceinline__ void ask(const KvView &kv, const StepView &st, const CUtensorMap *k_map, const CUtensorMap *v_map, int key0, int key_end,
+					    const int (&page)[2], int head, int lane)
+	{
+		const int in_page = (1 << kv.page_shift) - 1;
+		const bool one = (1 << kv.page_shift) >= C::GROUP;
+		long long row[2];
+		unsigned ok = 0;
+#pragma unroll
+		for (int h = 0; h < C::HALVES; h++) {
+			const int key = key0 + 16 * h;
+			row[h] = key < key_end ? kv_page_row(kv, st, page[h], head) : -1;
+			ok |= (row[h] >= 0 ? 1u : 0u) << h;
+			row[h] += key & in_page;
+		}
+		there = there << 2 | ok;
+		if (lane == 0) {
+			const int rows = one ? ((ok & 1) ? C::GROUP : 0) : 16 * __popc(ok);
+			ptx::mbar_arrive_expect_tx(bar(asked), rows * (2 * C::ROW + (C::Q8 ? 8 : 0)));
+#pragma unroll
+			for (int h = 0; h < C::HALVES; h++) {
+				if (!(ok >> h & 1) || (h && one))
+					continue;
+				const uint32_t to = slot(asked), k_to = to + h * 16 * C::BOX_BYTES, v_to = k_to + C::GROUP * C::ROW;
+#pragma unroll
+				for (int b = 0; b < C::BOXES; b++) {
+					ptx::tma_load_2d(k_to + b * C::PANEL, k_map, bar(asked), b * 64, (int)row[h]);
+					ptx::tma_load_2d(v_to + b * C::PANEL, v_map, bar(asked), b * 64, (int)row[h]);
+				}
+				if constexpr (C::Q8) {
+					const uint32_t f = factor(asked) + 64 * h, bytes = one ? C::GROUP * 4 : 64;
+					bulk_g2s(f, kv.k_scale + row[h], bytes, bar(asked));
+					bulk_g2s(f + 4 * C::GROUP, kv.v_scale + row[h], bytes, bar(asked));
+				}
+			}
+		}
+		asked++;
+	}
+};
+
 // One warp's state over the groups of keys it takes: S^T = K Q^T and O^T = V^T P^T on m16n8k16, keys (then dims) on the
 // 16-row side, query rows on the 8-column side, so that a single token's 8 heads fill the columns.  A lane holds rows
 // 2c and 2c + 1 (c = lane % 4) of each block of 8.
 template <int KIND, int D, int NB>
 struct Warp {
 	using C = Cfg<KIND, D>;
-	static constexpr int KS = D / 16, MB = D / 16;
+	static constexpr int KS = D / 16, MB = D / 16, H = C::HALVES;
 	uint32_t q[NB][C::PARTS][KS][2];
 	float row_scale[NB][2];	 // scale * log2 e, and what the row's parts were divided by
-	float acc[NB][MB][4];
+	float acc[NB][MB][4];	 // Q8: in units of v_unit
 	float m[NB][2], l[NB][2];  // running maximum (of the whole column), sum (of this lane's keys)
+	float v_unit;		 // Q8: a power of two, of the largest value factor so far
 
 	__device__ __forceinline__ void begin(const AttnArgs &a, const SeqView &seq, int head_kv, int row0, int lane)
 	{
@@ -158,15 +216,19 @@ struct Warp {
 				for (int i = 0; i < 4; i++)
 					acc[nb][mb][i] = 0.0f;
 		}
+		v_unit = 0.0f;
 	}
 
-	// 16 keys from key0 on, in shared memory at `stage`; keys at or behind key_end, and all of them unless `there`, are nobody's.
-	__device__ __forceinline__ void group(const AttnArgs &a, const StepView &st, const SeqView &seq, uint32_t stage, int key0, int key_end, bool there, int row0, int lane)
+	// The group of keys from key0 on, in shared memory at `stage`; keys at or behind key_end, and 16 of them whose bit of `there`
+	// is not set, are nobody's.
+	__device__ __forceinline__ void group(const AttnArgs &a, const StepView &st, const SeqView &seq, uint32_t stage, uint32_t factors, int key0, int key_end, unsigned there, int row0,
+					      int lane)
 	{
 		const int g = lane >> 2, c = lane & 3;
-		const uint32_t ks = stage, vs = stage + GROUP * C::ROW;
-		float s[NB][4];
-		{
+		const uint32_t ks = stage, vs = stage + C::GROUP * C::ROW;
+		float s[H][NB][4];
+#pragma unroll
+		for (int h = 0; h < H; h++) {
 			float part[NB][C::PARTS][4];  // a chain each: the tensor cores cut every sum off
 #pragma unroll
 			for (int nb = 0; nb < NB; nb++)
@@ -175,24 +237,24 @@ struct Warp {
 #pragma unroll
 					for (int i = 0; i < 4; i++)
 						part[nb][p][i] = 0.0f;
-			const int krow = lane & 15, kch = lane >> 4;
+			const int krow = 16 * h + (lane & 15), kch = lane >> 4;
 #pragma unroll
-			for (int j = 0; j < (KIND == TIE_CUDA_KV_Q8 ? KS / 2 : KS); j++) {
+			for (int j = 0; j < (C::Q8 ? KS / 2 : KS); j++) {
 				uint32_t r[4];
 				ldsm4(r, ks + C::place(krow, 2 * j + kch));
-				if constexpr (KIND == TIE_CUDA_KV_Q8) {
+				if constexpr (C::Q8) {
 #pragma unroll
 					for (int i = 0; i < 4; i++)
 						r[i] ^= 0x80808080u;
 #pragma unroll
-					for (int h = 0; h < 2; h++) {
-						const uint32_t f[4] = {int8_pair<0x4140>(r[2 * h]), int8_pair<0x4140>(r[2 * h + 1]), int8_pair<0x4342>(r[2 * h]),
-								       int8_pair<0x4342>(r[2 * h + 1])};
+					for (int k = 0; k < 2; k++) {
+						const uint32_t f[4] = {int8_pair<0x4140>(r[2 * k]), int8_pair<0x4140>(r[2 * k + 1]), int8_pair<0x4342>(r[2 * k]),
+								       int8_pair<0x4342>(r[2 * k + 1])};
 #pragma unroll
 						for (int nb = 0; nb < NB; nb++)
 #pragma unroll
 							for (int p = 0; p < C::PARTS; p++)
-								mma<KIND>(part[nb][p], f, q[nb][p][2 * j + h][0], q[nb][p][2 * j + h][1]);
+								mma<KIND>(part[nb][p], f, q[nb][p][2 * j + k][0], q[nb][p][2 * j + k][1]);
 					}
 				} else {
 #pragma unroll
@@ -210,34 +272,46 @@ struct Warp {
 #pragma unroll
 					for (int p = C::PARTS - 2; p >= 0; p--)
 						v += part[nb][p][i];
-					s[nb][i] = v * row_scale[nb][i & 1];
+					s[h][nb][i] = v * row_scale[nb][i & 1];
 				}
 		}
-		float v_top = 1.0f, v_rel[2] = {1.0f, 1.0f};
-		if constexpr (KIND == TIE_CUDA_KV_Q8) {
-			float f[4];
+		float v_rel[H][2], unit_change = 1.0f;
+		if constexpr (C::Q8) {
+			float f[H][2], top = 0.0f;
 #pragma unroll
-			for (int i = 0; i < 2; i++) {
-				const uint32_t at = stage + 2 * GROUP * C::ROW + 4 * (g + 8 * i);
-				asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[i]) : "r"(at) : "memory");
-				asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[2 + i]) : "r"(at + 4 * GROUP) : "memory");
-				// (an infinite factor is as little a number as NaN, and NaN does not reach the group's largest)
-				f[2 + i] = fabsf(f[2 + i]) <= FLT_MAX ? f[2 + i] : __int_as_float(0x7fc00000);
+			for (int h = 0; h < H; h++)
+#pragma unroll
+				for (int i = 0; i < 2; i++) {
+					const int k = 16 * h + 8 * i + g;
+					const uint32_t at = factors + 4 * k;
+					float kf;
+					asm volatile("ld.shared.f32 %0, [%1];" : "=f"(kf) : "r"(at) : "memory");
+					asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[h][i]) : "r"(at + 4 * C::GROUP) : "memory");
+#pragma unroll
+					for (int nb = 0; nb < NB; nb++) {
+						s[h][nb][2 * i] *= kf;
+						s[h][nb][2 * i + 1] *= kf;
+					}
+					// (nobody's factor is none; an infinite one is as little a number as NaN, and NaN does not reach the largest)
+					f[h][i] = key0 + k < key_end && (there >> h & 1) ? f[h][i] : 0.0f;
+					f[h][i] = fabsf(f[h][i]) <= FLT_MAX ? f[h][i] : __int_as_float(0x7fc00000);
+					top = fmaxf(top, fabsf(f[h][i]));
+				}
+			// the unit: a power of two that no factor so far has reached the double of
+			const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(top)) & 0x7f800000u;
+			const float unit = __uint_as_float(min(max(e, 0x00800000u), 253u << 23));
+			if (unit > v_unit) {
+				unit_change = v_unit * __uint_as_float((254u << 23) - __float_as_uint(unit));
+				v_unit = unit;
 			}
+			const float inv = __uint_as_float((254u << 23) - __float_as_uint(v_unit));
 #pragma unroll
-			for (int nb = 0; nb < NB; nb++)
+			for (int h = 0; h < H; h++)
 #pragma unroll
-				for (int i = 0; i < 4; i++)
-					s[nb][i] *= f[i >> 1];
-			v_top = fmaxf(fabsf(f[2]), fabsf(f[3]));
-			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 4));
-			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 8));
-			v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 16));
-			v_top = v_top > 0.0f ? v_top : 1.0f;
-			v_rel[0] = f[2] / v_top;
-			v_rel[1] = f[3] / v_top;
+				for (int i = 0; i < 2; i++)
+					v_rel[h][i] = f[h][i] * inv;
 		}
-		const bool masked = !there || key0 + GROUP > min(seq.kv_len, key_end);
+		const bool masked = there != (1u << H) - 1u || key0 + C::GROUP > min(seq.kv_len, key_end);
 		if (masked) {
 #pragma unroll
 			for (int nb = 0; nb < NB; nb++)
@@ -248,57 +322,70 @@ struct Warp {
 					if (st.tree)
 						bits = st.tree[seq.tok0 + tok];
 #pragma unroll
-					for (int h = 0; h < 2; h++) {
-						const int key = key0 + g + 8 * h, j = key - seq.kv_len;
-						const bool sees = there && key < key_end && (j < 0 || (st.tree ? j < KV_MAX_TREE && (bits >> j & 1) : j <= tok));
-						if (!sees)
-							s[nb][2 * h + i] = -INFINITY;
-					}
+					for (int h = 0; h < H; h++)
+#pragma unroll
+						for (int k = 0; k < 2; k++) {
+							const int key = key0 + 16 * h + g + 8 * k, j = key - seq.kv_len;
+							const bool sees =
+								(there >> h & 1) && key < key_end && (j < 0 || (st.tree ? j < KV_MAX_TREE && (bits >> j & 1) : j <= tok));
+							if (!sees)
+								s[h][nb][2 * k + i] = -INFINITY;
+						}
 				}
 		}
-		uint32_t b[NB][C::PARTS][2];  // P^T as the second operand
+		uint32_t b[NB][H][C::PARTS][2];  // P^T as the second operand
 		float alpha[NB][2];
 #pragma unroll
 		for (int nb = 0; nb < NB; nb++) {
 			float base[2];
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
-				float top = fmaxf(s[nb][i], s[nb][2 + i]);
+				float top = m[nb][i];
+#pragma unroll
+				for (int h = 0; h < H; h++)
+					top = fmaxf(top, fmaxf(s[h][nb][i], s[h][nb][2 + i]));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-				top = fmaxf(top, m[nb][i]);
 				base[i] = (top == -INFINITY ? 0.0f : top) - ATTN_P_SHIFT;
-				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2f(m[nb][i] - top);
+				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2_ftz(m[nb][i] - top);
 				m[nb][i] = top;
+				l[nb][i] *= alpha[nb][i];
+				alpha[nb][i] *= unit_change;
 			}
 #pragma unroll
-			for (int i = 0; i < 4; i++)
-				s[nb][i] = exp2f(s[nb][i] - base[i & 1]);
-#pragma unroll
-			for (int i = 0; i < 2; i++)
-				l[nb][i] = fmaf(l[nb][i], alpha[nb][i], s[nb][i] + s[nb][2 + i]);
-			if constexpr (KIND == TIE_CUDA_KV_Q8) {
+			for (int h = 0; h < H; h++) {
 #pragma unroll
 				for (int i = 0; i < 4; i++)
-					s[nb][i] = s[nb][i] == 0.0f ? 0.0f : s[nb][i] * v_rel[i >> 1];
-			}
+					s[h][nb][i] = exp2_ftz(s[h][nb][i] - base[i & 1]);
 #pragma unroll
-			for (int h = 0; h < 2; h++) {
-				uint32_t part[C::PARTS];
-				split_pair<KIND>(s[nb][2 * h], s[nb][2 * h + 1], part);
+				for (int i = 0; i < 2; i++)
+					l[nb][i] += s[h][nb][i] + s[h][nb][2 + i];
+				if constexpr (C::Q8) {
 #pragma unroll
-				for (int p = 0; p < C::PARTS; p++)
-					b[nb][p][h] = transpose8x8(part[p]);
+					for (int i = 0; i < 4; i++) {
+						const float z = s[h][nb][i] * v_rel[h][i >> 1];
+						// (where a row does not see every key, a factor that is no number is nothing to it)
+						s[h][nb][i] = masked && s[h][nb][i] == 0.0f ? 0.0f : z;
+					}
+				}
+#pragma unroll
+				for (int k = 0; k < 2; k++) {
+					uint32_t part[C::PARTS];
+					split_pair<KIND>(s[h][nb][2 * k], s[h][nb][2 * k + 1], part);
+#pragma unroll
+					for (int p = 0; p < C::PARTS; p++)
+						b[nb][h][p][k] = transpose8x8(part[p]);
+				}
 			}
 		}
-		if constexpr (KIND != TIE_CUDA_KV_Q8) {
-			// 0 * infinity is not nothing: where a group that not every row sees holds a value that is no number, its products
-			// are made one by one
+		if constexpr (!C::Q8) {
+			// 0 * infinity is not nothing: where a group that not every row sees holds a value that is no number (or that nobody
+			// has written), its products are made one by one
 			bool odd = false;
 			if (masked) {
 				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
-				for (int i = lane; i < GROUP * C::ROW / 4; i += 32) {
+				for (int i = lane; i < C::GROUP * C::ROW / 4; i += 32) {
 					uint32_t w;
 					asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vs + 4 * i) : "memory");
 					odd = odd || nonfinite16(w, EXPONENT);
@@ -311,55 +398,52 @@ struct Warp {
 			}
 		}
 #pragma unroll
-		for (int mb = 0; mb < MB; mb++) {
-			uint32_t f[4];
-			if constexpr (KIND == TIE_CUDA_KV_Q8) {
-				if (mb & 1)
-					continue;
-				uint32_t r[4];	// (keys 0-7, 8-15) of 16 dims, then of the next 16; a unit of 16 bits is two neighbouring dims
-				ldsm4_trans(r, vs + C::place(lane & 15, mb + (lane >> 4)));
+		for (int mb = 0; mb < MB; mb += C::Q8 ? 2 : 1) {
+			uint32_t f[C::Q8 ? 2 : 1][H][4];
 #pragma unroll
-				for (int i = 0; i < 4; i++)
-					r[i] ^= 0x80808080u;
+			for (int h = 0; h < H; h++) {
+				if constexpr (C::Q8) {
+					uint32_t r[4];	// (keys 0-7, 8-15) of 16 dims, then of the next 16; a unit of 16 bits is two neighbouring dims
+					ldsm4_trans(r, vs + C::place(16 * h + (lane & 15), mb + (lane >> 4)));
 #pragma unroll
-				for (int h = 0; h < 2; h++) {
-					const uint32_t e[4] = {int8_pair<0x4240>(r[2 * h]), int8_pair<0x4341>(r[2 * h]), int8_pair<0x4240>(r[2 * h + 1]),
-							       int8_pair<0x4341>(r[2 * h + 1])};
-					fold(mb + h, e, b, alpha, v_top);
+					for (int i = 0; i < 4; i++)
+						r[i] ^= 0x80808080u;
+#pragma unroll
+					for (int k = 0; k < 2; k++) {
+						f[k][h][0] = int8_pair<0x4240>(r[2 * k]);
+						f[k][h][1] = int8_pair<0x4341>(r[2 * k]);
+						f[k][h][2] = int8_pair<0x4240>(r[2 * k + 1]);
+						f[k][h][3] = int8_pair<0x4341>(r[2 * k + 1]);
+					}
+				} else {
+					ldsm4_trans(f[0][h], vs + C::place(16 * h + (lane & 7) + 8 * (lane >> 4), 2 * mb + (lane >> 3 & 1)));
 				}
-			} else {
-				ldsm4_trans(f, vs + C::place((lane & 7) + 8 * (lane >> 4), 2 * mb + (lane >> 3 & 1)));
-				fold(mb, f, b, alpha, v_top);
 			}
-		}
-	}
-
-	// acc = acc * alpha + (the 16 keys' products, summed up from zero: lo parts first, one cut-off sum a part)
-	__device__ __forceinline__ void fold(int mb, const uint32_t (&f)[4], const uint32_t (&b)[NB][C::PARTS][2], const float (&alpha)[NB][2], float v_top)
-	{
+			// acc = acc * alpha + (the group's products, summed up from zero, lo parts first: the tensor cores cut sums off)
 #pragma unroll
-		for (int nb = 0; nb < NB; nb++) {
-			float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+			for (int k = 0; k < (C::Q8 ? 2 : 1); k++)
 #pragma unroll
-			for (int p = C::PARTS - 1; p >= 0; p--)
-				mma<KIND>(d, f, b[nb][p][0], b[nb][p][1]);
+				for (int nb = 0; nb < NB; nb++) {
+					float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-			for (int i = 0; i < 4; i++) {
-				if constexpr (KIND == TIE_CUDA_KV_Q8)
-					acc[nb][mb][i] = fmaf(d[i], v_top, acc[nb][mb][i] * alpha[nb][i & 1]);
-				else
-					acc[nb][mb][i] = fmaf(acc[nb][mb][i], alpha[nb][i & 1], d[i]);
-			}
+					for (int p = C::PARTS - 1; p >= 0; p--)
+#pragma unroll
+						for (int h = 0; h < H; h++)
+							mma<KIND>(d, f[k][h], b[nb][h][p][0], b[nb][h][p][1]);
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						acc[nb][mb + k][i] = fmaf(acc[nb][mb + k][i], alpha[nb][i & 1], d[i]);
+				}
 		}
 	}
 
 	// dim of acc[..][mb][i]
 	__device__ static __forceinline__ int dim(int mb, int i, int lane)
 	{
-		return KIND == TIE_CUDA_KV_Q8 ? 16 * mb + 2 * (lane >> 2) + (i >> 1) : 16 * mb + (lane >> 2) + 8 * (i >> 1);
+		return C::Q8 ? 16 * mb + 2 * (lane >> 2) + (i >> 1) : 16 * mb + (lane >> 2) + 8 * (i >> 1);
 	}
 
-	__device__ __forceinline__ void one_by_one(uint32_t vs, const float (&p)[NB][4], const float (&alpha)[NB][2], int lane)
+	__device__ __forceinline__ void one_by_one(uint32_t vs, const float (&p)[H][NB][4], const float (&alpha)[NB][2], int lane)
 	{
 #pragma unroll
 		for (int nb = 0; nb < NB; nb++)
@@ -369,13 +453,17 @@ struct Warp {
 				for (int i = 0; i < 4; i++)
 					acc[nb][mb][i] *= alpha[nb][i & 1];
 #pragma unroll 1
-		for (int k = 0; k < GROUP; k++) {
+		for (int k = 0; k < C::GROUP; k++) {
 			float pk[NB][2];
 #pragma unroll
 			for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-				for (int i = 0; i < 2; i++)
-					pk[nb][i] = __shfl_sync(0xffffffffu, k < 8 ? p[nb][i] : p[nb][2 + i], (k & 7) * 4 + (lane & 3));
+				for (int i = 0; i < 2; i++) {
+					float mine = k & 8 ? p[0][nb][2 + i] : p[0][nb][i];
+					if (H == 2 && k >= 16)
+						mine = k & 8 ? p[H - 1][nb][2 + i] : p[H - 1][nb][i];
+					pk[nb][i] = __shfl_sync(0xffffffffu, mine, (k & 7) * 4 + (lane & 3));
+				}
 #pragma unroll
 			for (int mb = 0; mb < MB; mb++)
 #pragma unroll
@@ -399,27 +487,36 @@ template <int KIND, int D, int NB>
 constexpr size_t smem_bytes()
 {
 	using C = Cfg<KIND, D>;
-	constexpr size_t stages = (size_t)WARPS * C::STAGES * C::STAGE, rows = (size_t)WARPS * 8 * NB * D * 4;
+	constexpr size_t stages = (size_t)WARPS * C::STAGES * (C::STAGE + C::FACTORS), rows = (size_t)WARPS * 8 * NB * D * 4;
 	return (stages > rows ? stages : rows) + 1024;
 }
 
 template <int KIND, int D, int NB>
-__global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const StepView st, const AttnArgs a)
+__global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const StepView st, const AttnArgs a, const __grid_constant__ CUtensorMap k_map,
+							const __grid_constant__ CUtensorMap v_map)
 {
 	using C = Cfg<KIND, D>;
-	constexpr int ROWS = 8 * NB;
+	constexpr int ROWS = 8 * NB, D4 = D / 4, UNIT_GROUPS = ATTN_UNIT / C::GROUP;
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ AttnWork work;
-	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS];
+	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS], s_unit[WARPS];
+	__shared__ uint64_t s_bar[WARPS][C::STAGES];
 	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+	Ring<KIND, D> ring = {ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE,
+			      ptx::smem_u32(smem) + WARPS * C::STAGES * C::STAGE + warp * C::STAGES * C::FACTORS, ptx::smem_u32(s_bar[warp])};
+	if (lane == 0) {
+		for (int i = 0; i < C::STAGES; i++)
+			ptx::mbar_init(ring.bars + 8 * i, 1);
+		ptx::fence_barrier_init();
+		ptx::fence_proxy_async_smem();
+	}
 	attn_share_work<THREADS>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
 	const long long total = work.start[st.n_seq];
 	const int n_cta = (int)min((long long)gridDim.x, total);  // (each of them has a unit at least)
 	if (cta >= n_cta)
 		return;
 	const long long u_begin = attn_div(total * cta, n_cta), u_end = attn_div(total * (cta + 1), n_cta);
-	const uint32_t stages = ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE;
 	Warp<KIND, D, NB> w;
 	for (long long u = u_begin; u < u_end;) {
 		const int s = attn_sequence_of(work, st.n_seq, u);
@@ -435,54 +532,37 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 		const int key_end = st.tree ? n_keys : seq.kv_len + last_tok + 1;
 		if (st.tree && seq.n_tok > KV_MAX_TREE && threadIdx.x == 0)
 			kv_report(st, ST_BAD_STEP);
-		const int g_first = unit0 * WARPS + warp, g_end = min(unit1 * WARPS, (key_end + GROUP - 1) / GROUP);
-		w.begin(a, seq, head, row0, lane);
+		const int g_first = unit0 * UNIT_GROUPS + warp, g_end = min(unit1 * UNIT_GROUPS, (key_end + C::GROUP - 1) / C::GROUP);
 		const int *pages = st.page_table + (long long)s * st.max_pages;
-		const int page_mask = (1 << kv.page_shift) - 1;
-		unsigned there = 0;  // a bit per group in flight, the oldest highest
-		auto fetch = [&](int g, int page, int slot) {
-			const int key0 = g * GROUP;
-			const long long first = g < g_end ? kv_page_row(kv, st, page, head) : -1;
-			there = there << 1 | (first >= 0);
-			if (g < g_end) {
-				const uint32_t dst = stages + slot * C::STAGE;
-				const long long row0 = max(first, 0ll) + (key0 & page_mask);
+		auto pages_of = [&](int g, int (&page)[2]) {
 #pragma unroll
-				for (int i = 0; i < GROUP * C::CHUNKS / 32; i++) {
-					const int r = (lane + 32 * i) / C::CHUNKS, ch = (lane + 32 * i) % C::CHUNKS;
-					const bool in = first >= 0 && key0 + r < key_end;
-					const long long at = in ? (row0 + r) * C::ROW + ch * 16 : 0;
-					cp_async16_or_zero(dst + C::place(r, ch), kv.k + at, in);
-					cp_async16_or_zero(dst + GROUP * C::ROW + C::place(r, ch), kv.v + at, in);
-				}
-				if constexpr (KIND == TIE_CUDA_KV_Q8) {
-					const bool in = first >= 0 && key0 + (lane & 15) < key_end;
-					cp_async4_or_zero(dst + 2 * GROUP * C::ROW + 4 * lane, (lane < 16 ? kv.k_scale : kv.v_scale) + (in ? row0 + (lane & 15) : 0), in);
-				}
-			}
-			ptx::cp_async_commit();
+			for (int h = 0; h < 2; h++)
+				page[h] = h < C::HALVES && g < g_end && g * C::GROUP + 16 * h < key_end ? pages[(g * C::GROUP + 16 * h) >> kv.page_shift] : 0;
 		};
-		auto page_of = [&](int g) { return g < g_end ? pages[g * GROUP >> kv.page_shift] : 0; };
-		int ahead[C::STAGES];
+		auto ask = [&](int g, const int (&page)[2]) {
+			if (g < g_end)
+				ring.ask(kv, st, &k_map, &v_map, g * C::GROUP, key_end, page, head, lane);
+			else
+				ring.there <<= 2;
+		};
+		int page[C::STAGES][2];
 #pragma unroll
 		for (int i = 0; i < C::STAGES; i++)
-			ahead[i] = page_of(g_first + i * WARPS);
+			pages_of(g_first + i * WARPS, page[i]);
 #pragma unroll
 		for (int i = 0; i < C::STAGES - 1; i++)
-			fetch(g_first + i * WARPS, ahead[i], i);
-		int next_page = ahead[C::STAGES - 1], slot = 0;
+			ask(g_first + i * WARPS, page[i]);
+		w.begin(a, seq, head, row0, lane);
 		for (int g = g_first; g < g_end; g += WARPS) {
 			const int behind = g + (C::STAGES - 1) * WARPS;
-			const int page = next_page;
-			next_page = page_of(behind + WARPS);
-			fetch(behind, page, slot == 0 ? C::STAGES - 1 : slot - 1);
-			ptx::cp_async_wait<C::STAGES - 1>();
+			const int now[2] = {page[C::STAGES - 1][0], page[C::STAGES - 1][1]};
+			pages_of(behind + WARPS, page[C::STAGES - 1]);
+			ask(behind, now);
+			dec_wait(ring.bar(ring.taken), st.status, ring.taken / C::STAGES & 1u);
+			w.group(a, st, seq, ring.slot(ring.taken), ring.factor(ring.taken), g * C::GROUP, key_end, ring.there >> (2 * (C::STAGES - 1)) & 3u, row0, lane);
+			ring.taken++;
 			__syncwarp();
-			w.group(a, st, seq, stages + slot * C::STAGE, g * GROUP, key_end, there >> (C::STAGES - 1) & 1, row0, lane);
-			__syncwarp();
-			slot = slot + 1 == C::STAGES ? 0 : slot + 1;
 		}
-		ptx::cp_async_wait<0>();
 
 		// the warps' keys together
 #pragma unroll
@@ -498,15 +578,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 					s_l[warp][nb * 8 + 2 * lane + i] = sum;
 				}
 			}
+		if (lane == 0)
+			s_unit[warp] = C::Q8 ? w.v_unit : 1.0f;
 		__syncthreads();  // (and nobody reads keys any more)
 		if (threadIdx.x < ROWS) {
 			const int r = threadIdx.x;
 			float top = -INFINITY, sum = 0.0f;
+#pragma unroll
 			for (int i = 0; i < WARPS; i++)
 				top = fmaxf(top, s_m[i][r]);
+#pragma unroll
 			for (int i = 0; i < WARPS; i++) {
-				const float f = s_m[i][r] == -INFINITY ? 0.0f : exp2f(s_m[i][r] - top);
-				s_w[r][i] = f;
+				const float f = s_m[i][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[i][r] - top);
+				s_w[r][i] = f * s_unit[i];
 				sum = fmaf(s_l[i][r], f, sum);
 			}
 			s_top[r] = top;
@@ -528,9 +612,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + head * a.group + (r - tok * a.group)) * D;
 		};
 		float *part = a.part + (2 * cta + (unit0 == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS);
-		for (int i = threadIdx.x; i < ROWS * D / 4; i += THREADS) {
-			const int r = i / (D / 4), col = i % (D / 4) * 4;
+		for (int i = threadIdx.x; i < ROWS * D4; i += THREADS) {
+			const int r = i / D4, col = i % D4 * 4;
 			float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll
 			for (int k = 0; k < WARPS; k++) {
 				const float f = s_w[r][k];
 				const float4 v = *reinterpret_cast<const float4 *>(rows + (k * ROWS + r) * D + col);
@@ -557,21 +642,82 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			}
 			// the CTAs of the item: those of its first and last unit, and all between
 			const long long i0 = work.start[s] + item * item_units, i1 = i0 + item_units - 1;
-			const int c0 = attn_cta_of(i0, total, n_cta), c1 = attn_cta_of(i1, total, n_cta);
+			const int c0 = attn_cta_of(i0, total, n_cta), c1 = attn_cta_of(i1, total, n_cta), n = c1 - c0 + 1;
 			__threadfence();
 			__syncthreads();
 			if (threadIdx.x == 0)
 				work.last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
 			__syncthreads();
 			if (work.last) {
+				// Joined in the order of the CTAs: warp w takes parts w, w + 8 .. of all rows (a lane 4 dims), then the warps' sums.
 				__threadfence();
-				for (int r = warp; r < ROWS && row0 + r < n_rows; r += WARPS)
-					attn_join_row<D, MAX_ROWS>(a.part, c0, c1, r, lane, out_row(row0 + r));
+				auto at = [&](int i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS); };
+				constexpr int PER = 32 / D4, STEPS = ROWS / PER;  // rows at once
+				float4 sum[STEPS];
+				float top[STEPS], l[STEPS];
+#pragma unroll
+				for (int k = 0; k < STEPS; k++) {
+					sum[k] = make_float4(0, 0, 0, 0);
+					top[k] = -INFINITY;
+					l[k] = 0.0f;
+				}
+				for (int i = warp; i < n; i += WARPS) {
+					const float *p = at(i);
+					float4 v[STEPS];
+					float pm[STEPS], pl[STEPS];
+#pragma unroll
+					for (int k = 0; k < STEPS; k++) {
+						const int r = k * PER + lane / D4;
+						v[k] = __ldcg(reinterpret_cast<const float4 *>(p + r * D) + lane % D4);
+						pm[k] = __ldcg(p + MAX_ROWS * 128 + r);
+						pl[k] = __ldcg(p + MAX_ROWS * 128 + MAX_ROWS + r);
+					}
+#pragma unroll
+					for (int k = 0; k < STEPS; k++) {
+						const float next = fmaxf(top[k], pm[k]);
+						const float f = pm[k] == -INFINITY ? 0.0f : exp2_ftz(pm[k] - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
+						top[k] = next;
+						l[k] = fmaf(pl[k], f, l[k] * o);
+						if (f != 0.0f)
+							sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
+									     fmaf(v[k].w, f, sum[k].w * o));
+					}
+				}
+#pragma unroll
+				for (int k = 0; k < STEPS; k++) {
+					const int r = k * PER + lane / D4;
+					*reinterpret_cast<float4 *>(rows + (warp * ROWS + r) * D + lane % D4 * 4) = sum[k];
+					if (lane % D4 == 0) {
+						s_m[warp][r] = top[k];
+						s_l[warp][r] = l[k];
+					}
+				}
+				__syncthreads();
+				for (int i = threadIdx.x; i < ROWS * D4; i += THREADS) {
+					const int r = i / D4, col = i % D4 * 4;
+					if (row0 + r >= n_rows)
+						break;
+					float t = -INFINITY, all = 0.0f;
+					float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+					for (int k = 0; k < WARPS; k++)
+						t = fmaxf(t, s_m[k][r]);
+#pragma unroll
+					for (int k = 0; k < WARPS; k++) {
+						const float f = s_m[k][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[k][r] - t);
+						const float4 v = *reinterpret_cast<const float4 *>(rows + (k * ROWS + r) * D + col);
+						all = fmaf(s_l[k][r], f, all);
+						y = make_float4(fmaf(v.x, f, y.x), fmaf(v.y, f, y.y), fmaf(v.z, f, y.z), fmaf(v.w, f, y.w));
+					}
+					const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+					*reinterpret_cast<float4 *>(out_row(row0 + r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+				}
 				if (threadIdx.x == 0)
 					a.count[c0] = 0;  // at rest again
 			}
 		}
-		__syncthreads();  // shared memory is the next item's
+		ptx::fence_proxy_async_smem();	// the next item's boxes land where these rows were
+		__syncthreads();
 		u += unit1 - unit0;
 	}
 }
@@ -579,7 +725,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 template <int KIND, int D, int NB>
 int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
-	attn_rows<KIND, D, NB><<<c->sm_count, THREADS, smem_bytes<KIND, D, NB>(), c->stream>>>(kv, st, a);
+	using C = Cfg<KIND, D>;
+	CUtensorMap map[2];
+	const int rc = attn_maps(c, kv, C::Q8 ? 1 : 2, D, C::BOX_BYTES, C::GROUP, C::ROW == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, map);
+	if (rc)
+		return rc;
+	attn_rows<KIND, D, NB><<<c->sm_count, THREADS, smem_bytes<KIND, D, NB>(), c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
 	return TIE_CUDA_OK;
 }
@@ -606,6 +757,16 @@ int go_kind(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int head_dim,
 }
 
 }  // namespace
+
+// Maps of keys and values for boxes of up to box_rows rows of a page x box_bytes.
+int attn_maps(tie_cuda_ctx *c, const KvView &kv, int elem, int head_dim, int box_bytes, int box_rows, CUtensorMapSwizzle swizzle, CUtensorMap *map)
+{
+	const size_t rows = ((size_t)kv.n_pages * kv.n_head_kv) << kv.page_shift;
+	const int n = 1 << kv.page_shift < box_rows ? 1 << kv.page_shift : box_rows;
+	const CUtensorMapDataType type = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+	const int rc = tc_encode_2d(c, &map[0], type, elem, kv.k, rows, head_dim, box_bytes / elem, n, swizzle);
+	return rc ? rc : tc_encode_2d(c, &map[1], type, elem, kv.v, rows, head_dim, box_bytes / elem, n, swizzle);
+}
 
 size_t attn_scratch_floats(const tie_cuda_ctx *c)
 {

@@ -122,57 +122,18 @@ __device__ __forceinline__ int attn_cta_of(long long u, long long total, int n_c
 	return (int)attn_div((u + 1) * n_cta - 1, total);
 }
 
-// Row r of what the CTAs c0 .. c1 left of an item, joined by a warp: lane l gets values l, l + 32 .. of the finished row.
-template <int D, int ROWS>
-__device__ __forceinline__ void attn_join_row(const float *parts, int c0, int c1, int r, int lane, float *dst)
+// 2^x to 2^-22, results below 2^-126 zero
+__device__ __forceinline__ float exp2_ftz(float x)
 {
-	constexpr size_t PART = attn_part_floats(ROWS);
-	auto at = [&](int i) { return parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART; };
-	const int n = c1 - c0 + 1;
-	float top = -INFINITY, sum = 0.0f;
-	for (int i = lane; i < n; i += 32)
-		top = fmaxf(top, __ldcg(at(i) + ROWS * 128 + r));
-#pragma unroll
-	for (int o = 16; o; o >>= 1)
-		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-	float acc[D / 32];
-#pragma unroll
-	for (int j = 0; j < D / 32; j++)
-		acc[j] = 0.0f;
-	for (int b = 0; b < n; b += 32) {
-		float f = 0.0f, li = 0.0f;
-		if (b + lane < n) {
-			const float mi = __ldcg(at(b + lane) + ROWS * 128 + r);
-			f = mi == -INFINITY ? 0.0f : exp2f(mi - top);
-			li = __ldcg(at(b + lane) + ROWS * 128 + ROWS + r) * f;
-		}
-#pragma unroll 8
-		for (int i = 0; i < min(32, n - b); i++) {
-			const float fi = __shfl_sync(0xffffffffu, f, i);
-			sum += __shfl_sync(0xffffffffu, li, i);
-			if (fi != 0.0f) {
-				const float *src = at(b + i) + r * D + lane;
-#pragma unroll
-				for (int j = 0; j < D / 32; j++)
-					acc[j] = fmaf(__ldcg(src + 32 * j), fi, acc[j]);
-			}
-		}
-	}
-	const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-	for (int j = 0; j < D / 32; j++)
-		dst[lane + 32 * j] = acc[j] * inv;
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
 }
 
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool there)
 {
 	const int n = there ? 16 : 0;
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void *src, bool there)
-{
-	const int n = there ? 4 : 0;
-	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exponent)
 {
@@ -188,6 +149,7 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t x_biased)
 	return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+int attn_maps(tie_cuda_ctx *c, const KvView &kv, int elem, int head_dim, int box_bytes, int box_rows, CUtensorMapSwizzle swizzle, CUtensorMap *map);
 // attn_tc.cu: tiles of 128 rows on tcgen05
 int attn_tc_setup(tie_cuda_ctx *c);
 int launch_attn_tc(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const AttnArgs &a);

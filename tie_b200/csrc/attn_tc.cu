@@ -239,14 +239,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
 	return r;
 }
-// 2^x to 2^-22, results below 2^-126 zero
-__device__ __forceinline__ float exp2_ftz(float x)
-{
-	float r;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-	return r;
-}
-
 // The 16-bit parts of a pair, the largest first: fp16 hi and lo, or three of bf16.
 template <int KIND, int PARTS>
 __device__ __forceinline__ void split2(float2 x, uint32_t (&part)[PARTS])
@@ -975,18 +967,10 @@ template <int KIND, int D>
 int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
 	using T = Tile<KIND, D>;
-	// boxes: the rows of a page, up to a tile's, x 128 bytes of each
-	const size_t rows = ((size_t)kv.n_pages * kv.n_head_kv) << kv.page_shift;
-	const unsigned box_rows = 1 << kv.page_shift < T::TK ? 1u << kv.page_shift : T::TK;
-	const size_t elem = T::SCALED ? 1 : 2;
-	const CUtensorMapDataType type = T::SCALED ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
 	CUtensorMap map[2];
-	for (int i = 0; i < 2; i++) {
-		const int rc = tc_encode_2d(c, &map[i], type, elem, i ? kv.v : kv.k, rows, D, T::BOX_BYTES / elem, box_rows,
-					    T::RAW ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
-		if (rc)
-			return rc;
-	}
+	const int rc = attn_maps(c, kv, T::SCALED ? 1 : 2, D, T::BOX_BYTES, T::TK, T::RAW ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, map);
+	if (rc)
+		return rc;
 	attn_tiles<KIND, D><<<c->sm_count, THREADS, T::SMEM, c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
 	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / 32 * (D / 32)), JOIN_THREADS, 0, a);
