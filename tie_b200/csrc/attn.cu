@@ -15,7 +15,8 @@
 namespace tie {
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int WARPS = 8, WORKERS = 32 * WARPS;	// warps and threads that work on keys
+constexpr int ASKERS = 4, EACH = WARPS / ASKERS, THREADS = WORKERS + 32 * ASKERS;  // warps that request keys and values for them
 constexpr int MAX_ROWS = 16;  // query rows of a CTA's tile
 
 template <int KIND, int D>
@@ -24,12 +25,14 @@ struct Cfg {
 	static constexpr int ROW = Q8 ? D : 2 * D;  // bytes of a head row of the cache
 	static constexpr int GROUP = ROW == 256 ? 16 : 32;  // keys a warp takes at a time
 	static constexpr int HALVES = GROUP / 16;
-	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128, BOXES = ROW / BOX_BYTES;  // of a row, per TMA box
-	static constexpr int PANEL = GROUP * 128;	 // a box's bytes, where rows are wider than one
+	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128;	// of a row, side by side in a TMA box; what is further comes behind: [64 dims][row]
+	static constexpr int PANEL = GROUP * 128;
+	static_assert(ROW <= 128 || HALVES == 1, "a box is a group's rows");
 	static constexpr int STAGE = 2 * GROUP * ROW, STAGES = STAGE > 4096 ? 3 : 6;
 	static constexpr int FACTORS = Q8 ? 2 * GROUP * 4 : 0;	// of a stage's keys, then of its values: behind all warps' stages
 	static_assert(STAGE % 1024 == 0, "the swizzle is by address");
-	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	// parts of an fp32 operand: 3 x 8 or 2 x 11 bits
+	// parts of an fp32 operand: bf16 3 x 8 bits, fp16 2 x 11; Q8's queries are 3 bytes (whole numbers of 24 bits, sums exact)
+	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2, Q_PARTS = Q8 ? 3 : PARTS, Q_STEP = Q8 ? 32 : 16;
 	// where TMA puts a 16-byte chunk of a row: eight consecutive keys' chunks of a column lie in eight different bank groups
 	__device__ static __forceinline__ int place(int row, int ch)
 	{
@@ -39,6 +42,10 @@ struct Cfg {
 	}
 };
 
+__device__ __forceinline__ void workers_sync()
+{
+	asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory");
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
 {
 	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -71,6 +78,13 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 		mma_16816(c, a[0], a[1], a[2], a[3], b0, b1);
 }
 
+__device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+	asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+	    : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+	    : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // (a, b) as PARTS pairs of 16-bit parts, the largest first, that add up to them (to 22 bits in fp16, all 24 in bf16).
 template <int KIND, int PARTS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PARTS])
@@ -91,57 +105,97 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PA
 	}
 }
 
-// What the warps of a CTA request from: TMA boxes of a group's rows in one page, and the factors of Q8's rows.
+// The groups in flight of each worker warp.
 template <int KIND, int D>
 struct Ring {
 	using C = Cfg<KIND, D>;
-	uint32_t stages, factors, bars;	 // this warp's, in shared memory
-	uint32_t asked = 0, taken = 0;
-	unsigned there = 0;  // per group in flight 2 bits, the oldest highest: which 16 keys have a page
+	uint64_t full[WARPS][C::STAGES], empty[WARPS][C::STAGES];
+	unsigned there[WARPS][C::STAGES];  // which 16 keys of a group have a page
+};
 
-	__device__ __forceinline__ uint32_t slot(uint32_t n) const { return stages + n % C::STAGES * C::STAGE; }
-	__device__ __forceinline__ uint32_t factor(uint32_t n) const { return factors + n % C::STAGES * C::FACTORS; }
-	__device__ __forceinline__ uint32_t bar(uint32_t n) const { return bars + n % C::STAGES * 8; }
+// The pieces of work of a CTA, one after the other.
+struct Piece {
+	SeqView seq;
+	int s, head, row0, unit0, unit1, item_units, key_end;
+	long long first_unit;  // of the item
+};
+template <int ROWS>
+__device__ __forceinline__ Piece piece_at(long long u, long long u_end, const AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a)
+{
+	Piece p;
+	p.s = attn_sequence_of(work, st.n_seq, u);
+	p.seq = kv_sequence(st, kv.page_shift, p.s);
+	p.item_units = attn_units(p.seq);
+	const int tiles = (p.seq.n_tok * a.group + ROWS - 1) / ROWS;
+	const long long in_seq = u - work.start[p.s], item = attn_div(in_seq, p.item_units);
+	p.unit0 = (int)(in_seq - item * p.item_units);
+	p.unit1 = (int)min((long long)p.item_units, p.unit0 + (u_end - u));
+	p.first_unit = u - p.unit0;
+	p.head = (int)attn_div(item, tiles);
+	p.row0 = (int)(item - (long long)p.head * tiles) * ROWS;
+	// a tile's last row sees the furthest unless a tree says otherwise
+	p.key_end = p.seq.kv_len + (st.tree ? p.seq.n_tok : min((p.row0 + ROWS - 1) / a.group, p.seq.n_tok - 1) + 1);
+	return p;
+}
 
-	// The group whose first key is key0; page[h]: of its 16-key halves (the same where a page holds the group).
-	__device__ __forceinline__ void ask(const KvView &kv, const StepView &st, const CUtensorMap *k_map, const CUtensorMap *v_map, int key0, int key_end,
-					    const int (&page)[2], int head, int lane)
-	{
-		const int in_page = (1 << kv.page_shift) - 1;
-		const bool one = (1 << kv.page_shift) >= C::GROUP;
-		long long row[2];
-		unsigned ok = 0;
+// The last warps: a lane requests a worker's groups, a TMA box per page for keys and for values, as its slots get free, and runs
+// ahead of the workers into the next piece while they join the one before.  A request holds up the warp that makes it for about a
+// hundred cycles: each worker for itself, it was 900 a group of 32 keys; one warp for all eight, 80 us instead of 73 for 48
+// sequences of 5000.
+template <int KIND, int D, int ROWS>
+__device__ __forceinline__ void request(Ring<KIND, D> *ring, uint32_t stages, uint32_t factors, long long u, long long u_end, const AttnWork &work, const KvView &kv,
+					const StepView &st, const AttnArgs &a, const CUtensorMap *k_map, const CUtensorMap *v_map, int worker, bool mine)
+{
+	using C = Cfg<KIND, D>;
+	const int in_page = (1 << kv.page_shift) - 1;
+	const bool one = (1 << kv.page_shift) >= C::GROUP;
+	uint32_t n = 0;
+	while (u < u_end) {
+		const Piece p = piece_at<ROWS>(u, u_end, work, kv, st, a);
+		const int *pages = st.page_table + (long long)p.s * st.max_pages;
+		const int g0 = p.unit0 * (ATTN_UNIT / C::GROUP) + worker, g_end = min(p.unit1 * (ATTN_UNIT / C::GROUP), (p.key_end + C::GROUP - 1) / C::GROUP);
+		int next[C::HALVES];
+		auto pages_of = [&](int g) {
 #pragma unroll
-		for (int h = 0; h < C::HALVES; h++) {
-			const int key = key0 + 16 * h;
-			row[h] = key < key_end ? kv_page_row(kv, st, page[h], head) : -1;
-			ok |= (row[h] >= 0 ? 1u : 0u) << h;
-			row[h] += key & in_page;
-		}
-		there = there << 2 | ok;
-		if (lane == 0) {
+			for (int h = 0; h < C::HALVES; h++)
+				next[h] = mine && g < g_end && g * C::GROUP + 16 * h < p.key_end ? pages[(g * C::GROUP + 16 * h) >> kv.page_shift] : 0;
+		};
+		pages_of(g0);
+		for (int g = g0; mine && g < g_end; g += WARPS, n++) {
+			long long row[C::HALVES];
+			unsigned ok = 0;
+#pragma unroll
+			for (int h = 0; h < C::HALVES; h++) {
+				const int key = g * C::GROUP + 16 * h;
+				row[h] = key < p.key_end ? kv_page_row(kv, st, next[h], p.head) : -1;
+				ok |= (row[h] >= 0 ? 1u : 0u) << h;
+				row[h] += key & in_page;
+			}
+			pages_of(g + WARPS);
+			const uint32_t slot = n % C::STAGES, bar = ptx::smem_u32(&ring->full[worker][slot]);
+			if (n >= C::STAGES)
+				dec_wait(ptx::smem_u32(&ring->empty[worker][slot]), st.status, (n / C::STAGES & 1u) ^ 1u);
+			ring->there[worker][slot] = ok;
 			const int rows = one ? ((ok & 1) ? C::GROUP : 0) : 16 * __popc(ok);
-			ptx::mbar_arrive_expect_tx(bar(asked), rows * (2 * C::ROW + (C::Q8 ? 8 : 0)));
+			ptx::mbar_arrive_expect_tx(bar, rows * (2 * C::ROW + (C::Q8 ? 8 : 0)));
+			const uint32_t to = stages + (worker * C::STAGES + slot) * C::STAGE;
 #pragma unroll
 			for (int h = 0; h < C::HALVES; h++) {
 				if (!(ok >> h & 1) || (h && one))
 					continue;
-				const uint32_t to = slot(asked), k_to = to + h * 16 * C::BOX_BYTES, v_to = k_to + C::GROUP * C::ROW;
-#pragma unroll
-				for (int b = 0; b < C::BOXES; b++) {
-					ptx::tma_load_2d(k_to + b * C::PANEL, k_map, bar(asked), b * 64, (int)row[h]);
-					ptx::tma_load_2d(v_to + b * C::PANEL, v_map, bar(asked), b * 64, (int)row[h]);
-				}
+				const uint32_t k_to = to + h * 16 * C::BOX_BYTES, v_to = k_to + C::GROUP * C::ROW;
+				ptx::tma_load_3d(k_to, k_map, bar, 0, (int)row[h], 0);
+				ptx::tma_load_3d(v_to, v_map, bar, 0, (int)row[h], 0);
 				if constexpr (C::Q8) {
-					const uint32_t f = factor(asked) + 64 * h, bytes = one ? C::GROUP * 4 : 64;
-					bulk_g2s(f, kv.k_scale + row[h], bytes, bar(asked));
-					bulk_g2s(f + 4 * C::GROUP, kv.v_scale + row[h], bytes, bar(asked));
+					const uint32_t f = factors + (worker * C::STAGES + slot) * C::FACTORS + 64 * h, bytes = one ? C::GROUP * 4 : 64;
+					bulk_g2s(f, kv.k_scale + row[h], bytes, bar);
+					bulk_g2s(f + 4 * C::GROUP, kv.v_scale + row[h], bytes, bar);
 				}
 			}
 		}
-		asked++;
+		u += p.unit1 - p.unit0;
 	}
-};
+}
 
 // One warp's state over the groups of keys it takes: S^T = K Q^T and O^T = V^T P^T on m16n8k16, keys (then dims) on the
 // 16-row side, query rows on the 8-column side, so that a single token's 8 heads fill the columns.  A lane holds rows
@@ -149,8 +203,8 @@ struct Ring {
 template <int KIND, int D, int NB>
 struct Warp {
 	using C = Cfg<KIND, D>;
-	static constexpr int KS = D / 16, MB = D / 16, H = C::HALVES;
-	uint32_t q[NB][C::PARTS][KS][2];
+	static constexpr int KS = D / C::Q_STEP, MB = D / 16, H = C::HALVES;
+	uint32_t q[NB][C::Q_PARTS][KS][2];
 	float row_scale[NB][2];	 // scale * log2 e, and what the row's parts were divided by
 	float acc[NB][MB][4];	 // Q8: in units of v_unit
 	float m[NB][2], l[NB][2];  // running maximum (of the whole column), sum (of this lane's keys)
@@ -166,44 +220,80 @@ struct Warp {
 			const bool there = r < n_rows;
 			const int tok = there ? r / a.group : 0;
 			const float *src = a.q + ((long long)(seq.tok0 + tok) * a.n_head + head_kv * a.group + (there ? r - tok * a.group : 0)) * D;
-			float2 v[KS][2];
-			float top = 0.0f;
+			float top = 0.0f, up = 1.0f;
+			if constexpr (C::Q8) {
+				// Whole numbers of -127 * 2^16 .. 127 * 2^16 in units of the row's largest, as three signed bytes: bytes against bytes
+				// need no expansion of the keys and their sums are exact.
+				float4 v[KS][2];
 #pragma unroll
-			for (int j = 0; j < KS; j++) {
-				// the order of a step's 16 dims is free as long as keys have the same: that of packed bytes for Q8
-				if constexpr (KIND == TIE_CUDA_KV_Q8) {
-					const float4 f = there ? *reinterpret_cast<const float4 *>(src + 16 * j + 4 * c) : make_float4(0, 0, 0, 0);
-					v[j][0] = make_float2(f.x, f.y);
-					v[j][1] = make_float2(f.z, f.w);
-				} else {
-					v[j][0] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 2 * c) : make_float2(0, 0);
-					v[j][1] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 8 + 2 * c) : make_float2(0, 0);
-				}
+				for (int j = 0; j < KS; j++)
 #pragma unroll
-				for (int h = 0; h < 2; h++)
-					top = fmaxf(top, fmaxf(fabsf(v[j][h].x), fabsf(v[j][h].y)));
-			}
-			// fp16 parts: the row is brought to 1 .. 2 by a power of two (any fp32 row then keeps its 22 bits)
-			float down = 1.0f, up = 1.0f;
-			if constexpr (KIND != TIE_CUDA_KV_BF16) {
+					for (int h = 0; h < 2; h++) {
+						const float4 f = there ? *reinterpret_cast<const float4 *>(src + 32 * j + 16 * h + 4 * c) : make_float4(0, 0, 0, 0);
+						v[j][h] = f;
+						top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+					}
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-				const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-				if (top > 0.0f) {
-					down = __uint_as_float((unsigned)(254 - e) << 23);
-					up = __uint_as_float((unsigned)e << 23);
+				constexpr float MOST = 127.0f * 65536.0f;
+				// (a row below 2^-100 of anything is brought up by two factors, since the inverse of its largest is no fp32 number)
+				const float lift = top < 0x1p-100f ? 0x1p100f : 1.0f;
+				const float down = top > 0.0f ? MOST / (top * lift) : 0.0f;
+				up = top * (1.0f / MOST);
+				bool odd = false;
+#pragma unroll
+				for (int j = 0; j < KS; j++)
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						const float x[4] = {v[j][h].x, v[j][h].y, v[j][h].z, v[j][h].w};
+						uint32_t n[4];
+#pragma unroll
+						for (int i = 0; i < 4; i++) {
+							odd = odd || !(fabsf(x[i]) <= FLT_MAX);
+							// + 128 in each byte makes signed digits of them
+							n[i] = (uint32_t)__float2int_rn(x[i] * lift * down) + 0x00808080u;
+						}
+#pragma unroll
+						for (int p = 0; p < 3; p++) {  // the highest byte first
+							const uint32_t s = p == 0 ? 0x0062 : p == 1 ? 0x0051 : 0x0040;
+							q[nb][p][j][h] = (__byte_perm(n[0], n[1], s) & 0xffffu | __byte_perm(n[2], n[3], s) << 16) ^ 0x80808080u;
+						}
+					}
+				odd = odd || __shfl_xor_sync(0xffffffffu, (int)odd, 1);
+				odd = odd || __shfl_xor_sync(0xffffffffu, (int)odd, 2);
+				up = odd ? __int_as_float(0x7fc00000) : up;  // a row with an infinity or NaN has no scores
+			} else {
+				float2 v[KS][2];
+#pragma unroll
+				for (int j = 0; j < KS; j++) {
+					v[j][0] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 2 * c) : make_float2(0, 0);
+					v[j][1] = there ? *reinterpret_cast<const float2 *>(src + 16 * j + 8 + 2 * c) : make_float2(0, 0);
+#pragma unroll
+					for (int h = 0; h < 2; h++)
+						top = fmaxf(top, fmaxf(fabsf(v[j][h].x), fabsf(v[j][h].y)));
 				}
+				// fp16 parts: the row is brought to 1 .. 2 by a power of two (any fp32 row then keeps its 22 bits)
+				float down = 1.0f;
+				if constexpr (KIND != TIE_CUDA_KV_BF16) {
+					top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+					top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+					const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+					if (top > 0.0f) {
+						down = __uint_as_float((unsigned)(254 - e) << 23);
+						up = __uint_as_float((unsigned)e << 23);
+					}
+				}
+#pragma unroll
+				for (int j = 0; j < KS; j++)
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						uint32_t part[C::PARTS];
+						split_pair<KIND>(v[j][h].x * down, v[j][h].y * down, part);
+#pragma unroll
+						for (int p = 0; p < C::PARTS; p++)
+							q[nb][p][j][h] = part[p];
+					}
 			}
-#pragma unroll
-			for (int j = 0; j < KS; j++)
-#pragma unroll
-				for (int h = 0; h < 2; h++) {
-					uint32_t part[C::PARTS];
-					split_pair<KIND>(v[j][h].x * down, v[j][h].y * down, part);
-#pragma unroll
-					for (int p = 0; p < C::PARTS; p++)
-						q[nb][p][j][h] = part[p];
-				}
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
 				row_scale[nb][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4) * a.scale_log2e;
@@ -229,51 +319,61 @@ struct Warp {
 		float s[H][NB][4];
 #pragma unroll
 		for (int h = 0; h < H; h++) {
-			float part[NB][C::PARTS][4];  // a chain each: the tensor cores cut every sum off
-#pragma unroll
-			for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-				for (int p = 0; p < C::PARTS; p++)
-#pragma unroll
-					for (int i = 0; i < 4; i++)
-						part[nb][p][i] = 0.0f;
 			const int krow = 16 * h + (lane & 15), kch = lane >> 4;
+			if constexpr (C::Q8) {
+				int part[NB][3][4];
 #pragma unroll
-			for (int j = 0; j < (C::Q8 ? KS / 2 : KS); j++) {
-				uint32_t r[4];
-				ldsm4(r, ks + C::place(krow, 2 * j + kch));
-				if constexpr (C::Q8) {
+				for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+					for (int p = 0; p < 3; p++)
+#pragma unroll
+						for (int i = 0; i < 4; i++)
+							part[nb][p][i] = 0;
+#pragma unroll
+				for (int j = 0; j < KS; j++) {
+					uint32_t r[4];
+					ldsm4(r, ks + C::place(krow, 2 * j + kch));
+#pragma unroll
+					for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+						for (int p = 0; p < 3; p++)
+							mma_bytes(part[nb][p], r, q[nb][p][j][0], q[nb][p][j][1]);
+				}
+#pragma unroll
+				for (int nb = 0; nb < NB; nb++)
 #pragma unroll
 					for (int i = 0; i < 4; i++)
-						r[i] ^= 0x80808080u;
+						s[h][nb][i] = fmaf((float)part[nb][0][i], 65536.0f, (float)(part[nb][1][i] * 256 + part[nb][2][i])) * row_scale[nb][i & 1];
+			} else {
+				float part[NB][C::PARTS][4];  // a chain each: the tensor cores cut every sum off
 #pragma unroll
-					for (int k = 0; k < 2; k++) {
-						const uint32_t f[4] = {int8_pair<0x4140>(r[2 * k]), int8_pair<0x4140>(r[2 * k + 1]), int8_pair<0x4342>(r[2 * k]),
-								       int8_pair<0x4342>(r[2 * k + 1])};
+				for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-						for (int nb = 0; nb < NB; nb++)
+					for (int p = 0; p < C::PARTS; p++)
 #pragma unroll
-							for (int p = 0; p < C::PARTS; p++)
-								mma<KIND>(part[nb][p], f, q[nb][p][2 * j + k][0], q[nb][p][2 * j + k][1]);
-					}
-				} else {
+						for (int i = 0; i < 4; i++)
+							part[nb][p][i] = 0.0f;
+#pragma unroll
+				for (int j = 0; j < KS; j++) {
+					uint32_t r[4];
+					ldsm4(r, ks + C::place(krow, 2 * j + kch));
 #pragma unroll
 					for (int nb = 0; nb < NB; nb++)
 #pragma unroll
 						for (int p = 0; p < C::PARTS; p++)
 							mma<KIND>(part[nb][p], r, q[nb][p][j][0], q[nb][p][j][1]);
 				}
+#pragma unroll
+				for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						float v = part[nb][C::PARTS - 1][i];
+#pragma unroll
+						for (int p = C::PARTS - 2; p >= 0; p--)
+							v += part[nb][p][i];
+						s[h][nb][i] = v * row_scale[nb][i & 1];
+					}
 			}
-#pragma unroll
-			for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-				for (int i = 0; i < 4; i++) {
-					float v = part[nb][C::PARTS - 1][i];
-#pragma unroll
-					for (int p = C::PARTS - 2; p >= 0; p--)
-						v += part[nb][p][i];
-					s[h][nb][i] = v * row_scale[nb][i & 1];
-				}
 		}
 		float v_rel[H][2], unit_change = 1.0f;
 		if constexpr (C::Q8) {
@@ -487,8 +587,7 @@ template <int KIND, int D, int NB>
 constexpr size_t smem_bytes()
 {
 	using C = Cfg<KIND, D>;
-	constexpr size_t stages = (size_t)WARPS * C::STAGES * (C::STAGE + C::FACTORS), rows = (size_t)WARPS * 8 * NB * D * 4;
-	return (stages > rows ? stages : rows) + 1024;
+	return (size_t)WARPS * C::STAGES * (C::STAGE + C::FACTORS) + (size_t)WARPS / 2 * 8 * D * 4 + 1024;
 }
 
 template <int KIND, int D, int NB>
@@ -499,15 +598,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 	constexpr int ROWS = 8 * NB, D4 = D / 4, UNIT_GROUPS = ATTN_UNIT / C::GROUP;
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ AttnWork work;
+	__shared__ Ring<KIND, D> ring;
 	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS], s_unit[WARPS];
-	__shared__ uint64_t s_bar[WARPS][C::STAGES];
-	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+	const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u, factors = stages + WARPS * C::STAGES * C::STAGE;
+	// [half of the warps][8 rows][D]: sums on their way together
+	float *sums = reinterpret_cast<float *>(smem_raw + (factors - ptx::smem_u32(smem_raw)) + WARPS * C::STAGES * C::FACTORS);
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
-	Ring<KIND, D> ring = {ptx::smem_u32(smem) + warp * C::STAGES * C::STAGE,
-			      ptx::smem_u32(smem) + WARPS * C::STAGES * C::STAGE + warp * C::STAGES * C::FACTORS, ptx::smem_u32(s_bar[warp])};
-	if (lane == 0) {
-		for (int i = 0; i < C::STAGES; i++)
-			ptx::mbar_init(ring.bars + 8 * i, 1);
+	if (threadIdx.x == 0) {
+		for (int w = 0; w < WARPS; w++)
+			for (int i = 0; i < C::STAGES; i++) {
+				ptx::mbar_init(ptx::smem_u32(&ring.full[w][i]), 1);
+				ptx::mbar_init(ptx::smem_u32(&ring.empty[w][i]), 1);
+			}
 		ptx::fence_barrier_init();
 		ptx::fence_proxy_async_smem();
 	}
@@ -517,51 +619,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 	if (cta >= n_cta)
 		return;
 	const long long u_begin = attn_div(total * cta, n_cta), u_end = attn_div(total * (cta + 1), n_cta);
+	if (warp >= WARPS) {
+		const int worker = (warp - WARPS) * EACH + lane % EACH;
+		request<KIND, D, ROWS>(&ring, stages, factors, u_begin, u_end, work, kv, st, a, &k_map, &v_map, worker, lane < EACH);
+		return;
+	}
 	Warp<KIND, D, NB> w;
+	uint32_t taken = 0;
 	for (long long u = u_begin; u < u_end;) {
-		const int s = attn_sequence_of(work, st.n_seq, u);
-		const SeqView seq = kv_sequence(st, kv.page_shift, s);
-		const int n_keys = seq.kv_len + seq.n_tok, item_units = attn_units(seq);
-		const int tiles = (seq.n_tok * a.group + ROWS - 1) / ROWS;
-		const long long in_seq = u - work.start[s], item = attn_div(in_seq, item_units);
-		const int unit0 = (int)(in_seq - item * item_units);
-		const int unit1 = (int)min((long long)item_units, unit0 + (u_end - u));
-		const int head = (int)attn_div(item, tiles), row0 = (int)(item - (long long)head * tiles) * ROWS;
-		// a tile's last row sees the furthest unless a tree says otherwise
-		const int last_tok = min((row0 + ROWS - 1) / a.group, seq.n_tok - 1);
-		const int key_end = st.tree ? n_keys : seq.kv_len + last_tok + 1;
+		const Piece p = piece_at<ROWS>(u, u_end, work, kv, st, a);
+		const SeqView seq = p.seq;
 		if (st.tree && seq.n_tok > KV_MAX_TREE && threadIdx.x == 0)
 			kv_report(st, ST_BAD_STEP);
-		const int g_first = unit0 * UNIT_GROUPS + warp, g_end = min(unit1 * UNIT_GROUPS, (key_end + C::GROUP - 1) / C::GROUP);
-		const int *pages = st.page_table + (long long)s * st.max_pages;
-		auto pages_of = [&](int g, int (&page)[2]) {
-#pragma unroll
-			for (int h = 0; h < 2; h++)
-				page[h] = h < C::HALVES && g < g_end && g * C::GROUP + 16 * h < key_end ? pages[(g * C::GROUP + 16 * h) >> kv.page_shift] : 0;
-		};
-		auto ask = [&](int g, const int (&page)[2]) {
-			if (g < g_end)
-				ring.ask(kv, st, &k_map, &v_map, g * C::GROUP, key_end, page, head, lane);
-			else
-				ring.there <<= 2;
-		};
-		int page[C::STAGES][2];
-#pragma unroll
-		for (int i = 0; i < C::STAGES; i++)
-			pages_of(g_first + i * WARPS, page[i]);
-#pragma unroll
-		for (int i = 0; i < C::STAGES - 1; i++)
-			ask(g_first + i * WARPS, page[i]);
-		w.begin(a, seq, head, row0, lane);
-		for (int g = g_first; g < g_end; g += WARPS) {
-			const int behind = g + (C::STAGES - 1) * WARPS;
-			const int now[2] = {page[C::STAGES - 1][0], page[C::STAGES - 1][1]};
-			pages_of(behind + WARPS, page[C::STAGES - 1]);
-			ask(behind, now);
-			dec_wait(ring.bar(ring.taken), st.status, ring.taken / C::STAGES & 1u);
-			w.group(a, st, seq, ring.slot(ring.taken), ring.factor(ring.taken), g * C::GROUP, key_end, ring.there >> (2 * (C::STAGES - 1)) & 3u, row0, lane);
-			ring.taken++;
+		const int g_end = min(p.unit1 * UNIT_GROUPS, (p.key_end + C::GROUP - 1) / C::GROUP);
+		w.begin(a, seq, p.head, p.row0, lane);
+		for (int g = p.unit0 * UNIT_GROUPS + warp; g < g_end; g += WARPS, taken++) {
+			const uint32_t slot = taken % C::STAGES, at = warp * C::STAGES + slot;
+			dec_wait(ptx::smem_u32(&ring.full[warp][slot]), st.status, taken / C::STAGES & 1u);
+			w.group(a, st, seq, stages + at * C::STAGE, factors + at * C::FACTORS, g * C::GROUP, p.key_end, ring.there[warp][slot], p.row0, lane);
 			__syncwarp();
+			if (lane == 0)
+				ptx::mbar_arrive(ptx::smem_u32(&ring.empty[warp][slot]));
 		}
 
 		// the warps' keys together
@@ -580,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			}
 		if (lane == 0)
 			s_unit[warp] = C::Q8 ? w.v_unit : 1.0f;
-		__syncthreads();  // (and nobody reads keys any more)
+		workers_sync();
 		if (threadIdx.x < ROWS) {
 			const int r = threadIdx.x;
 			float top = -INFINITY, sum = 0.0f;
@@ -596,129 +674,156 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 			s_top[r] = top;
 			s_sum[r] = sum;
 		}
-		float *rows = reinterpret_cast<float *>(smem);	// [warp][row][D]
-#pragma unroll
-		for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-			for (int mb = 0; mb < D / 16; mb++)
-#pragma unroll
-				for (int i = 0; i < 4; i++)
-					rows[(warp * ROWS + nb * 8 + 2 * (lane & 3) + (i & 1)) * D + w.dim(mb, i, lane)] = w.acc[nb][mb][i];
-		__syncthreads();
-		const bool whole = unit0 == 0 && unit1 == item_units;
+		workers_sync();
+		const bool whole = p.unit0 == 0 && p.unit1 == p.item_units;
 		const int n_rows = seq.n_tok * a.group;
+		float *part = a.part + (2 * cta + (p.unit0 == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS);
 		auto out_row = [&](int r) {
 			const int tok = r / a.group;
-			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + head * a.group + (r - tok * a.group)) * D;
+			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + p.head * a.group + (r - tok * a.group)) * D;
 		};
-		float *part = a.part + (2 * cta + (unit0 == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS);
-		for (int i = threadIdx.x; i < ROWS * D4; i += THREADS) {
-			const int r = i / D4, col = i % D4 * 4;
-			float4 sum = make_float4(0, 0, 0, 0);
+		// 8 rows: the later warps' sums to the earlier ones, and these by all threads (4 dims of a row each)
+		auto together = [&](auto give, auto take) {
 #pragma unroll
-			for (int k = 0; k < WARPS; k++) {
-				const float f = s_w[r][k];
-				const float4 v = *reinterpret_cast<const float4 *>(rows + (k * ROWS + r) * D + col);
-				if (f != 0.0f) {  // (a warp whose keys the row does not see has nothing to give)
-					sum.x = fmaf(v.x, f, sum.x);
-					sum.y = fmaf(v.y, f, sum.y);
-					sum.z = fmaf(v.z, f, sum.z);
-					sum.w = fmaf(v.w, f, sum.w);
-				}
+			for (int half = 1; half >= 0; half--) {
+				if ((warp >= WARPS / 2) == (half == 1))
+					give(sums + warp % (WARPS / 2) * 8 * D, half == 0);
+				workers_sync();
 			}
-			if (whole) {
-				if (row0 + r < n_rows) {
-					const float inv = s_sum[r] == 0.0f ? 0.0f : 1.0f / s_sum[r];
-					*reinterpret_cast<float4 *>(out_row(row0 + r) + col) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+			for (int i = threadIdx.x; i < 8 * D4; i += WORKERS) {
+				float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+				for (int k = 0; k < WARPS / 2; k++) {
+					const float4 v = *reinterpret_cast<const float4 *>(sums + (k * 8 + i / D4) * D + i % D4 * 4);
+					y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
 				}
-			} else {
-				*reinterpret_cast<float4 *>(part + r * D + col) = sum;
+				take(i / D4, i % D4 * 4, y);
 			}
-		}
+			workers_sync();
+		};
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++)
+			together(
+				[&](float *to, bool add) {
+#pragma unroll
+					for (int i = 0; i < 2; i++) {
+						const int r = 2 * (lane & 3) + i;
+						const float f = s_w[nb * 8 + r][warp];
+#pragma unroll
+						for (int mb = 0; mb < D / 16; mb++)
+#pragma unroll
+							for (int h = 0; h < 2; h++) {
+								float &d = to[r * D + w.dim(mb, 2 * h, lane)];
+								// (a warp whose keys the row does not see has nothing to give)
+								const float v = f == 0.0f ? 0.0f : w.acc[nb][mb][2 * h + i] * f;
+								d = add ? d + v : v;
+							}
+					}
+				},
+				[&](int r8, int col, float4 y) {
+					const int r = nb * 8 + r8;
+					if (!whole) {
+						*reinterpret_cast<float4 *>(part + r * D + col) = y;
+					} else if (p.row0 + r < n_rows) {
+						const float inv = s_sum[r] == 0.0f ? 0.0f : 1.0f / s_sum[r];
+						*reinterpret_cast<float4 *>(out_row(p.row0 + r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+					}
+				});
 		if (!whole) {
 			if (threadIdx.x < ROWS) {
 				part[MAX_ROWS * 128 + threadIdx.x] = s_top[threadIdx.x];
 				part[MAX_ROWS * 128 + MAX_ROWS + threadIdx.x] = s_sum[threadIdx.x];
 			}
 			// the CTAs of the item: those of its first and last unit, and all between
-			const long long i0 = work.start[s] + item * item_units, i1 = i0 + item_units - 1;
-			const int c0 = attn_cta_of(i0, total, n_cta), c1 = attn_cta_of(i1, total, n_cta), n = c1 - c0 + 1;
+			const int c0 = attn_cta_of(p.first_unit, total, n_cta), c1 = attn_cta_of(p.first_unit + p.item_units - 1, total, n_cta), n = c1 - c0 + 1;
 			__threadfence();
-			__syncthreads();
+			workers_sync();
 			if (threadIdx.x == 0)
 				work.last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
-			__syncthreads();
+			workers_sync();
 			if (work.last) {
-				// Joined in the order of the CTAs: warp w takes parts w, w + 8 .. of all rows (a lane 4 dims), then the warps' sums.
+				// Joined in the order of the CTAs: warp w takes parts w, w + 8 .. of 8 rows (a lane 4 dims), then the warps' sums.
 				__threadfence();
 				auto at = [&](int i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * attn_part_floats(MAX_ROWS); };
-				constexpr int PER = 32 / D4, STEPS = ROWS / PER;  // rows at once
-				float4 sum[STEPS];
-				float top[STEPS], l[STEPS];
-#pragma unroll
-				for (int k = 0; k < STEPS; k++) {
-					sum[k] = make_float4(0, 0, 0, 0);
-					top[k] = -INFINITY;
-					l[k] = 0.0f;
-				}
-				for (int i = warp; i < n; i += WARPS) {
-					const float *p = at(i);
-					float4 v[STEPS];
-					float pm[STEPS], pl[STEPS];
+				constexpr int PER = 32 / D4, STEPS = 8 / PER;  // rows at once
+#pragma unroll 1
+				for (int nb = 0; nb < NB; nb++) {
+					float4 sum[STEPS];
+					float top[STEPS], l[STEPS];
 #pragma unroll
 					for (int k = 0; k < STEPS; k++) {
-						const int r = k * PER + lane / D4;
-						v[k] = __ldcg(reinterpret_cast<const float4 *>(p + r * D) + lane % D4);
-						pm[k] = __ldcg(p + MAX_ROWS * 128 + r);
-						pl[k] = __ldcg(p + MAX_ROWS * 128 + MAX_ROWS + r);
+						sum[k] = make_float4(0, 0, 0, 0);
+						top[k] = -INFINITY;
+						l[k] = 0.0f;
+					}
+					for (int i = warp; i < n; i += WARPS) {
+						const float *src = at(i);
+						float4 v[STEPS];
+						float pm[STEPS], pl[STEPS];
+#pragma unroll
+						for (int k = 0; k < STEPS; k++) {
+							const int r = nb * 8 + k * PER + lane / D4;
+							v[k] = __ldcg(reinterpret_cast<const float4 *>(src + r * D) + lane % D4);
+							pm[k] = __ldcg(src + MAX_ROWS * 128 + r);
+							pl[k] = __ldcg(src + MAX_ROWS * 128 + MAX_ROWS + r);
+						}
+#pragma unroll
+						for (int k = 0; k < STEPS; k++) {
+							const float next = fmaxf(top[k], pm[k]);
+							const float f = pm[k] == -INFINITY ? 0.0f : exp2_ftz(pm[k] - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
+							top[k] = next;
+							l[k] = fmaf(pl[k], f, l[k] * o);
+							if (f != 0.0f)
+								sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
+										     fmaf(v[k].w, f, sum[k].w * o));
+						}
 					}
 #pragma unroll
-					for (int k = 0; k < STEPS; k++) {
-						const float next = fmaxf(top[k], pm[k]);
-						const float f = pm[k] == -INFINITY ? 0.0f : exp2_ftz(pm[k] - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
-						top[k] = next;
-						l[k] = fmaf(pl[k], f, l[k] * o);
-						if (f != 0.0f)
-							sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
-									     fmaf(v[k].w, f, sum[k].w * o));
-					}
-				}
+					for (int k = 0; k < STEPS; k++)
+						if (lane % D4 == 0) {
+							s_m[warp][k * PER + lane / D4] = top[k];
+							s_l[warp][k * PER + lane / D4] = l[k];
+						}
+					workers_sync();
+					if (threadIdx.x < 8) {
+						const int r = threadIdx.x;
+						float t = -INFINITY, all = 0.0f;
 #pragma unroll
-				for (int k = 0; k < STEPS; k++) {
-					const int r = k * PER + lane / D4;
-					*reinterpret_cast<float4 *>(rows + (warp * ROWS + r) * D + lane % D4 * 4) = sum[k];
-					if (lane % D4 == 0) {
-						s_m[warp][r] = top[k];
-						s_l[warp][r] = l[k];
-					}
-				}
-				__syncthreads();
-				for (int i = threadIdx.x; i < ROWS * D4; i += THREADS) {
-					const int r = i / D4, col = i % D4 * 4;
-					if (row0 + r >= n_rows)
-						break;
-					float t = -INFINITY, all = 0.0f;
-					float4 y = make_float4(0, 0, 0, 0);
+						for (int k = 0; k < WARPS; k++)
+							t = fmaxf(t, s_m[k][r]);
 #pragma unroll
-					for (int k = 0; k < WARPS; k++)
-						t = fmaxf(t, s_m[k][r]);
-#pragma unroll
-					for (int k = 0; k < WARPS; k++) {
-						const float f = s_m[k][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[k][r] - t);
-						const float4 v = *reinterpret_cast<const float4 *>(rows + (k * ROWS + r) * D + col);
-						all = fmaf(s_l[k][r], f, all);
-						y = make_float4(fmaf(v.x, f, y.x), fmaf(v.y, f, y.y), fmaf(v.z, f, y.z), fmaf(v.w, f, y.w));
+						for (int k = 0; k < WARPS; k++) {
+							const float f = s_m[k][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[k][r] - t);
+							s_w[r][k] = f;
+							all = fmaf(s_l[k][r], f, all);
+						}
+						s_sum[r] = all;
 					}
-					const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-					*reinterpret_cast<float4 *>(out_row(row0 + r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+					workers_sync();
+					together(
+						[&](float *to, bool add) {
+#pragma unroll
+							for (int k = 0; k < STEPS; k++) {
+								const int r = k * PER + lane / D4;
+								const float f = s_w[r][warp];
+								float4 *d = reinterpret_cast<float4 *>(to + r * D) + lane % D4;
+								const float4 o = add ? *d : make_float4(0, 0, 0, 0);
+								*d = make_float4(fmaf(sum[k].x, f, o.x), fmaf(sum[k].y, f, o.y), fmaf(sum[k].z, f, o.z), fmaf(sum[k].w, f, o.w));
+							}
+						},
+						[&](int r8, int col, float4 y) {
+							const int r = p.row0 + nb * 8 + r8;
+							if (r >= n_rows)
+								return;
+							const float inv = s_sum[r8] == 0.0f ? 0.0f : 1.0f / s_sum[r8];
+							*reinterpret_cast<float4 *>(out_row(r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+						});
 				}
 				if (threadIdx.x == 0)
 					a.count[c0] = 0;  // at rest again
 			}
 		}
-		ptx::fence_proxy_async_smem();	// the next item's boxes land where these rows were
-		__syncthreads();
-		u += unit1 - unit0;
+		u += p.unit1 - p.unit0;
 	}
 }
 
@@ -758,14 +863,20 @@ int go_kind(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int head_dim,
 
 }  // namespace
 
-// Maps of keys and values for boxes of up to box_rows rows of a page x box_bytes.
+// Maps of keys and values: boxes of up to box_rows rows of a page x the whole row, box_bytes of it side by side (the shared-memory
+// row that is swizzled), the next box_bytes of all rows behind these; of pages with fewer rows, one of these panels a box.
 int attn_maps(tie_cuda_ctx *c, const KvView &kv, int elem, int head_dim, int box_bytes, int box_rows, CUtensorMapSwizzle swizzle, CUtensorMap *map)
 {
 	const size_t rows = ((size_t)kv.n_pages * kv.n_head_kv) << kv.page_shift;
 	const int n = 1 << kv.page_shift < box_rows ? 1 << kv.page_shift : box_rows;
 	const CUtensorMapDataType type = elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
-	const int rc = tc_encode_2d(c, &map[0], type, elem, kv.k, rows, head_dim, box_bytes / elem, n, swizzle);
-	return rc ? rc : tc_encode_2d(c, &map[1], type, elem, kv.v, rows, head_dim, box_bytes / elem, n, swizzle);
+	for (int i = 0; i < 2; i++) {
+		const int rc = tc_encode_panels(c, &map[i], type, elem, i ? kv.v : kv.k, rows, head_dim, box_bytes / elem, n,
+						n == box_rows ? head_dim * elem / box_bytes : 1, swizzle);
+		if (rc)
+			return rc;
+	}
+	return TIE_CUDA_OK;
 }
 
 size_t attn_scratch_floats(const tie_cuda_ctx *c)

@@ -54,7 +54,7 @@ __device__ __forceinline__ int attn_units(const SeqView &q)
 template <int THREADS, class F>
 __device__ __forceinline__ void attn_share_work(AttnWork &w, const KvView &kv, const StepView &st, F of)
 {
-	constexpr int PER = KV_MAX_SEQ / THREADS;
+	constexpr int PER = (KV_MAX_SEQ + THREADS - 1) / THREADS;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	if (st.n_seq == 1) {
 		if (threadIdx.x == 0) {
@@ -91,7 +91,7 @@ __device__ __forceinline__ void attn_share_work(AttnWork &w, const KvView &kv, c
 			w.start[s] = at;
 		at += mine[i];
 	}
-	if (threadIdx.x == THREADS - 1 && st.n_seq == KV_MAX_SEQ)
+	if (threadIdx.x == THREADS - 1 && THREADS * PER <= st.n_seq)
 		w.start[st.n_seq] = at;
 	__syncthreads();
 }

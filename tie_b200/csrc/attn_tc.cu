@@ -314,9 +314,13 @@ __device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared
 				const uint32_t bar = ptx::smem_u32(&raw_bar[slot]);
 				const uint32_t dst = T::RAW ? raw + slot * T::RAW + lane * run * T::ROW
 							    : ring + slot * T::BYTES + (T::SCALED ? T::PANEL : 0u) + lane * run * 128;
+				if (run == T::TK || T::BOXES == 1) {
+					ptx::tma_load_3d(dst, map, bar, 0, (int)row, 0);
+				} else {
 #pragma unroll
-				for (int b = 0; b < T::BOXES; b++)
-					ptx::tma_load_2d(dst + b * T::PANEL, map, bar, b * 64, (int)row);
+					for (int b = 0; b < T::BOXES; b++)  // (the halves of a page's rows lie a tile's panel apart)
+						ptx::tma_load_3d(dst + b * T::PANEL, map, bar, 0, (int)row, b);
+				}
 				if constexpr (T::SCALED)
 					bulk_g2s(ptx::smem_u32(VALUES ? sh->v_got[slot] : sh->k_scale[n % T::FACTS]) + 4 * lane * run, (VALUES ? kv.v_scale : kv.k_scale) + row,
 						  run * 4, bar);

@@ -61,9 +61,8 @@ int launch_split_rows(tie_cuda_ctx *c, const float *x, int n_src, int n_cols, __
 int launch_swiglu(tie_cuda_ctx *c, float *gate, const float *up, int n);
 // tensor.cu
 int tc_setup(tie_cuda_ctx *c);
-// a map of rows x cols elements (rows one behind the other) with boxes of box_rows x box_cols
-int tc_encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols, unsigned box_cols,
-		 unsigned box_rows, CUtensorMapSwizzle swz);
+int tc_encode_panels(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols, unsigned box_cols,
+		     unsigned box_rows, unsigned box_panels, CUtensorMapSwizzle swz);
 int tc_make_weight_map(tie_cuda_ctx *c, DevTensor &t, bool half_tiles, int n_experts = -1);  // default: the context's local experts
 bool tc_dense_supported(const tie_cuda_ctx *c, const DevTensor &t);
 int tc_make_dense_view(tie_cuda_ctx *c, DevTensor &t);

@@ -1038,8 +1038,8 @@ static PFN_encodeTiled get_encode_fn()
 	return fn;
 }
 
-int tc_encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols,
-		 unsigned box_cols, unsigned box_rows, CUtensorMapSwizzle swz)
+static int encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols,
+		     unsigned box_cols, unsigned box_rows, CUtensorMapSwizzle swz)
 {
 	PFN_encodeTiled enc = get_encode_fn();
 	if (!enc) {
@@ -1054,6 +1054,28 @@ int tc_encode_2d(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, siz
 			 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 	if (r != CUDA_SUCCESS) {
 		snprintf(c->cuda_err, sizeof(c->cuda_err), "cuTensorMapEncodeTiled failed: %d", (int)r);
+		return TIE_CUDA_ECUDA;
+	}
+	return TIE_CUDA_OK;
+}
+
+// The same rows as [cols / box_cols] panels side by side: a box is box_rows rows x box_cols columns of each of box_panels panels.
+int tc_encode_panels(tie_cuda_ctx *c, CUtensorMap *tm, CUtensorMapDataType type, size_t elem, void *base, size_t rows, size_t cols, unsigned box_cols,
+		     unsigned box_rows, unsigned box_panels, CUtensorMapSwizzle swz)
+{
+	PFN_encodeTiled enc = get_encode_fn();
+	if (!enc) {
+		snprintf(c->cuda_err, sizeof(c->cuda_err), "cuTensorMapEncodeTiled entry point not found");
+		return TIE_CUDA_ECUDA;
+	}
+	cuuint64_t dims[3] = {box_cols, (cuuint64_t)rows, (cuuint64_t)(cols / box_cols)};
+	cuuint64_t strides[2] = {(cuuint64_t)(cols * elem), (cuuint64_t)(box_cols * elem)};
+	cuuint32_t box[3] = {box_cols, box_rows, box_panels};
+	cuuint32_t estr[3] = {1, 1, 1};
+	CUresult r = enc(tm, type, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+			 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+	if (r != CUDA_SUCCESS) {
+		snprintf(c->cuda_err, sizeof(c->cuda_err), "cuTensorMapEncodeTiled (key and value rows) failed: %d", (int)r);
 		return TIE_CUDA_ECUDA;
 	}
 	return TIE_CUDA_OK;
@@ -1115,7 +1137,7 @@ int tc_make_weight_map(tie_cuda_ctx *c, DevTensor &t, bool half_tiles, int n_exp
 	const int nb = t.k / QK_K;
 	const unsigned box_rows = half_tiles ? TC_BM / 2 : TC_BM;
 	if (t.kind == W_Q4K) {
-		int rc = tc_encode_2d(c, &t.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, t.ptr, (size_t)t.rows * n_experts, (size_t)nb * Q4K_BYTES,
+		int rc = encode_2d(c, &t.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, t.ptr, (size_t)t.rows * n_experts, (size_t)nb * Q4K_BYTES,
 				   Q4K_BYTES, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 		if (rc)
 			return rc;
