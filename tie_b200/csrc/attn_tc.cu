@@ -40,7 +40,9 @@ constexpr long long WAIT_CYCLES = 1ll << 30;
 struct Piece {
 	SeqView seq;
 	int s, head, row0;
-	int unit0, unit1, item_units;
+	int unit0, unit1;
+	bool whole, first;  // the item, its first part
+	int n_parts;	// first: parts of the item
 	int n_tiles;	// from unit0 on: tiles that some row of the item sees keys of
 	int key_end;	// first key that nobody sees
 	int all_see;	// keys in front of this one are seen by every row
@@ -65,77 +67,111 @@ struct Shared {
 	uint32_t tmem_base, abort;
 };
 
+// How a launch's work is shared out.  WHOLE: items, several to a CTA.  EVEN: each CTA the same number of units, whatever items
+// they belong to (a CTA then mostly has the end of one and the beginning of another).  PARTS: no more items than CTAs,
+// each cut into as many equal parts as leave one part to a CTA.
+enum Share : int { WHOLE, EVEN, PARTS };
+// What a piece costs besides its tiles (set-up, first loads, joins), in units: 20,000 cycles against 2500 a unit.
+constexpr int PIECE_UNITS = 8;
 struct Walk {
-	bool shared;
+	Share share;
 	long long total, u, u_end;
 	int n_cta, round;
+	int part_units;	 // PARTS: units of a part, at most
 };
-
-template <int TK>
-__device__ __forceinline__ void finish_piece(Piece &p, const StepView &st, const AttnArgs &a)
-{
-	const int first_tok = p.row0 / a.group, last_tok = min((p.row0 + ROWS - 1) / a.group, p.seq.n_tok - 1);
-	p.key_end = p.seq.kv_len + (st.tree ? p.seq.n_tok : last_tok + 1);
-	p.all_see = p.seq.kv_len + (st.tree ? 0 : first_tok + 1);
-	p.n_tiles = max(0, (min(p.unit1 * ATTN_UNIT, p.key_end) - p.unit0 * ATTN_UNIT + TK - 1) / TK);
-}
 
 template <int TK>
 __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
-	if (w.shared) {
-		if (w.u >= w.u_end)
-			return false;
-		p.s = attn_sequence_of(work, st.n_seq, w.u);
-		p.seq = kv_sequence(st, kv.page_shift, p.s);
-		const int tiles = (int)(((long long)p.seq.n_tok * a.group + ROWS - 1) / ROWS);
-		p.item_units = attn_units(p.seq);
-		const long long in_seq = w.u - work.start[p.s], item = attn_div(in_seq, p.item_units);
-		p.unit0 = (int)(in_seq - item * p.item_units);
-		p.unit1 = (int)min((long long)p.item_units, p.unit0 + (w.u_end - w.u));
-		p.head = (int)attn_div(item, tiles);
-		p.row0 = (int)(item - (long long)p.head * tiles) * ROWS;
-		w.u += p.unit1 - p.unit0;
-	} else {
-		// whole items, a sequence's last rows (the ones that see most) first, there and back over the CTAs
-		long long i;
+	long long i = w.u;  // unit, item or part
+	if (w.share == WHOLE) {
+		// a sequence's last rows (the ones that see most) first, there and back over the CTAs
 		do {
 			if ((long long)w.round * w.n_cta >= w.total)
 				return false;
 			i = (w.round & 1) ? (long long)(w.round + 1) * w.n_cta - 1 - blockIdx.x : (long long)w.round * w.n_cta + blockIdx.x;
 			w.round++;
 		} while (i >= w.total);
-		p.s = attn_sequence_of(work, st.n_seq, i);
-		p.seq = kv_sequence(st, kv.page_shift, p.s);
-		const int tiles = (int)(((long long)p.seq.n_tok * a.group + ROWS - 1) / ROWS);
-		const int in_seq = (int)(i - work.start[p.s]);
-		p.row0 = (tiles - 1 - in_seq / kv.n_head_kv) * ROWS;
-		p.head = in_seq % kv.n_head_kv;
-		p.unit0 = 0;
-		p.unit1 = p.item_units = attn_units(p.seq);
+	} else if (w.u >= w.u_end) {
+		return false;
 	}
-	finish_piece<TK>(p, st, a);
+	p.s = attn_sequence_of(work, st.n_seq, i);
+	p.seq = kv_sequence(st, kv.page_shift, p.s);
+	const int tiles = (int)(((long long)p.seq.n_tok * a.group + ROWS - 1) / ROWS), units = attn_units(p.seq);
+	const long long in_seq = i - work.start[p.s];
+	const int parts = w.share == PARTS ? (units + w.part_units - 1) / w.part_units : 1;
+	const long long item = attn_div(in_seq, w.share == EVEN ? units : parts);
+	const int rest = (int)(in_seq - item * (w.share == EVEN ? units : parts));
+	if (w.share == WHOLE) {
+		p.row0 = (tiles - 1 - (int)attn_div(item, kv.n_head_kv)) * ROWS;
+		p.head = (int)(item % kv.n_head_kv);
+	} else {
+		p.head = (int)attn_div(item, tiles);
+		p.row0 = (int)(item - (long long)p.head * tiles) * ROWS;
+	}
+	const int first_tok = p.row0 / a.group, last_tok = min((p.row0 + ROWS - 1) / a.group, p.seq.n_tok - 1);
+	p.key_end = p.seq.kv_len + (st.tree ? p.seq.n_tok : last_tok + 1);
+	p.all_see = p.seq.kv_len + (st.tree ? 0 : first_tok + 1);
+	const int used = (p.key_end + ATTN_UNIT - 1) / ATTN_UNIT;  // units that some row sees keys of
+	p.n_parts = 1;
+	if (w.share == EVEN) {
+		p.unit0 = rest;
+		p.unit1 = (int)min((long long)units, rest + (w.u_end - w.u));
+		p.whole = p.unit0 == 0 && p.unit1 == units;
+		if (p.unit0 == 0 && !p.whole)  // the item goes on in the next CTAs
+			p.n_parts = attn_cta_of(i + units - 1, w.total, w.n_cta) - (int)blockIdx.x + 1;
+		w.u += p.unit1 - p.unit0;
+	} else {
+		p.unit0 = (int)((long long)used * rest / parts);
+		p.unit1 = (int)((long long)used * (rest + 1) / parts);
+		p.whole = parts == 1;
+		if (rest == 0)
+			p.n_parts = parts;
+		w.u++;
+	}
+	p.first = w.share == EVEN ? p.unit0 == 0 : rest == 0;
+	p.n_tiles = max(0, (min(p.unit1 * ATTN_UNIT, p.key_end) - p.unit0 * ATTN_UNIT + TK - 1) / TK);
 	return true;
 }
 
-// Whole items where each CTA has several, else their units shared out evenly.
 template <int N>
 __device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, const StepView &st, const AttnArgs &a, int n_cta, int cta)
 {
 	Walk w = {};
+	w.n_cta = n_cta;
 	attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS); });
 	w.total = work.start[st.n_seq];
-	w.n_cta = n_cta;
-	w.shared = w.total < 3ll * n_cta;
-	if (w.shared) {
+	w.share = WHOLE;
+	const long long items = w.total;
+	if (items == 0 || items >= 3ll * n_cta)
+		return w;
+	__syncthreads();
+	attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
+	const long long units = work.start[st.n_seq];
+	const int even = (int)min(attn_div(units + n_cta - 1, n_cta), 1ll << 30);
+	if (items <= n_cta) {
+		// the smallest part size with which there are no more parts than CTAs, tried in steps of an eighth; not kept where it
+		// costs more than a second piece in each CTA would
+		w.share = PARTS;
+		for (w.part_units = even; w.part_units <= even + PIECE_UNITS || st.n_seq == 1; w.part_units += max(1, w.part_units >> 3)) {
+			__syncthreads();
+			attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * ((attn_units(q) + w.part_units - 1) / w.part_units); });
+			w.total = work.start[st.n_seq];
+			if (w.total <= n_cta) {
+				w.u = cta;
+				w.u_end = cta < w.total ? cta + 1 : cta;
+				return w;
+			}
+		}
 		__syncthreads();
 		attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
-		w.total = work.start[st.n_seq];
-		w.n_cta = (int)min((long long)n_cta, w.total);
-		if (cta < w.n_cta) {
-			w.u = attn_div(w.total * cta, w.n_cta);
-			w.u_end = attn_div(w.total * (cta + 1), w.n_cta);
-		}
+	}
+	w.share = EVEN;
+	w.total = units;
+	w.n_cta = (int)min((long long)n_cta, units);
+	if (cta < w.n_cta) {
+		w.u = attn_div(w.total * cta, w.n_cta);
+		w.u_end = attn_div(w.total * (cta + 1), w.n_cta);
 	}
 	return w;
 }
@@ -759,8 +795,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 								      __float_as_uint(acc[2 * j + 1].y)));
 			}
 			bar_sync<1, SOFT_THREADS>();
-			const bool whole = p.unit0 == 0 && p.unit1 == p.item_units;
-			float *part = a.part + (2 * blockIdx.x + (p.unit0 == 0 ? 1 : 0)) * attn_part_floats(ROWS);
+			const bool whole = p.whole;
+			float *part = a.part + (2 * blockIdx.x + (p.first ? 1 : 0)) * attn_part_floats(ROWS);
 			if (wg == 0) {
 				const float2 other = sh->ml[r];
 				const float top = fmaxf(m, other.x);
@@ -872,15 +908,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		} else if (lane == 0) {
 			Piece p;
 			Walk walk_on = walk;
+			AttnJoin join = {0, 0, 0, 0, 0};
 			for (uint32_t n = 0;; n++) {
 				const bool any = next_piece<T::TK>(walk_on, p, work, kv, st, a);
-				if (!any) {
-					// the last piece's item goes on in other CTAs: its join
-					AttnJoin join = {0, 0, 0, 0, 0};
-					if (n > 0 && walk.shared && p.unit0 == 0 && p.unit1 < p.item_units) {
-						const long long i0 = walk_on.u - p.unit1;
-						join = {attn_cta_of(i0 + p.item_units - 1, walk.total, walk.n_cta) - (int)blockIdx.x + 1, p.seq.tok0, p.head, p.row0, p.seq.n_tok * a.group};
-					}
+				if (any) {
+					join = {0, 0, 0, 0, 0};
+					if (p.first && !p.whole)  // the CTA's last piece: its item goes on in others
+						join = {p.n_parts, p.seq.tok0, p.head, p.row0, p.seq.n_tok * a.group};
+				} else {
 					a.join[blockIdx.x] = join;
 					p.s = -1;
 				}
