@@ -154,8 +154,8 @@ int tie_cuda_moe_block_inplace(tie_cuda_ctx *c, int layer, float *hidden_dev, in
 
 /* The same for n_layers consecutive layers, first_layer first: hidden += MoE_l(RMSNorm_l(hidden)) layer
  * after layer, the residual stream staying on the device — the FFN halves of a stack of MoE blocks
- * with nothing between them (a model's attention halves, model_qwen3.c:303-389, are not part of
- * this library; a caller that has them calls tie_cuda_moe_block_inplace per layer).  The layers'
+ * with nothing between them (a layer's attention half is tie_cuda_attn_block_inplace; a
+ * caller that runs both calls the two in turn).  The layers'
  * kernels are enqueued back to back; with TIE_CUDA_GRAPH the whole stack replays from ONE CUDA
  * graph (one launch call per token instead of one per layer). */
 int tie_cuda_moe_stack_inplace(tie_cuda_ctx *c, int first_layer, int n_layers, float *hidden_dev, int n_tokens, unsigned flags);
@@ -327,6 +327,27 @@ int tie_cuda_kv_read(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_
  * meet the cache's elements in parts that keep 22 bits (BF16: 24).  out may be q. */
 int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const float *q, int n_head,
 		  float scale, float *out, unsigned flags);
+
+/* hidden += Wo . attention(rotate(norm(Wq . x)), the cache with rotate(norm(Wk . x)) and Wv . x written into it), x =
+ * RMSNorm(hidden) * norm_w: the attention half of a layer, model_qwen3.c:303-389, as tie_cuda_moe_block_inplace is its
+ * feed-forward half; the two together are a layer of the model.  hidden_dev: device fp32 [step->n_tokens][hidden]; rows
+ * that no sequence has are left as they are.  The four projections are tensors registered with tie_cuda_register_tensor
+ * (Q4_K or Q6_K, named by their host addresses; wq [n_head * head_dim][hidden], wk and wv [n_head_kv * head_dim][hidden], wo
+ * [hidden][n_head * head_dim]; as for tie_cuda_mat_mat rows in multiples of 128 and inputs in multiples of 256, else
+ * TIE_CUDA_ENOTSUP); the norms' weights are device memory, 16-byte aligned, or NULL.  Uses the config's norm_eps for all three norms.
+ * step->n_tokens is at most max_tokens, and what the projections put out has to fit the context's scratch (n_tokens * (n_head +
+ * 2 n_head_kv) * head_dim floats in max_tokens * top_k * hidden; TIE_CUDA_ETOOBIG).  TIE_CUDA_GRAPH is ignored; with
+ * TIE_CUDA_NO_SYNC a caller may capture the call. */
+typedef struct {
+	int n_head;
+	const void *wq, *wk, *wv, *wo;
+	const float *norm_w, *q_norm_w, *k_norm_w;
+	float rope_base;
+	int rope_interleaved;
+	float scale; /* of q . k; 0: 1 / sqrt(head_dim) */
+} tie_cuda_attn_weights;
+int tie_cuda_attn_block_inplace(tie_cuda_ctx *c, const tie_cuda_attn_weights *w, const tie_cuda_kv_cache *cache,
+				const tie_cuda_kv_step *step, float *hidden_dev, unsigned flags);
 
 /* ---- math_dispatch.c rows (accel = 2) ----
  * Same argument meaning as the reference's kernels are CALLED with (math_dispatch.c:224,254):

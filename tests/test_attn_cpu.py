@@ -83,7 +83,8 @@ def test_no_context_host_pointers_and_null_descriptions_are_refused(lib):
 def test_descriptions_have_the_layout_of_the_header(tmp_path):
     """Field offsets of the ctypes structures against the header's, as a C compiler sees them."""
     from tie_b200 import moe
-    pairs = [("tie_cuda_kv_cache", moe.KvCache), ("tie_cuda_kv_step", moe.KvStep), ("tie_cuda_attn_qkv", moe.AttnQkv)]
+    pairs = [("tie_cuda_kv_cache", moe.KvCache), ("tie_cuda_kv_step", moe.KvStep), ("tie_cuda_attn_qkv", moe.AttnQkv),
+             ("tie_cuda_attn_weights", moe.AttnWeights)]
     body = "".join(f'printf("%zu\\n", offsetof({n}, {f}));' for n, t in pairs for f, _ in t._fields_)
     body += "".join(f'printf("%zu\\n", sizeof({n}));' for n, _ in pairs)
     src = tmp_path / "o.c"

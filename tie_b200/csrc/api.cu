@@ -1764,6 +1764,68 @@ int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cud
 	return check_status(c);
 }
 
+// The registered tensor at host address w as the dense products take it.
+static int dense_tensor(tie_cuda_ctx *c, const void *w, int in_dim, int out_dim, const DevTensor **t)
+{
+	const tie_cuda_ctx::Reg *reg = nullptr;
+	for (int i = 0; i < c->n_regs; i++)
+		if (c->regs[i].host == w)
+			reg = &c->regs[i];
+	if (!reg || reg->k != in_dim || reg->rows != out_dim)
+		return TIE_CUDA_EINVAL;
+	if (!reg->dense || !tc_dense_supported(c, *reg->dense))
+		return TIE_CUDA_ENOTSUP;
+	*t = reg->dense;
+	return TIE_CUDA_OK;
+}
+
+int tie_cuda_attn_block_inplace(tie_cuda_ctx *c, const tie_cuda_attn_weights *w, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step,
+				float *hidden_dev, unsigned flags)
+{
+	KvView kv;
+	StepView st;
+	bool idle;
+	TRY(kv_views(c, cache, step, flags, kv, st, idle));
+	if (!w || !w->wq || !w->wk || !w->wv || !w->wo || !aligned16(w->norm_w) || ((uintptr_t)w->q_norm_w | (uintptr_t)w->k_norm_w) & 3 ||
+	    !(w->rope_base >= 0.0f) || w->rope_base > FLT_MAX || !(fabsf(w->scale) <= FLT_MAX))
+		return TIE_CUDA_EINVAL;
+	TRY(attn_heads(cache, w->n_head));
+	const int T = step->n_tokens, H = c->cfg.hidden, d = cache->head_dim, qw = w->n_head * d, kw = cache->n_head_kv * d;
+	const DevTensor *wq, *wk, *wv, *wo;
+	TRY(dense_tensor(c, w->wq, H, qw, &wq));
+	TRY(dense_tensor(c, w->wk, H, kw, &wk));
+	TRY(dense_tensor(c, w->wv, H, kw, &wv));
+	TRY(dense_tensor(c, w->wo, qw, H, &wo));
+	if (idle)
+		return TIE_CUDA_OK;
+	if (!hidden_dev || !aligned16(hidden_dev) || T > c->cfg.max_tokens)
+		return TIE_CUDA_EINVAL;
+	Scratch &s = c->s;
+	const size_t F = c->cfg.ffn_dim, y_cap = s.rows_cap * ((size_t)H > 2 * F ? H : 2 * F);
+	// (a token box of up to 64 rows may start at the last row: keep that much of the views beyond the batch)
+	if ((size_t)T * (qw + 2 * kw) > y_cap || (size_t)T > s.rows_cap || (size_t)T + 64 > wq->view->rows || (size_t)T + 64 > wo->view->rows)
+		return TIE_CUDA_ETOOBIG;
+	TIE_CUDA_TRY(c, cudaSetDevice(c->device));
+	c->tc_no_pair = (flags & TIE_CUDA_PATH_NO_PAIR) != 0;
+	float *q = s.y, *k = q + (size_t)T * qw, *v = k + (size_t)T * kw;
+	TRY(launch_rms_norm(c, hidden_dev, w->norm_w, s.x, T));
+	// the three projections share the split of their input (and its sub-block sums, for the Q4_K ones)
+	const bool sums = wq->kind == W_Q4K || wk->kind == W_Q4K || wv->kind == W_Q4K;
+	TRY(launch_split_rows(c, s.x, T, H, s.xs_hi, s.xs_hi + wq->view->lo_off, sums ? s.xq : nullptr));
+	TRY(launch_tc_dense(c, *wq, T, q));
+	TRY(launch_tc_dense(c, *wk, T, k));
+	TRY(launch_tc_dense(c, *wv, T, v));
+	const tie_cuda_attn_qkv in = {w->n_head, q, k, v, qw, kw, kw, w->q_norm_w, w->k_norm_w, c->cfg.norm_eps, w->rope_base, w->rope_interleaved, q};
+	TRY(launch_qk_norm_rope(c, kv, st, cache->type, d, in));
+	TRY(launch_attn(c, kv, st, cache->type, d, q, q, w->n_head, w->scale != 0.0f ? w->scale : 1.0f / sqrtf((float)d)));
+	TRY(launch_split_rows(c, q, T, qw, s.xs_hi, s.xs_hi + wo->view->lo_off, wo->kind == W_Q4K ? s.xq : nullptr));
+	TRY(launch_tc_dense(c, *wo, T, s.out));
+	TRY(launch_add_sequence_rows(c, kv, st, hidden_dev, s.out));
+	if (flags & TIE_CUDA_NO_SYNC)
+		return TIE_CUDA_OK;
+	return check_status(c);
+}
+
 // ---- math_dispatch rows ----
 
 int tie_cuda_make_current(tie_cuda_ctx *c)
@@ -1851,16 +1913,10 @@ int tie_cuda_mat_mat(tie_cuda_ctx *c, const void *w_host, const float *x, float 
 {
 	if (!c || !w_host || !x || !o || batch_len <= 0 || in_dim <= 0 || out_dim <= 0)
 		return TIE_CUDA_EINVAL;
-	const tie_cuda_ctx::Reg *reg = nullptr;
-	for (int i = 0; i < c->n_regs; i++)
-		if (c->regs[i].host == w_host)
-			reg = &c->regs[i];
-	if (!reg || reg->k != in_dim || reg->rows != out_dim)
-		return TIE_CUDA_EINVAL;
-	if (!reg->dense || !tc_dense_supported(c, *reg->dense))
-		return TIE_CUDA_ENOTSUP;
+	const DevTensor *t;
+	TRY(dense_tensor(c, w_host, in_dim, out_dim, &t));
 	Scratch &s = c->s;
-	const DenseView &v = *reg->dense->view;
+	const DenseView &v = *t->view;
 	const size_t T = c->cfg.max_tokens, H = c->cfg.hidden, F = c->cfg.ffn_dim;
 	const size_t y_cap = s.rows_cap * (H > 2 * F ? H : 2 * F);
 	// (a token box of up to 64 rows may start at the last row: keep that much of the view beyond the batch)
@@ -1879,9 +1935,9 @@ int tie_cuda_mat_mat(tie_cuda_ctx *c, const void *w_host, const float *x, float 
 		o_dev = s.y;
 	}
 	// the batch, split into fp16 hi + lo (and its sub-block sums for Q4_K), in the tensor's view of the x arrays
-	const bool sums = reg->dense->kind == W_Q4K;
+	const bool sums = t->kind == W_Q4K;
 	TRY(launch_split_rows(c, x_dev, batch_len, in_dim, s.xs_hi, s.xs_hi + v.lo_off, sums ? s.xq : nullptr));
-	TRY(launch_tc_dense(c, *reg->dense, batch_len, o_dev));
+	TRY(launch_tc_dense(c, *t, batch_len, o_dev));
 	if (!dev) {
 		TIE_CUDA_TRY(c, cudaMemcpyAsync(o, o_dev, (size_t)batch_len * out_dim * sizeof(float), cudaMemcpyDeviceToHost, c->stream));
 		return check_status(c);

@@ -80,6 +80,7 @@ int launch_kv_read(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int ki
 size_t attn_scratch_floats(const tie_cuda_ctx *c);
 int attn_setup(tie_cuda_ctx *c);
 int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale);
+int launch_add_sequence_rows(tie_cuda_ctx *c, const KvView &kv, const StepView &st, float *hidden, const float *y);  // misc.cu
 // ep.cu
 int launch_ep_signal(tie_cuda_ctx *c, int which);
 int launch_ep_push_tokens(tie_cuda_ctx *c, const float *x, int n_tokens);

@@ -2,6 +2,7 @@
 // the fp16 hi/lo split of activations for the tensor-core path, and the table SwiGLU on its own.
 #include "common.cuh"
 #include "kernels.cuh"
+#include "kv_cache.cuh"
 #include "split8.cuh"
 
 namespace tie {
@@ -197,6 +198,29 @@ int launch_gather_rows(tie_cuda_ctx *c, const float *x, const int *row_expert, c
 		       float *rows_out, int *expert_out, int *inv)
 {
 	gather_rows<<<n_rows, 256, 0, c->stream>>>(x, row_expert, perm, src_div, c->cfg.hidden, rows_out, expert_out, inv);
+	TIE_CUDA_LAUNCHED(c);
+	return TIE_CUDA_OK;
+}
+
+// hidden[t] += y[t] for the tokens that a sequence of the step has (and has a slot for); a CTA a token.
+__global__ void __launch_bounds__(128) add_sequence_rows(const StepView st, int page_shift, float *hidden, const float *y, int n)
+{
+	const int t = blockIdx.x, s = kv_find_sequence(st, t, threadIdx.x & 31);
+	if (s < 0)
+		return;
+	const SeqView seq = kv_sequence(st, page_shift, s);
+	if (t < seq.tok0 || t - seq.tok0 >= seq.n_tok)
+		return;
+	float4 *h = reinterpret_cast<float4 *>(hidden + (size_t)t * n);
+	const float4 *v = reinterpret_cast<const float4 *>(y + (size_t)t * n);
+	for (int i = threadIdx.x; i < n / 4; i += 128) {
+		const float4 a = h[i], b = v[i];
+		h[i] = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+	}
+}
+int launch_add_sequence_rows(tie_cuda_ctx *c, const KvView &kv, const StepView &st, float *hidden, const float *y)
+{
+	add_sequence_rows<<<st.n_tokens, 128, 0, c->stream>>>(st, kv.page_shift, hidden, y, c->cfg.hidden);
 	TIE_CUDA_LAUNCHED(c);
 	return TIE_CUDA_OK;
 }

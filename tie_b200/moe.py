@@ -37,6 +37,7 @@ EXPORTS = [
     "tie_cuda_ep_attach", "tie_cuda_ep_detach", "tie_cuda_ep_set_timeout_ms", "tie_cuda_ep_publish", "tie_cuda_ep_compute",
     "tie_cuda_ep_gather", "tie_cuda_moe_ffn_ep", "tie_cuda_mat_mat",
     "tie_cuda_moe_block_inplace_ep", "tie_cuda_qk_norm_rope", "tie_cuda_kv_read", "tie_cuda_attn",
+    "tie_cuda_attn_block_inplace",
 ]
 EP_HANDLE_BYTES = 64
 EP_PEER_POINTERS, EP_PEER_IPC_HANDLES = 0, 1
@@ -161,6 +162,8 @@ def load_library() -> ctypes.CDLL:
     L.tie_cuda_qk_norm_rope.argtypes = [vp, vp, vp, vp, u32]
     L.tie_cuda_kv_read.restype = i32
     L.tie_cuda_kv_read.argtypes = [vp, vp, vp, vp, vp, i32, u32]
+    L.tie_cuda_attn_block_inplace.restype = i32
+    L.tie_cuda_attn_block_inplace.argtypes = [vp, vp, vp, vp, vp, u32]
     L.tie_cuda_attn.restype = i32
     L.tie_cuda_attn.argtypes = [vp, vp, vp, vp, i32, f32, vp, u32]
     _lib = L
@@ -228,6 +231,21 @@ class AttnQkv(ctypes.Structure):
         ("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p), ("norm_eps", ctypes.c_float),
         ("rope_base", ctypes.c_float), ("rope_interleaved", ctypes.c_int), ("q_out", ctypes.c_void_p),
     ]
+
+
+class AttnWeights(ctypes.Structure):
+    """tie_cuda_attn_weights: wq, wk, wv, wo are the host arrays given to register_tensor; the norms' weights are device tensors."""
+    _fields_ = [
+        ("n_head", ctypes.c_int), ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("wv", ctypes.c_void_p), ("wo", ctypes.c_void_p),
+        ("norm_w", ctypes.c_void_p), ("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p), ("rope_base", ctypes.c_float),
+        ("rope_interleaved", ctypes.c_int), ("scale", ctypes.c_float),
+    ]
+
+    def __init__(self, n_head: int, wq, wk, wv, wo, norm_w=None, q_norm_w=None, k_norm_w=None, rope_base: float = 1e6,
+                 rope_interleaved: bool = False, scale: float = 0.0):
+        super().__init__(n_head, _ptr(wq), _ptr(wk), _ptr(wv), _ptr(wo), _ptr(norm_w), _ptr(q_norm_w), _ptr(k_norm_w), rope_base,
+                         int(rope_interleaved), scale)
+        self.keep = (wq, wk, wv, wo, norm_w, q_norm_w, k_norm_w)
 
 
 def _rows_ptr(a, width: int):
@@ -460,6 +478,10 @@ class MoeBackend:
     def attn_ptr(self, cache: KvCache, step: KvStep, q, out, n_head: int, scale: float, flags: int = DEVICE):
         rc = self.L.tie_cuda_attn(self.h, ctypes.byref(cache), ctypes.byref(step), _ptr(q), n_head, scale, _ptr(out), flags)
         self._check(rc, "tie_cuda_attn")
+
+    def attn_block_inplace_ptr(self, weights: AttnWeights, cache: KvCache, step: KvStep, hidden, flags: int = DEVICE):
+        rc = self.L.tie_cuda_attn_block_inplace(self.h, ctypes.byref(weights), ctypes.byref(cache), ctypes.byref(step), _ptr(hidden), flags)
+        self._check(rc, "tie_cuda_attn_block_inplace")
 
     # -- math_dispatch rows --
     def make_current(self):
