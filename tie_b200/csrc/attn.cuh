@@ -37,7 +37,7 @@ __host__ __device__ constexpr size_t attn_part_floats(int rows)
 // CTAs, so that the result does not depend on which was last.
 struct AttnWork {
 	long long start[KV_MAX_SEQ + 1];  // units (or items) in front of a sequence
-	long long warp_sum[16];
+	long long warp_sum[32];
 	int last;
 };
 

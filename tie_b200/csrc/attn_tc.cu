@@ -8,9 +8,10 @@
 // keys, since tensor memory holds no more.  The products of a tile start from zero and are added to fp32 registers: the
 // tensor cores cut every sum off, which over a long cache would add up.
 //
-// One CTA per SM, 512 threads:
-//   * two warpgroups of softmax threads, a thread per row, take key tiles in turn, each with a running maximum, sum and
-//     output row of its own (joined at the end), so that one's exponentials run under the other's MMAs;
+// One CTA per SM, 640 threads:
+//   * two warpgroups of softmax threads, a thread per row, take key tiles in turn, each with a running maximum and sum of its own,
+//     so that one's exponentials run under the other's MMAs; a third adds the tiles' products up, a thread per row, with the
+//     row in registers (where the softmax threads did that too, they waited for half of the time for products);
 //   * a warp requests keys, another values, by TMA straight into the swizzled operand layout, a box per page (as one
 //     cp.async per 16 bytes the address arithmetic alone took 5000 cycles a tile from two warps);
 //   * two warps each make operands of what came in where it is not one yet: Q8's bytes become fp16 in place, values behind
@@ -30,11 +31,12 @@ namespace tie {
 namespace {
 
 constexpr int ROWS = ATTN_MAX_ROWS;
-constexpr int THREADS = 512, SOFT_THREADS = 256, MAKE_THREADS = 64;
-constexpr int W_KEYS = 8, W_VALUES = 10, W_MMA = 12, W_PIECES = 13, W_ASK = 14;  // first warps of the roles behind the softmax warps
-constexpr int SOFT_REGS = 192, MAKE_REGS = 80, REST_REGS = 48;
-static_assert(2 * SOFT_REGS + MAKE_REGS + REST_REGS <= 512, "a launch of 512 threads holds 128 registers a thread");
+constexpr int THREADS = 640, SOFT_THREADS = 256, FOLD_THREADS = 128, MAKE_THREADS = 64;
+constexpr int W_FOLD = 8, W_KEYS = 12, W_VALUES = 14, W_MMA = 16, W_PIECES = 17, W_ASK = 18;	// first warps of the roles behind the softmax warps
+constexpr int SOFT_REGS = 104, FOLD_REGS = 176, MAKE_REGS = 56, REST_REGS = 40;
+static_assert(2 * SOFT_REGS + FOLD_REGS + MAKE_REGS + REST_REGS <= 5 * 96, "a launch of 640 threads holds 96 registers a thread");
 constexpr long long WAIT_CYCLES = 1ll << 30;
+constexpr int OUT_BYTES = ROWS * 16 * 4;  // 16 dims of a tile's rows, on their way out
 
 // A piece of work of a CTA: an item, or (few items: shared) some units of one.  No more of them: s < 0.
 struct Piece {
@@ -53,7 +55,7 @@ struct Shared {
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
 	uint64_t k_raw[MAX_STAGES], k_full[MAX_STAGES], k_free[MAX_STAGES];  // keys have come in; are the operand; have been used
 	uint64_t v_raw[MAX_STAGES], v_full[MAX_STAGES], v_free[MAX_STAGES];
-	uint64_t s_full[2], p_full[2], o_full[2], o_free, q_full, fin;	// (a warpgroup's own where only it waits: it sees every phase)
+	uint64_t s_full[2], p_full[2], o_full, o_free, q_full, ml_full[2], fin;	 // (one for each warpgroup, or piece, in turn where only these wait: they see every phase)
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
 	// made: tile n + FACTS is requested after the scores of tile n + 2 at the least, these after the products of n.
 	uint64_t f_full[MAX_FACTS];
@@ -63,7 +65,10 @@ struct Shared {
 	float v_top[2], make_max[2][2];
 	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
 	float q_max[2][ROWS];
-	float2 ml[ROWS];
+	// what the products of a tile have to be added up with: maximum of a row, factor; whether values are no numbers, bad pages
+	float t_top[4][ROWS], t_unit[4];
+	uint32_t t_odd[4], t_bad[4];
+	float2 ml[2][2][ROWS];	// per piece in turn and warpgroup: maximum and sum of a row
 	uint32_t tmem_base, abort;
 };
 
@@ -71,7 +76,7 @@ struct Shared {
 // they belong to (a CTA then mostly has the end of one and the beginning of another).  PARTS: no more items than CTAs,
 // each cut into as many equal parts as leave one part to a CTA.
 enum Share : int { WHOLE, EVEN, PARTS };
-// What a piece costs besides its tiles (set-up, first loads, joins), in units: 20,000 cycles against 2500 a unit.
+// What a piece costs besides its tiles (set-up, first loads, joins), in units.
 constexpr int PIECE_UNITS = 8;
 struct Walk {
 	Share share;
@@ -192,7 +197,7 @@ struct Tile {
 	static constexpr int ROW = SCALED ? D : 2 * D;	 // bytes of a head row of the cache
 	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128, BOXES = ROW / BOX_BYTES;  // of a row, per TMA box
 	static constexpr uint32_t RAW = SCALED && D == 64 ? TK * ROW : 0;  // rows of 64 bytes come in beside the operand
-	static constexpr size_t SMEM = 2 * (size_t)STAGES * (BYTES + RAW) + (size_t)ROWS * D * 4 + 1024;
+	static constexpr size_t SMEM = 2 * (size_t)STAGES * (BYTES + RAW) + (size_t)ROWS * D * 4 + OUT_BYTES + 1024;
 	// where a 16-byte chunk of row r's 16-bit values lies in the operand tile
 	__device__ static __forceinline__ uint32_t place(int r, int ch) { return (ch >> 3) * PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
 };
@@ -303,6 +308,41 @@ __device__ __forceinline__ uint32_t finite16(uint32_t w, uint32_t exponent)
 	return ((w & exponent) == exponent ? 0u : 0xffffu) | ((w >> 16 & exponent) == exponent ? 0u : 0xffff0000u);
 }
 
+// Which keys a query row sees.
+struct RowView {
+	bool tree;
+	int kv_len, sees_to;
+	unsigned long long bits;  // tree: the step's tokens
+	// of 32 keys from `key` on, without those of bad pages (a bit per 16)
+	__device__ __forceinline__ uint32_t keys(int key, uint32_t bad) const
+	{
+		uint32_t vis = ~0u;
+		if (tree) {
+			const int j = key - kv_len;
+			if (j >= 0)
+				vis = j < 64 ? (uint32_t)(bits >> j) : 0u;
+			else if (j > -32)
+				vis = ((1u << -j) - 1u) | (uint32_t)bits << -j;
+		} else {
+			const int n = sees_to - key;
+			vis = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+		}
+		return vis & ~((bad & 1 ? 0x0000ffffu : 0u) | (bad & 2 ? 0xffff0000u : 0u));
+	}
+};
+__device__ __forceinline__ RowView row_view(const StepView &st, const Piece &p, int tok, bool report)
+{
+	RowView v = {st.tree != nullptr, p.seq.kv_len, p.seq.kv_len + tok + 1, 0};
+	if (st.tree) {
+		v.bits = st.tree[p.seq.tok0 + tok];
+		if (p.seq.n_tok < 64)
+			v.bits &= (1ull << p.seq.n_tok) - 1;
+		else if (p.seq.n_tok > KV_MAX_TREE && report)
+			kv_report(st, ST_BAD_STEP);
+	}
+	return v;
+}
+
 // Requests the tiles of keys (VALUES false) or values: a warp, a lane per page of a tile.
 template <int KIND, int D, bool VALUES>
 __device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared *sh, const CUtensorMap *map, uint32_t ring, uint32_t raw, const Waiter &wait,
@@ -386,7 +426,7 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 			// the keys that are somebody's: the others' values are zeros, whatever has come in
 			auto there = [&](int r) { return key0 + r < p.key_end && !(bad >> (r >> 4) & 1u); };
 			if constexpr (T::SCALED) {
-				constexpr int CHUNKS = T::ROW / 16, AT_ONCE = MAKE_THREADS / CHUNKS, PASSES = T::TK / AT_ONCE, B = 8;
+				constexpr int CHUNKS = T::ROW / 16, AT_ONCE = MAKE_THREADS / CHUNKS, PASSES = T::TK / AT_ONCE, B = 4;
 				const int ch = t % CHUNKS, r0 = t / CHUNKS;
 #pragma unroll 1
 				for (int j0 = 0; j0 < PASSES; j0 += B) {
@@ -482,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
 	constexpr int TK = T::TK;
 	const uint32_t k_ring = smem, v_ring = k_ring + T::STAGES * T::BYTES, k_raw = v_ring + T::STAGES * T::BYTES, v_raw = k_raw + T::STAGES * T::RAW;
-	const uint32_t hand = v_raw + T::STAGES * T::RAW;
+	const uint32_t hand = v_raw + T::STAGES * T::RAW, out_stage = hand + ROWS * D * 4;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	if (threadIdx.x == 0) {
 		for (int i = 0; i < T::STAGES; i++) {
@@ -496,15 +536,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		for (int i = 0; i < 2; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->s_full[i]), 1);
 			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS / 2);
-			ptx::mbar_init(ptx::smem_u32(&sh->o_full[i]), 1);
+			ptx::mbar_init(ptx::smem_u32(&sh->ml_full[i]), SOFT_THREADS);
 		}
 		for (int i = 0; i < T::FACTS; i++)
 			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), T::SCALED ? MAKE_THREADS : 1);
 		for (int i = 0; i < PIECES; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->piece_full[i]), 1);
-			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), SOFT_THREADS / 32 + 1 + 2 + (T::SCALED ? 4 : 2));  // softmax, MMA, ask, make
+			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), SOFT_THREADS / 32 + FOLD_THREADS / 32 + 1 + 2 + (T::SCALED ? 4 : 2));  // softmax, fold, MMA, ask, make
 		}
-		ptx::mbar_init(ptx::smem_u32(&sh->o_free), SOFT_THREADS / 2);
+		ptx::mbar_init(ptx::smem_u32(&sh->o_full), 1);
+		ptx::mbar_init(ptx::smem_u32(&sh->o_free), FOLD_THREADS);
 		ptx::mbar_init(ptx::smem_u32(&sh->q_full), SOFT_THREADS);
 		ptx::mbar_init(ptx::smem_u32(&sh->fin), 1);
 		sh->abort = 0;
@@ -522,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	const uint32_t tmem = sh->tmem_base;
 	const Waiter wait = {&sh->abort, st.status};
 
-	if (warp < W_KEYS) {
+	if (warp < W_FOLD) {
 		// ================= softmax: a thread per row and warpgroup =================
 		ptx::setmaxnreg_inc<SOFT_REGS>();
 		const int wg = threadIdx.x >> 7, r = threadIdx.x & 127;
@@ -553,7 +594,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			// 4 dims of a row of the tile, in shared memory: no conflicts, neither along a row nor across the rows
 			auto spot = [&](int d4, int line) { return hand + ((uint32_t)d4 * ROWS + (line ^ (d4 & 7))) * 16; };
 			float row_scale = 0.0f;
-			bar_sync<1, SOFT_THREADS>();  // shared memory has nothing of the piece before any more
+			bar_sync<1, SOFT_THREADS>();  // nobody reads rows or makes scores of the piece before any more
 			if (p.n_tiles > 0) {
 				// The rows as they lie, through shared memory (a thread's own row from global memory: 32 lines a load), and this
 				// thread's half of its row, in parts, into tensor memory.
@@ -601,20 +642,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tc_fence_before();
 				ptx::mbar_arrive(ptx::smem_u32(&sh->q_full));
 			}
-			unsigned long long bits = 0;  // tree: the step's tokens that this row sees
-			if (st.tree) {
-				bits = st.tree[p.seq.tok0 + tok];
-				if (p.seq.n_tok < 64)
-					bits &= (1ull << p.seq.n_tok) - 1;
-				else if (p.seq.n_tok > KV_MAX_TREE && r == 0)
-					kv_report(st, ST_BAD_STEP);
-			}
-			const int sees_to = p.seq.kv_len + tok + 1;  // no tree
-			float2 acc[HALF];
+			const RowView view = row_view(st, p, tok, r == 0);
 			float m = -INFINITY, l = 0.0f;
-#pragma unroll
-			for (int i = 0; i < HALF; i++)
-				acc[i] = make_float2(0.0f, 0.0f);
 			for (int i = 0; i < p.n_tiles; i++, tiles++) {
 				if ((int)(tiles & 1) != wg)
 					continue;
@@ -626,22 +655,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tc_fence_after();
 				const uint32_t bad = sh->bad[fslot];
 				const bool masked = key0 + TK > p.all_see || bad != 0;
-				// which of 32 keys this row sees
-				auto visible = [&](int c) {
-					const int key = key0 + 32 * c;
-					uint32_t vis = ~0u;
-					if (st.tree) {
-						const int j = key - p.seq.kv_len;
-						if (j >= 0)
-							vis = j < 64 ? (uint32_t)(bits >> j) : 0u;
-						else if (j > -32)
-							vis = ((1u << -j) - 1u) | (uint32_t)bits << -j;
-					} else {
-						const int n = sees_to - key;
-						vis = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-					}
-					return vis & ~((bad >> (2 * c) & 1 ? 0x0000ffffu : 0u) | (bad >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
-				};
 				// scores of 32 keys, times their rows' factors; -infinity where the row does not see
 				auto scores = [&](int c, float2 (&x)[16], bool scaled) {
 					uint32_t v[32];
@@ -659,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 						}
 					}
 					if (masked && !(T::SCALED && scaled)) {
-						const uint32_t vis = visible(c);
+						const uint32_t vis = view.keys(key0 + 32 * c, bad >> (2 * c));
 #pragma unroll
 						for (int k = 0; k < 16; k++) {
 							x[k].x = vis >> (2 * k) & 1 ? x[k].x : -INFINITY;
@@ -697,13 +710,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				m = top;
 				// the values' factors, and whether all of them are numbers; read before P is handed over: when its products are
 				// made the slot is another tile's
-				bool odd = false;
-				float v_top = 1.0f;
-				if (T::SCALED || masked) {
+				if (T::SCALED || masked)
 					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
-					odd = sh->odd[slot][0] | sh->odd[slot][1];
-					if constexpr (T::SCALED)
-						v_top = sh->v_top[slot];
+				sh->t_top[tiles & 3u][r] = top;
+				if (r == 0) {
+					sh->t_odd[tiles & 3u] = masked ? sh->odd[slot][0] | sh->odd[slot][1] : 0u;
+					sh->t_bad[tiles & 3u] = bad;
+					sh->t_unit[tiles & 3u] = T::SCALED ? sh->v_top[slot] : 1.0f;
 				}
 				float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
@@ -743,95 +756,118 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tc_fence_before();
 				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[wg]));
 				l = fmaf(l, alpha, sum.x + sum.y);
-				wait(sh->o_full[wg], ph);
+			}
+			sh->ml[n & 1u][wg][r] = make_float2(m, l);
+			ptx::mbar_arrive(ptx::smem_u32(&sh->ml_full[n & 1u]));
+		}
+	} else if (warp < W_KEYS) {
+		// ================= fold: a thread per row adds the tiles' products up =================
+		ptx::setmaxnreg_inc<FOLD_REGS>();
+		const int r = threadIdx.x & 127;
+		const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+		uint32_t tiles = 0;
+		for (uint32_t n = 0;; n++) {
+			const Piece p = take_piece(sh, wait, n);
+			drop_piece(sh, n, lane);
+			if (p.s < 0)
+				break;
+			const int n_rows = p.seq.n_tok * a.group, row = p.row0 + r;
+			const RowView view = row_view(st, p, row < n_rows ? row / a.group : p.seq.n_tok - 1, false);
+			float2 acc[HALF];
+			float top = -INFINITY;
+#pragma unroll
+			for (int i = 0; i < HALF; i++)
+				acc[i] = make_float2(0.0f, 0.0f);
+			for (int i = 0; i < p.n_tiles; i++, tiles++) {
+				const uint32_t at = tiles & 3u;
+				wait(sh->o_full, tiles & 1u);
 				ptx::tc_fence_after();
+				// relative to the largest maximum so far (the tiles' are those of the two warpgroups)
+				const float t_top = sh->t_top[at][r], next = fmaxf(top, t_top);
+				const float f = t_top == -INFINITY ? 0.0f : exp2_ftz(t_top - next) * sh->t_unit[at], g = top == -INFINITY ? 0.0f : exp2_ftz(top - next);
+				const bool odd = KIND != TIE_CUDA_KV_Q8 && sh->t_odd[at];
+				const uint32_t bad = sh->t_bad[at];
+				top = next;
+				const float2 f2 = make_float2(f, f), g2 = make_float2(g, g);
 #pragma unroll
 				for (int c = 0; c < D / 32; c++) {
 					uint32_t v[32];
 					ptx::tmem_ld32(lanes + T::COL_O + 32 * c, v);
 					ptx::tmem_ld_wait();
 #pragma unroll
-					for (int k = 0; k < 16; k++) {
-						const float2 o = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f = make_float2(alpha, alpha);
-						if constexpr (T::SCALED)
-							acc[16 * c + k] = fma2(o, make_float2(v_top, v_top), mul2(acc[16 * c + k], f));
-						else
-							acc[16 * c + k] = fma2(acc[16 * c + k], f, o);
-					}
+					for (int k = 0; k < 16; k++)
+						acc[16 * c + k] = fma2(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f2, mul2(acc[16 * c + k], g2));
 				}
 				ptx::tc_fence_before();
-				ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
-				if (KIND != TIE_CUDA_KV_Q8 && odd) {  // infinities and NaN among values that not every row sees: p > 0 times them is what they are
+				if (i == p.n_tiles - 1)	 // (what the piece is finished with is read before the piece after the next can be)
+					wait(sh->ml_full[n & 1u], n >> 1 & 1u);
+				if (odd) {  // infinities and NaN among values that not every row sees: p > 0 times them is what they are
+					const int key0 = p.unit0 * ATTN_UNIT + i * TK;
 #pragma unroll 1
-					for (int k = 0; k < TK; k++) {
-						if (key0 + k >= p.key_end)
-							break;
-						if (!(visible(k >> 5) >> (k & 31) & 1))
+					for (int k = 0; k < TK && key0 + k < p.key_end; k++) {
+						if (!(view.keys(key0 + (k & ~31), bad >> (k >> 4 & ~1)) >> (k & 31) & 1))
 							continue;
 						const int page = st.page_table[(long long)p.s * st.max_pages + ((key0 + k) >> kv.page_shift)];
-						const long long at = (((long long)page * kv.n_head_kv + p.head) << kv.page_shift) + ((key0 + k) & ((1 << kv.page_shift) - 1));
-						const uint32_t *src = reinterpret_cast<const uint32_t *>(kv.v + at * T::ROW);
+						const long long src_row = (((long long)page * kv.n_head_kv + p.head) << kv.page_shift) + ((key0 + k) & ((1 << kv.page_shift) - 1));
+						const uint32_t *src = reinterpret_cast<const uint32_t *>(kv.v + src_row * T::ROW);
 						constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
 						for (int d = 0; d < HALF; d++) {
 							const uint32_t x = src[d];
 							if (nonfinite16(x, EXPONENT)) {
-								const float2 f = KIND == TIE_CUDA_KV_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&x))
+								const float2 y = KIND == TIE_CUDA_KV_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&x))
 													 : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-								acc[d].x += (x & EXPONENT) == EXPONENT ? f.x : 0.0f;
-								acc[d].y += (x >> 16 & EXPONENT) == EXPONENT ? f.y : 0.0f;
+								acc[d].x += (x & EXPONENT) == EXPONENT ? y.x : 0.0f;
+								acc[d].y += (x >> 16 & EXPONENT) == EXPONENT ? y.y : 0.0f;
 							}
 						}
 					}
 				}
+				if (i < p.n_tiles - 1)
+					ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
 			}
-
-			// the two warpgroups' keys together: the second's through shared memory to the first
-			if (wg == 1) {
-				sh->ml[r] = make_float2(m, l);
+			if (p.n_tiles == 0)
+				wait(sh->ml_full[n & 1u], n >> 1 & 1u);
+			const float2 m0 = sh->ml[n & 1u][0][r], m1 = sh->ml[n & 1u][1][r];
+			if (p.n_tiles > 0)
+				ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
+			// the sums of p, as the products relative to the largest maximum
+			const float sum = (m0.x == -INFINITY ? 0.0f : m0.y * exp2_ftz(m0.x - top)) + (m1.x == -INFINITY ? 0.0f : m1.y * exp2_ftz(m1.x - top));
+			if (!p.whole) {
+				float *part = a.part + (2 * blockIdx.x + (p.first ? 1 : 0)) * attn_part_floats(ROWS);
+				part[ROWS * 128 + r] = top;
+				part[ROWS * 128 + ROWS + r] = sum;
 #pragma unroll
-				for (int j = 0; j < D4; j++)
-					sts128(spot(j, r), make_uint4(__float_as_uint(acc[2 * j].x), __float_as_uint(acc[2 * j].y), __float_as_uint(acc[2 * j + 1].x),
-								      __float_as_uint(acc[2 * j + 1].y)));
+				for (int j = 0; j < D4; j++)  // [4 dims][row]
+					reinterpret_cast<float4 *>(part)[j * ROWS + r] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
+				continue;
 			}
-			bar_sync<1, SOFT_THREADS>();
-			const bool whole = p.whole;
-			float *part = a.part + (2 * blockIdx.x + (p.first ? 1 : 0)) * attn_part_floats(ROWS);
-			if (wg == 0) {
-				const float2 other = sh->ml[r];
-				const float top = fmaxf(m, other.x);
-				// (a warpgroup whose keys the row does not see has sums of zero)
-				float own = m == -INFINITY ? 0.0f : exp2_ftz(m - top), theirs = other.x == -INFINITY ? 0.0f : exp2_ftz(other.x - top);
-				const float sum = l * own + other.y * theirs;
-				if (whole) {
-					const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-					own *= inv;
-					theirs *= inv;
-				} else {
-					part[ROWS * 128 + r] = top;
-					part[ROWS * 128 + ROWS + r] = sum;
-				}
-				const float2 f = make_float2(own, own), g = make_float2(theirs, theirs);
+			// whole rows go out by 16 dims through shared memory: 4 lanes then store 64 bytes of a row
+			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+			long long at[4];
 #pragma unroll
-				for (int j = 0; j < D4; j++) {
-					const uint4 x = lds128(spot(j, r));
-					const float2 y0 = fma2(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), g, mul2(acc[2 * j], f));
-					const float2 y1 = fma2(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), g, mul2(acc[2 * j + 1], f));
-					const uint4 y = make_uint4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y));
-					sts128(spot(j, r), y);
+			for (int i = 0; i < 4; i++) {
+				const int line = p.row0 + (warp & 3) * 32 + i * 8 + lane / 4, t = line / a.group;
+				at[i] = line < n_rows ? ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + (line - t * a.group)) * D + lane % 4 * 4 : -1;
+			}
+			const float2 i2 = make_float2(inv, inv);
+#pragma unroll
+			for (int c = 0; c < D / 16; c++) {
+				bar_sync<2, FOLD_THREADS>();
+#pragma unroll
+				for (int j = 0; j < 4; j++) {
+					const float2 y0 = mul2(acc[8 * c + 2 * j], i2), y1 = mul2(acc[8 * c + 2 * j + 1], i2);
+					sts128(out_stage + (j * ROWS + (r ^ j)) * 16, make_uint4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y)));
+				}
+				bar_sync<2, FOLD_THREADS>();
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					const int line = (warp & 3) * 32 + i * 8 + lane / 4, j = lane % 4;
+					const uint4 y = lds128(out_stage + (j * ROWS + (line ^ j)) * 16);
+					if (at[i] >= 0)
+						*reinterpret_cast<uint4 *>(a.out + at[i] + 16 * c) = y;
 				}
 			}
-			bar_sync<1, SOFT_THREADS>();
-			if (whole)
-				my_rows([&](int line, long long at) {
-					const uint4 y = lds128(spot(lane % D4, line));
-					if (p.row0 + line < n_rows)
-						*reinterpret_cast<uint4 *>(a.out + at) = y;
-				});
-			else
-#pragma unroll 4
-				for (int j = wg; j < D4; j += 2)  // [4 dims][row]
-					reinterpret_cast<uint4 *>(part)[j * ROWS + r] = lds128(spot(j, r));
 		}
 	} else if (warp < W_MMA) {
 		ptx::setmaxnreg_dec<MAKE_REGS>();
@@ -864,7 +900,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 										part < T::PARTS - 1 || k > 0);
 					}
 					ptx::mma_commit(ptx::smem_u32(&sh->v_free[slot]));
-					ptx::mma_commit(ptx::smem_u32(&sh->o_full[n & 1u]));
+					ptx::mma_commit(ptx::smem_u32(&sh->o_full));
 				};
 				Piece p;
 				for (uint32_t n = 0;; n++) {
