@@ -49,25 +49,25 @@ struct Piece {
 	int key_end;	// first key that nobody sees
 	int all_see;	// keys in front of this one are seen by every row
 };
-constexpr int PIECES = 4, MAX_STAGES = 4, MAX_FACTS = 8, MAX_TILE = 128;
+constexpr int PIECES = 4, MAX_STAGES = 4, MAX_SLOTS = 4, MAX_FACTS = 8, TILE_FACTS = 8;
 struct Shared {
 	uint64_t piece_full[PIECES], piece_free[PIECES];
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
 	uint64_t k_raw[MAX_STAGES], k_full[MAX_STAGES], k_free[MAX_STAGES];  // keys have come in; are the operand; have been used
 	uint64_t v_raw[MAX_STAGES], v_full[MAX_STAGES], v_free[MAX_STAGES];
-	uint64_t s_full[2], p_full[2], o_full, o_free, q_full, ml_full[2], fin;	 // (one for each warpgroup, or piece, in turn where only these wait: they see every phase)
+	uint64_t s_full[MAX_SLOTS], p_full[MAX_SLOTS], o_full, o_free, q_full, ml_full[2], fin;
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
-	// made: tile n + FACTS is requested after the scores of tile n + 2 at the least, these after the products of n.
+	// made: tile n + FACTS is requested after the scores of tile n + SLOTS at the least, these after the products of n.
 	uint64_t f_full[MAX_FACTS];
 	uint32_t bad[MAX_FACTS], bad_values[MAX_STAGES];  // groups of 16 keys of a tile whose page does not exist
-	alignas(16) float k_scale[MAX_FACTS][MAX_TILE];
-	alignas(16) float v_got[2][MAX_TILE], v_scale[2][MAX_TILE];
-	float v_top[2], make_max[2][2];
+	alignas(16) float k_scale[640];	 // [FACTS][TK]
+	alignas(16) float v_got[256], v_scale[256];  // [STAGES][TK]: factors as they came, and relative to the tile's largest
+	float v_top[MAX_STAGES], make_max[MAX_STAGES][2];
 	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
 	float q_max[2][ROWS];
 	// what the products of a tile have to be added up with: maximum of a row, factor; whether values are no numbers, bad pages
-	float t_top[4][ROWS], t_unit[4];
-	uint32_t t_odd[4], t_bad[4];
+	float t_top[TILE_FACTS][ROWS], t_unit[TILE_FACTS];
+	uint32_t t_odd[TILE_FACTS], t_bad[TILE_FACTS];
 	float2 ml[2][2][ROWS];	// per piece in turn and warpgroup: maximum and sum of a row
 	uint32_t tmem_base, abort;
 };
@@ -184,13 +184,17 @@ __device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, con
 template <int KIND, int D>
 struct Tile {
 	static constexpr bool SCALED = KIND == TIE_CUDA_KV_Q8;
-	static constexpr int TK = KIND == TIE_CUDA_KV_BF16 ? 64 : 128;	 // keys
 	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	 // of a value of Q and of P
-	static constexpr int STAGES = KIND == TIE_CUDA_KV_BF16 || (KIND == TIE_CUDA_KV_F16 && D == 64) ? 4 : 2;
-	static constexpr int FACTS = 2 * STAGES;
-	static_assert(FACTS >= STAGES + 2 && FACTS <= MAX_FACTS && STAGES <= MAX_STAGES && (!SCALED || STAGES == 2), "rings");
-	// tensor memory: parts of Q, two score tiles (and what P's parts need beyond their columns), O
-	static constexpr int SLOT = PARTS == 3 ? TK + TK / 2 : TK, COL_Q = 0, COL_S = PARTS * D / 2, COL_O = COL_S + 2 * SLOT;
+	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  More than two let a warpgroup work on one
+	// tile while the products of its last and the scores of its next are made (with two tiles of 128 keys it waited for half of
+	// the time).
+	static constexpr int TK = PARTS == 3 || D == 128 ? 64 : 128;
+	static constexpr int SLOTS = PARTS == 3 ? (D == 128 ? 2 : 3) : (D == 128 ? 4 : 3);
+	static constexpr int STAGES = SCALED && D == 64 ? 2 : 4;
+	static constexpr int FACTS = STAGES + SLOTS;
+	static_assert(FACTS <= MAX_FACTS && (!SCALED || (FACTS * TK <= 640 && STAGES * TK <= 256)) && STAGES <= MAX_STAGES && SLOTS <= MAX_SLOTS && TILE_FACTS >= SLOTS + 2, "rings");
+	// tensor memory: parts of Q, score tiles (and what P's parts need beyond their columns), O
+	static constexpr int SLOT = PARTS == 3 ? TK + TK / 2 : TK, COL_Q = 0, COL_S = PARTS * D / 2, COL_O = COL_S + SLOTS * SLOT;
 	static_assert(COL_O + D <= 512, "tensor memory");
 	static constexpr uint32_t PANEL = TK * 128;  // 64 dims of a tile: rows of 128 bytes
 	static constexpr uint32_t BYTES = TK * D * 2;
@@ -398,7 +402,7 @@ __device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared
 						ptx::tma_load_3d(dst + b * T::PANEL, map, bar, 0, (int)row, b);
 				}
 				if constexpr (T::SCALED)
-					bulk_g2s(ptx::smem_u32(VALUES ? sh->v_got[slot] : sh->k_scale[n % T::FACTS]) + 4 * lane * run, (VALUES ? kv.v_scale : kv.k_scale) + row,
+					bulk_g2s(ptx::smem_u32(VALUES ? sh->v_got + slot * T::TK : sh->k_scale + n % T::FACTS * T::TK) + 4 * lane * run, (VALUES ? kv.v_scale : kv.k_scale) + row,
 						  run * 4, bar);
 			}
 		}
@@ -448,11 +452,12 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 					}
 				}
 				if constexpr (VALUES) {	 // factors relative to the tile's largest, which multiplies the tile's sums
-					float f[2];
+					constexpr int EACH = T::TK / MAKE_THREADS;
+					float f[EACH];
 					float top = 0.0f;
 #pragma unroll
-					for (int j = 0; j < 2; j++) {
-						f[j] = there(t + MAKE_THREADS * j) ? sh->v_got[slot][t + MAKE_THREADS * j] : 0.0f;
+					for (int j = 0; j < EACH; j++) {
+						f[j] = there(t + MAKE_THREADS * j) ? sh->v_got[slot * T::TK + t + MAKE_THREADS * j] : 0.0f;
 						// (an infinite factor is as little a number as NaN, and NaN does not reach the largest)
 						f[j] = fabsf(f[j]) <= FLT_MAX ? f[j] : __int_as_float(0x7fc00000);
 						top = fmaxf(top, fabsf(f[j]));
@@ -467,8 +472,9 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 					top = top > 0.0f ? top : 1.0f;
 					if (t == 0)
 						sh->v_top[slot] = top;
-					sh->v_scale[slot][t] = f[0] / top;
-					sh->v_scale[slot][t + MAKE_THREADS] = f[1] / top;
+#pragma unroll
+					for (int j = 0; j < EACH; j++)
+						sh->v_scale[slot * T::TK + t + MAKE_THREADS * j] = f[j] / top;
 				}
 			} else if (masked) {
 				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
@@ -534,9 +540,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			ptx::mbar_init(ptx::smem_u32(&sh->v_free[i]), 1);
 		}
 		for (int i = 0; i < 2; i++) {
+			ptx::mbar_init(ptx::smem_u32(&sh->ml_full[i]), SOFT_THREADS);
+		}
+		for (int i = 0; i < T::SLOTS; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->s_full[i]), 1);
 			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS / 2);
-			ptx::mbar_init(ptx::smem_u32(&sh->ml_full[i]), SOFT_THREADS);
 		}
 		for (int i = 0; i < T::FACTS; i++)
 			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), T::SCALED ? MAKE_THREADS : 1);
@@ -648,10 +656,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				if ((int)(tiles & 1) != wg)
 					continue;
 				const int key0 = p.unit0 * ATTN_UNIT + i * TK;
-				const uint32_t ph = (tiles >> 1) & 1u, slot = tiles % T::STAGES, S = lanes + T::COL_S + wg * T::SLOT;
+				const uint32_t slot = tiles % T::STAGES, score = tiles % T::SLOTS, S = lanes + T::COL_S + score * T::SLOT;
 				const uint32_t fslot = tiles % T::FACTS;
 				wait(sh->f_full[fslot], tiles / T::FACTS & 1u);
-				wait(sh->s_full[wg], ph);
+				wait(sh->s_full[score], tiles / T::SLOTS & 1u);
 				ptx::tc_fence_after();
 				const uint32_t bad = sh->bad[fslot];
 				const bool masked = key0 + TK > p.all_see || bad != 0;
@@ -666,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					if (T::SCALED && !scaled) {
 #pragma unroll
 						for (int k = 0; k < 16; k += 2) {
-							const float4 f = *reinterpret_cast<const float4 *>(&sh->k_scale[fslot][32 * c + 2 * k]);
+							const float4 f = *reinterpret_cast<const float4 *>(&sh->k_scale[fslot * TK + 32 * c + 2 * k]);
 							x[k] = mul2(x[k], make_float2(f.x, f.y));
 							x[k + 1] = mul2(x[k + 1], make_float2(f.z, f.w));
 						}
@@ -712,11 +720,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				// made the slot is another tile's
 				if (T::SCALED || masked)
 					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
-				sh->t_top[tiles & 3u][r] = top;
+				sh->t_top[tiles % TILE_FACTS][r] = top;
 				if (r == 0) {
-					sh->t_odd[tiles & 3u] = masked ? sh->odd[slot][0] | sh->odd[slot][1] : 0u;
-					sh->t_bad[tiles & 3u] = bad;
-					sh->t_unit[tiles & 3u] = T::SCALED ? sh->v_top[slot] : 1.0f;
+					sh->t_odd[tiles % TILE_FACTS] = masked ? sh->odd[slot][0] | sh->odd[slot][1] : 0u;
+					sh->t_bad[tiles % TILE_FACTS] = bad;
+					sh->t_unit[tiles % TILE_FACTS] = T::SCALED ? sh->v_top[slot] : 1.0f;
 				}
 				float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
@@ -735,7 +743,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 							sum = add2(sum, pk);
 							if constexpr (T::SCALED) {
 								if ((k & 1) == 0)
-									vs = *reinterpret_cast<const float4 *>(&sh->v_scale[slot][32 * c + 16 * h + 2 * k]);
+									vs = *reinterpret_cast<const float4 *>(&sh->v_scale[slot * TK + 32 * c + 16 * h + 2 * k]);
 								const float2 z = mul2(pk, k & 1 ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
 								// (where a row does not see every key, a factor that is no number is nothing to it)
 								pk = masked ? make_float2(pk.x == 0.0f ? 0.0f : z.x, pk.y == 0.0f ? 0.0f : z.y) : z;
@@ -754,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				}
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
-				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[wg]));
+				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[score]));
 				l = fmaf(l, alpha, sum.x + sum.y);
 			}
 			sh->ml[n & 1u][wg][r] = make_float2(m, l);
@@ -779,7 +787,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			for (int i = 0; i < HALF; i++)
 				acc[i] = make_float2(0.0f, 0.0f);
 			for (int i = 0; i < p.n_tiles; i++, tiles++) {
-				const uint32_t at = tiles & 3u;
+				const uint32_t at = tiles % TILE_FACTS;
 				wait(sh->o_full, tiles & 1u);
 				ptx::tc_fence_after();
 				// relative to the largest maximum so far (the tiles' are those of the two warpgroups)
@@ -886,12 +894,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				auto products = [&](uint32_t n) {  // P V of tile n
 					const uint32_t slot = n % T::STAGES;
 					wait(sh->v_full[slot], n / T::STAGES & 1u);
-					wait(sh->p_full[n & 1u], (n >> 1) & 1u);
+					wait(sh->p_full[n % T::SLOTS], n / T::SLOTS & 1u);
 					const bool ok = n == 0 || wait(sh->o_free, (n - 1) & 1u);
 					ptx::tc_fence_after();
 					if (ok && !*wait.abort) {
 						// MN-major: 8 keys 1024 bytes apart, 64 dims a panel apart
-						const uint32_t b = ptx::umma_desc_lo(v_ring + slot * T::BYTES) | (T::PANEL >> 4) << 16, P = tmem + T::COL_S + (n & 1u) * T::SLOT;
+						const uint32_t b = ptx::umma_desc_lo(v_ring + slot * T::BYTES) | (T::PANEL >> 4) << 16, P = tmem + T::COL_S + n % T::SLOTS * T::SLOT;
 #pragma unroll
 						for (int part = T::PARTS - 1; part >= 0; part--)
 #pragma unroll
@@ -911,25 +919,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					if (p.n_tiles == 0)
 						continue;
 					wait(sh->q_full, pieces & 1u);
-					for (int i = 0; i < p.n_tiles; i++, tiles++) {
-						const uint32_t slot = tiles % T::STAGES;
-						wait(T::SCALED ? sh->k_full[slot] : sh->k_raw[slot], tiles / T::STAGES & 1u);
-						ptx::tc_fence_after();
-						if (!*wait.abort) {
-							const uint32_t b = ptx::umma_desc_lo(k_ring + slot * T::BYTES);
+					// scores as far ahead of the products as there are tiles for them
+					for (int i = 0; i < p.n_tiles + T::SLOTS - 1; i++) {
+						if (i < p.n_tiles) {
+							const uint32_t n = tiles + i, slot = n % T::STAGES;
+							wait(T::SCALED ? sh->k_full[slot] : sh->k_raw[slot], n / T::STAGES & 1u);
+							ptx::tc_fence_after();
+							if (!*wait.abort) {
+								const uint32_t b = ptx::umma_desc_lo(k_ring + slot * T::BYTES);
 #pragma unroll
-							for (int part = T::PARTS - 1; part >= 0; part--)
+								for (int part = T::PARTS - 1; part >= 0; part--)
 #pragma unroll
-								for (int k = 0; k < D / 16; k++)
-									ptx::mma_f16_ts(tmem + T::COL_S + (tiles & 1u) * T::SLOT, tmem + T::COL_Q + part * HALF + 8 * k,
-											b + (k >> 2) * (T::PANEL >> 4) + 2 * (k & 3), idesc_qk, part < T::PARTS - 1 || k > 0);
+									for (int k = 0; k < D / 16; k++)
+										ptx::mma_f16_ts(tmem + T::COL_S + n % T::SLOTS * T::SLOT, tmem + T::COL_Q + part * HALF + 8 * k,
+												b + (k >> 2) * (T::PANEL >> 4) + 2 * (k & 3), idesc_qk, part < T::PARTS - 1 || k > 0);
+							}
+							ptx::mma_commit(ptx::smem_u32(&sh->k_free[slot]));
+							ptx::mma_commit(ptx::smem_u32(&sh->s_full[n % T::SLOTS]));
 						}
-						ptx::mma_commit(ptx::smem_u32(&sh->k_free[slot]));
-						ptx::mma_commit(ptx::smem_u32(&sh->s_full[tiles & 1u]));
-						if (i > 0)
-							products(tiles - 1);
+						if (i >= T::SLOTS - 1)
+							products(tiles + i - (T::SLOTS - 1));
 					}
-					products(tiles - 1);
+					tiles += p.n_tiles;
 					pieces++;
 				}
 				ptx::mma_commit(ptx::smem_u32(&sh->fin));
