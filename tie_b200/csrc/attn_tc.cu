@@ -55,7 +55,7 @@ struct Shared {
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
 	uint64_t k_raw[MAX_STAGES], k_full[MAX_STAGES], k_free[MAX_STAGES];  // keys have come in; are the operand; have been used
 	uint64_t v_raw[MAX_STAGES], v_full[MAX_STAGES], v_free[MAX_STAGES];
-	uint64_t s_full[MAX_SLOTS], p_full[MAX_SLOTS], o_full, o_free, q_full, ml_full[2], fin;
+	uint64_t s_full[MAX_SLOTS], p_full[MAX_SLOTS], o_full, o_free, q_come, q_full, ml_full[2], fin;
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
 	// made: tile n + FACTS is requested after the scores of tile n + SLOTS at the least, these after the products of n.
 	uint64_t f_full[MAX_FACTS];
@@ -108,8 +108,9 @@ __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &wo
 	const long long item = attn_div(in_seq, w.share == EVEN ? units : parts);
 	const int rest = (int)(in_seq - item * (w.share == EVEN ? units : parts));
 	if (w.share == WHOLE) {
-		p.row0 = (tiles - 1 - (int)attn_div(item, kv.n_head_kv)) * ROWS;
-		p.head = (int)(item % kv.n_head_kv);
+		const int back = (int)attn_div(item, kv.n_head_kv);
+		p.row0 = (tiles - 1 - back) * ROWS;
+		p.head = (int)(item - (long long)back * kv.n_head_kv);
 	} else {
 		p.head = (int)attn_div(item, tiles);
 		p.row0 = (int)(item - (long long)p.head * tiles) * ROWS;
@@ -127,8 +128,8 @@ __device__ __forceinline__ bool next_piece(Walk &w, Piece &p, const AttnWork &wo
 			p.n_parts = attn_cta_of(i + units - 1, w.total, w.n_cta) - (int)blockIdx.x + 1;
 		w.u += p.unit1 - p.unit0;
 	} else {
-		p.unit0 = (int)((long long)used * rest / parts);
-		p.unit1 = (int)((long long)used * (rest + 1) / parts);
+		p.unit0 = (int)attn_div((long long)used * rest, parts);
+		p.unit1 = (int)attn_div((long long)used * (rest + 1), parts);
 		p.whole = parts == 1;
 		if (rest == 0)
 			p.n_parts = parts;
@@ -144,33 +145,54 @@ __device__ __forceinline__ Walk start_walk(AttnWork &work, const KvView &kv, con
 {
 	Walk w = {};
 	w.n_cta = n_cta;
-	attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS); });
-	w.total = work.start[st.n_seq];
-	w.share = WHOLE;
-	const long long items = w.total;
-	if (items == 0 || items >= 3ll * n_cta)
+	// Sums over the sequences, made by each warp for itself: a scan by all of them with its barriers for every size of part that
+	// is tried took 13000 cycles with 8 sequences.
+	auto total = [&](auto of) {
+		if (st.n_seq == 1)
+			return (long long)of(kv_sequence(st, kv.page_shift, 0));
+		long long sum = 0;
+		for (int s = threadIdx.x & 31; s < st.n_seq; s += 32)
+			sum += of(kv_sequence(st, kv.page_shift, s));
+#pragma unroll
+		for (int o = 16; o; o >>= 1)
+			sum += __shfl_xor_sync(0xffffffffu, sum, o);
+		return sum;
+	};
+	auto items_of = [&](const SeqView &q) { return attn_items(kv, a, q, ROWS); };
+	auto units_of = [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); };
+	const long long items = total(items_of);
+	if (items == 0 || items >= 3ll * n_cta) {
+		attn_share_work<N>(work, kv, st, items_of);
+		w.share = WHOLE;
+		w.total = items;
 		return w;
-	__syncthreads();
-	attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
-	const long long units = work.start[st.n_seq];
-	const int even = (int)min(attn_div(units + n_cta - 1, n_cta), 1ll << 30);
+	}
+	const long long units = total(units_of);
 	if (items <= n_cta) {
-		// the smallest part size with which there are no more parts than CTAs, tried in steps of an eighth; not kept where it
-		// costs more than a second piece in each CTA would
-		w.share = PARTS;
-		for (w.part_units = even; w.part_units <= even + PIECE_UNITS || st.n_seq == 1; w.part_units += max(1, w.part_units >> 3)) {
-			__syncthreads();
-			attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * ((attn_units(q) + w.part_units - 1) / w.part_units); });
-			w.total = work.start[st.n_seq];
-			if (w.total <= n_cta) {
-				w.u = cta;
-				w.u_end = cta < w.total ? cta + 1 : cta;
-				return w;
+		// The smallest part size with which there are no more parts than CTAs; with several sequences tried in steps of an
+		// eighth, and not kept where it costs more than a second piece in each CTA would.
+		const int even = (int)min(attn_div(units + n_cta - 1, n_cta), 1ll << 30);
+		auto parts_of = [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * ((attn_units(q) + w.part_units - 1) / w.part_units); };
+		if (st.n_seq == 1) {
+			const int each = (int)((unsigned)n_cta / (unsigned)items), of_item = attn_units(kv_sequence(st, kv.page_shift, 0));
+			w.part_units = (of_item + each - 1) / each;
+			w.total = total(parts_of);
+		} else {
+			for (w.part_units = even; w.part_units <= even + PIECE_UNITS; w.part_units += max(1, w.part_units >> 3)) {
+				w.total = total(parts_of);
+				if (w.total <= n_cta)
+					break;
 			}
 		}
-		__syncthreads();
-		attn_share_work<N>(work, kv, st, [&](const SeqView &q) { return attn_items(kv, a, q, ROWS) * attn_units(q); });
+		if (w.total <= n_cta) {
+			attn_share_work<N>(work, kv, st, parts_of);
+			w.share = PARTS;
+			w.u = cta;
+			w.u_end = cta < w.total ? cta + 1 : cta;
+			return w;
+		}
 	}
+	attn_share_work<N>(work, kv, st, units_of);
 	w.share = EVEN;
 	w.total = units;
 	w.n_cta = (int)min((long long)n_cta, units);
@@ -188,9 +210,9 @@ struct Tile {
 	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  More than two let a warpgroup work on one
 	// tile while the products of its last and the scores of its next are made (with two tiles of 128 keys it waited for half of
 	// the time).
-	static constexpr int TK = PARTS == 3 || D == 128 ? 64 : 128;
-	static constexpr int SLOTS = PARTS == 3 ? (D == 128 ? 2 : 3) : (D == 128 ? 4 : 3);
-	static constexpr int STAGES = SCALED && D == 64 ? 2 : 4;
+	static constexpr int TK = PARTS == 3 ? 64 : 128;
+	static constexpr int SLOTS = D == 128 ? 2 : 3;
+	static constexpr int STAGES = TK * D == 128 * 128 || (SCALED && D == 64) ? 2 : 4;
 	static constexpr int FACTS = STAGES + SLOTS;
 	static_assert(FACTS <= MAX_FACTS && (!SCALED || (FACTS * TK <= 640 && STAGES * TK <= 256)) && STAGES <= MAX_STAGES && SLOTS <= MAX_SLOTS && TILE_FACTS >= SLOTS + 2, "rings");
 	// tensor memory: parts of Q, score tiles (and what P's parts need beyond their columns), O
@@ -201,7 +223,8 @@ struct Tile {
 	static constexpr int ROW = SCALED ? D : 2 * D;	 // bytes of a head row of the cache
 	static constexpr int BOX_BYTES = ROW < 128 ? ROW : 128, BOXES = ROW / BOX_BYTES;  // of a row, per TMA box
 	static constexpr uint32_t RAW = SCALED && D == 64 ? TK * ROW : 0;  // rows of 64 bytes come in beside the operand
-	static constexpr size_t SMEM = 2 * (size_t)STAGES * (BYTES + RAW) + (size_t)ROWS * D * 4 + OUT_BYTES + 1024;
+	static constexpr int Q_ROW = D * 4 + 16;  // bytes from row to row of the queries' tile in shared memory
+	static constexpr size_t SMEM = 2 * (size_t)STAGES * (BYTES + RAW) + (size_t)ROWS * Q_ROW + OUT_BYTES + 1024;
 	// where a 16-byte chunk of row r's 16-bit values lies in the operand tile
 	__device__ static __forceinline__ uint32_t place(int r, int ch) { return (ch >> 3) * PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
 };
@@ -407,6 +430,9 @@ __device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared
 			}
 		}
 	}
+	// (nothing that was requested is still on its way when the block ends, whoever has given up)
+	for (uint32_t i = n < T::STAGES ? 0 : n - T::STAGES; i < n; i++)
+		wait(raw_bar[i % T::STAGES], i / T::STAGES & 1u, true);
 }
 
 // Makes operands of what has come in: two warps for keys (Q8 only), two for values.
@@ -467,7 +493,7 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 						top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 					if (lane == 0)
 						sh->make_max[slot][t >> 5] = top;
-					bar_sync<3, MAKE_THREADS>();
+					bar_sync<2, MAKE_THREADS>();
 					top = fmaxf(sh->make_max[slot][0], sh->make_max[slot][1]);
 					top = top > 0.0f ? top : 1.0f;
 					if (t == 0)
@@ -520,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 						     const __grid_constant__ CUtensorMap v_map)
 {
 	using T = Tile<KIND, D>;
-	constexpr int HALF = D / 2, D4 = D / 4, PER = 32 / D4;  // PER: rows a warp moves at once
+	constexpr int HALF = D / 2, D4 = D / 4, Q_ROW = T::Q_ROW;
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ Shared shared;
 	__shared__ AttnWork work;
@@ -528,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
 	constexpr int TK = T::TK;
 	const uint32_t k_ring = smem, v_ring = k_ring + T::STAGES * T::BYTES, k_raw = v_ring + T::STAGES * T::BYTES, v_raw = k_raw + T::STAGES * T::RAW;
-	const uint32_t hand = v_raw + T::STAGES * T::RAW, out_stage = hand + ROWS * D * 4;
+	const uint32_t hand = v_raw + T::STAGES * T::RAW, out_stage = hand + ROWS * Q_ROW;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	if (threadIdx.x == 0) {
 		for (int i = 0; i < T::STAGES; i++) {
@@ -554,6 +580,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		}
 		ptx::mbar_init(ptx::smem_u32(&sh->o_full), 1);
 		ptx::mbar_init(ptx::smem_u32(&sh->o_free), FOLD_THREADS);
+		ptx::mbar_init(ptx::smem_u32(&sh->q_come), ROWS);
 		ptx::mbar_init(ptx::smem_u32(&sh->q_full), SOFT_THREADS);
 		ptx::mbar_init(ptx::smem_u32(&sh->fin), 1);
 		sh->abort = 0;
@@ -576,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		ptx::setmaxnreg_inc<SOFT_REGS>();
 		const int wg = threadIdx.x >> 7, r = threadIdx.x & 127;
 		const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
-		uint32_t tiles = 0;
+		uint32_t tiles = 0, loads = 0;
 		Piece p;
 		for (uint32_t n = 0;; n++) {
 			p = take_piece(sh, wait, n);
@@ -586,37 +613,29 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const int n_rows = p.seq.n_tok * a.group, row = p.row0 + r;
 			const bool there = row < n_rows;
 			const int tok = there ? row / a.group : p.seq.n_tok - 1;
-			// This warp's rows of the tile (PER at once, D / 4 lanes a row): f(row of the tile, float offset in q and in out).
-			// The division by the group is done once: one per row made the loop over 16 rows take 6600 cycles.
-			auto my_rows = [&](auto f) {
-				int line = warp * (ROWS / 8) + lane / D4, t = (p.row0 + line) / a.group, g = p.row0 + line - t * a.group;
-#pragma unroll 4
-				for (int i = 0; i < ROWS / 8 / PER; i++, line += PER) {
-					f(line, ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + g) * D + lane % D4 * 4);
-#pragma unroll
-					for (int k = 0; k < PER; k++)
-						if (++g == a.group)
-							g = 0, t++;
-				}
-			};
-			// 4 dims of a row of the tile, in shared memory: no conflicts, neither along a row nor across the rows
-			auto spot = [&](int d4, int line) { return hand + ((uint32_t)d4 * ROWS + (line ^ (d4 & 7))) * 16; };
+			// 4 dims of a row of the tile, in shared memory: rows a bank group apart, no conflicts
+			auto spot = [&](int d4, int line) { return hand + (uint32_t)line * Q_ROW + d4 * 16; };
 			float row_scale = 0.0f;
 			bar_sync<1, SOFT_THREADS>();  // nobody reads rows or makes scores of the piece before any more
 			if (p.n_tiles > 0) {
-				// The rows as they lie, through shared memory (a thread's own row from global memory: 32 lines a load), and this
-				// thread's half of its row, in parts, into tensor memory.
-				my_rows([&](int line, long long at) {
-					const bool in = p.row0 + line < n_rows;
-					cp_async16_or_zero(spot(lane % D4, line), a.q + (in ? at : 0), in);
-				});
-				ptx::cp_async_commit();
-				ptx::cp_async_wait<0>();
-				bar_sync<1, SOFT_THREADS>();
+				// The rows as they lie, through shared memory (a thread's own row from global memory: 32 lines a load), a copy each (by
+				// cp.async, 16 a thread, the addresses alone took 5000 cycles), and this thread's half of its row, in parts, into
+				// tensor memory.
+				if (lane < ROWS / 8) {
+					const int line = warp * (ROWS / 8) + lane, q_row = p.row0 + line, t = q_row / a.group;
+					const uint32_t bar = ptx::smem_u32(&sh->q_come);
+					if (q_row < n_rows) {
+						ptx::mbar_arrive_expect_tx(bar, D * 4);
+						bulk_g2s(spot(0, line), a.q + ((long long)(p.seq.tok0 + t) * a.n_head + p.head * a.group + (q_row - t * a.group)) * D, D * 4, bar);
+					} else {
+						ptx::mbar_arrive(bar);
+					}
+				}
+				wait(sh->q_come, loads++ & 1u, true);
 				float top = 0.0f;
 #pragma unroll 4
 				for (int i = 0; i < HALF / 4; i++) {
-					const uint4 x = lds128(spot(wg * (HALF / 4) + i, r));
+					const uint4 x = there ? lds128(spot(wg * (HALF / 4) + i, r)) : make_uint4(0, 0, 0, 0);
 					top = fmaxf(fmaxf(fmaxf(top, fabsf(__uint_as_float(x.x))), fmaxf(fabsf(__uint_as_float(x.y)), fabsf(__uint_as_float(x.z)))),
 						    fabsf(__uint_as_float(x.w)));
 				}
@@ -632,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					uint32_t out[T::PARTS][8];
 #pragma unroll
 					for (int i = 0; i < 4; i++) {
-						const uint4 x = lds128(spot(wg * (HALF / 4) + 4 * c + i, r));
+						const uint4 x = there ? lds128(spot(wg * (HALF / 4) + 4 * c + i, r)) : make_uint4(0, 0, 0, 0);
 						uint32_t part[2][T::PARTS];
 						split2<KIND>(make_float2(__uint_as_float(x.x) * down, __uint_as_float(x.y) * down), part[0]);
 						split2<KIND>(make_float2(__uint_as_float(x.z) * down, __uint_as_float(x.w) * down), part[1]);
@@ -850,7 +869,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					reinterpret_cast<float4 *>(part)[j * ROWS + r] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
 				continue;
 			}
-			// whole rows go out by 16 dims through shared memory: 4 lanes then store 64 bytes of a row
+			// whole rows go out by 16 dims through shared memory, each warp its 32: 4 lanes then store 64 bytes of a row
 			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 			long long at[4];
 #pragma unroll
@@ -861,13 +880,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const float2 i2 = make_float2(inv, inv);
 #pragma unroll
 			for (int c = 0; c < D / 16; c++) {
-				bar_sync<2, FOLD_THREADS>();
+				__syncwarp();
 #pragma unroll
 				for (int j = 0; j < 4; j++) {
 					const float2 y0 = mul2(acc[8 * c + 2 * j], i2), y1 = mul2(acc[8 * c + 2 * j + 1], i2);
 					sts128(out_stage + (j * ROWS + (r ^ j)) * 16, make_uint4(__float_as_uint(y0.x), __float_as_uint(y0.y), __float_as_uint(y1.x), __float_as_uint(y1.y)));
 				}
-				bar_sync<2, FOLD_THREADS>();
+				__syncwarp();
 #pragma unroll
 				for (int i = 0; i < 4; i++) {
 					const int line = (warp & 3) * 32 + i * 8 + lane / 4, j = lane % 4;
@@ -946,7 +965,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::mma_commit(ptx::smem_u32(&sh->fin));
 			}
 			__syncwarp();
-			wait(sh->fin, 0);
+			wait(sh->fin, 0, true);
 		} else if (warp >= W_ASK) {
 			if (warp == W_ASK)
 				ask<KIND, D, false>(kv, st, sh, &k_map, k_ring, k_raw, wait, lane);
