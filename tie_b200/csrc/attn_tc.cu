@@ -49,7 +49,7 @@ struct Piece {
 	int key_end;	// first key that nobody sees
 	int all_see;	// keys in front of this one are seen by every row
 };
-constexpr int PIECES = 4, MAX_STAGES = 4, MAX_SLOTS = 4, MAX_FACTS = 8, TILE_FACTS = 8;
+constexpr int PIECES = 4, MAX_STAGES = 4, MAX_SLOTS = 3, MAX_FACTS = 7, TILE_FACTS = 5;
 struct Shared {
 	uint64_t piece_full[PIECES], piece_free[PIECES];
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
@@ -65,6 +65,7 @@ struct Shared {
 	float v_top[MAX_STAGES], make_max[MAX_STAGES][2];
 	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
 	float q_max[2][ROWS];
+	float half_top[2][2][ROWS];	 // per tile in turn and warpgroup: the largest score of a row
 	// what the products of a tile have to be added up with: maximum of a row, factor; whether values are no numbers, bad pages
 	float t_top[TILE_FACTS][ROWS], t_unit[TILE_FACTS];
 	uint32_t t_odd[TILE_FACTS], t_bad[TILE_FACTS];
@@ -307,7 +308,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
 	return r;
 }
-// The 16-bit parts of a pair, the largest first: fp16 hi and lo, or three of bf16.
+__device__ __forceinline__ float2 sub2(float2 a, float2 b)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tsub.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+// The 16-bit parts of a pair, the largest first: fp16 hi and lo, rounded (22 bits of 24), or three of bf16, cut off (8 bits
+// each, and so all).
 template <int KIND, int PARTS>
 __device__ __forceinline__ void split2(float2 x, uint32_t (&part)[PARTS])
 {
@@ -315,17 +325,16 @@ __device__ __forceinline__ void split2(float2 x, uint32_t (&part)[PARTS])
 	for (int p = 0; p < PARTS; p++) {
 		float2 f;
 		if constexpr (KIND == TIE_CUDA_KV_BF16) {
-			const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
-			part[p] = *reinterpret_cast<const uint32_t *>(&h);
-			f = make_float2(-__uint_as_float(part[p] << 16), -__uint_as_float(part[p] & 0xffff0000u));
+			const uint32_t a = __float_as_uint(x.x), b = __float_as_uint(x.y);
+			part[p] = __byte_perm(a, b, 0x7632);
+			f = make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u));
 		} else {
 			const __half2 h = __floats2half2_rn(x.x, x.y);
 			part[p] = *reinterpret_cast<const uint32_t *>(&h);
 			f = __half22float2(h);
-			f = make_float2(-f.x, -f.y);
 		}
 		if (p < PARTS - 1)
-			x = add2(x, f);
+			x = sub2(x, f);
 	}
 }
 
@@ -570,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 		}
 		for (int i = 0; i < T::SLOTS; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->s_full[i]), 1);
-			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS / 2);
+			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS);
 		}
 		for (int i = 0; i < T::FACTS; i++)
 			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), T::SCALED ? MAKE_THREADS : 1);
@@ -672,8 +681,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			const RowView view = row_view(st, p, tok, r == 0);
 			float m = -INFINITY, l = 0.0f;
 			for (int i = 0; i < p.n_tiles; i++, tiles++) {
-				if ((int)(tiles & 1) != wg)
-					continue;
 				const int key0 = p.unit0 * ATTN_UNIT + i * TK;
 				const uint32_t slot = tiles % T::STAGES, score = tiles % T::SLOTS, S = lanes + T::COL_S + score * T::SLOT;
 				const uint32_t fslot = tiles % T::FACTS;
@@ -708,14 +715,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					}
 				};
 				float top = -INFINITY;
+				float2 x[16];  // where a warpgroup has no more than these of a tile, they are read once
+				constexpr int CHUNKS = TK / 64;
 #pragma unroll 1
-				for (int c = 0; c < TK / 32; c++) {
-					float2 x[16];
+				for (int c = wg * CHUNKS; c < wg * CHUNKS + CHUNKS; c++) {
 					scores(c, x, false);
 #pragma unroll
 					for (int k = 0; k < 16; k++)
 						top = fmaxf(top, fmaxf(x[k].x, x[k].y));
-					if constexpr (T::SCALED) {
+					if constexpr (T::SCALED && CHUNKS > 1) {
 						// back with the factors in them: each read of those by all lanes costs the shared memory 512 cycles a tile
 #pragma unroll
 						for (int h = 0; h < 2; h++) {
@@ -729,9 +737,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 						}
 					}
 				}
-				if constexpr (T::SCALED)
+				if constexpr (T::SCALED && CHUNKS > 1)
 					ptx::tmem_st_wait();
-				top = fmaxf(m, top * row_scale);
+				sh->half_top[i & 1][wg][r] = top;
+				bar_sync<1, SOFT_THREADS>();
+				top = fmaxf(m, fmaxf(top, sh->half_top[i & 1][wg ^ 1][r]) * row_scale);
 				const float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
 				const float alpha = m == -INFINITY ? 0.0f : exp2_ftz(m - top);
 				m = top;
@@ -739,17 +749,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				// made the slot is another tile's
 				if (T::SCALED || masked)
 					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
-				sh->t_top[tiles % TILE_FACTS][r] = top;
-				if (r == 0) {
+				if (wg == 0)
+					sh->t_top[tiles % TILE_FACTS][r] = top;
+				if (threadIdx.x == 0) {
 					sh->t_odd[tiles % TILE_FACTS] = masked ? sh->odd[slot][0] | sh->odd[slot][1] : 0u;
 					sh->t_bad[tiles % TILE_FACTS] = bad;
 					sh->t_unit[tiles % TILE_FACTS] = T::SCALED ? sh->v_top[slot] : 1.0f;
 				}
 				float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-				for (int c = 0; c < TK / 32; c++) {
-					float2 x[16];
-					scores(c, x, true);
+				for (int c = wg * CHUNKS; c < wg * CHUNKS + CHUNKS; c++) {
+					if constexpr (CHUNKS > 1)
+						scores(c, x, true);
 					// the first two parts of 16 keys take the columns of their scores, 8 each; a third comes behind all of them
 #pragma unroll
 					for (int h = 0; h < 2; h++) {
