@@ -63,7 +63,7 @@ def test_caches_that_are_refused(lib, what, code):
 
 @pytest.mark.parametrize("what", [
     dict(n_seq=0), dict(n_seq=1025), dict(n_tokens=-1), dict(tok_start=None), dict(kv_len=None), dict(page_table=None),
-    dict(max_pages=0), dict(max_pages=1 << 27), dict(tok_start=FAKE + 2), dict(pos=FAKE + 1), dict(tree=FAKE + 4),
+    dict(max_pages=0), dict(max_pages=1 << 27), dict(n_tokens=1 << 30), dict(n_tokens=1 << 26), dict(tok_start=FAKE + 2), dict(pos=FAKE + 1), dict(tree=FAKE + 4),
 ])
 def test_steps_that_are_refused(lib, what):
     from tie_b200 import moe

@@ -537,6 +537,122 @@ def test_empty_steps_launch_nothing(be):
     assert be.launch_count == before
 
 
+# One of each way that work is shared out: few rows; parts of items; items in equal shares of keys; whole items.
+SHARES = [([1, 2], [700, 9001], None), ([90, 40], [300, 2000], None), ([700, 300], [64, 900], None), ([64, 3], [1000, 8], True), ([2200], [50], None)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("toks, lens, drafted", SHARES)
+def test_out_may_be_q(be, kind, toks, lens, drafted):
+    w = World(40, kind, toks, lens, 32, 4, 128, 32, pad=3, tree=trees(np.random.default_rng(3), toks) if drafted else None)
+    q, out, scale = w.attn(be)
+    both = q.clone()
+    w.attn(be, both, scale, out=both)
+    assert torch.equal(both[:w.n], out[:w.n]) and torch.equal(both[w.n:], q[w.n:])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_contexts_at_once(kind):
+    """Launches of two contexts overlap on their streams; each has the result that it has alone."""
+    from tie_b200 import moe
+    two = [moe.MoeBackend(hidden=256, n_expert=16, top_k=1, ffn_dim=256, max_tokens=64) for _ in range(2)]
+    try:
+        ws = [World(41 + i, kind, toks, lens, 32, 4, 128, 64) for i, (toks, lens) in enumerate([([1] * 5, [4000] * 5), ([150], [1000])])]
+        alone = [w.attn(b) for w, b in zip(ws, two)]
+        outs = [torch.zeros_like(a[1]) for a in alone]
+        torch.cuda.synchronize()
+        for _ in range(30):
+            for b, w, a, o in zip(two, ws, alone, outs):
+                b.attn_ptr(w.cache, w.step, a[0], o, 32, a[2], flags=moe.DEVICE | moe.NO_SYNC)
+        for b in two:
+            b.synchronize()
+        for a, o in zip(alone, outs):
+            assert torch.equal(a[1], o)
+    finally:
+        for b in two:
+            b.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_captured_prompt_step_follows_its_arrays(be, kind):
+    """One graph for steps of up to 600 rows: few rows and many, rows in front of the first sequence and behind the last, none at all."""
+    from tie_b200 import moe
+    w = World(43, kind, [300, 300], [400, 400], 16, 2, 64, 32)
+    q, _, scale = w.attn(be)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    try:
+        be.set_stream(side.cuda_stream)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            be.attn_ptr(w.cache, w.step, q, out, 16, scale, flags=moe.DEVICE | moe.NO_SYNC)
+        for first, toks, lens in ((0, [300, 300], [400, 400]), (0, [1, 1], [600, 2]), (5, [100, 0], [17, 300]), (0, [0, 0], [5, 5]), (600, [0, 0], [0, 0]), (0, [300, 300], [0, 0])):
+            with torch.cuda.stream(side):
+                w.tok_start.copy_(torch.tensor([first, first + toks[0], first + sum(toks)], dtype=torch.int32))
+                w.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+                out.fill_(7.25)
+                g.replay()
+                side.synchronize()
+            w.toks, w.lens = toks, lens
+            end = first + sum(toks)
+            assert (out[:first] == 7.25).all() and (out[end:] == 7.25).all()
+            if end > first:
+                w.check_attn(q[first:end], out[first:end], scale)
+    finally:
+        be.set_stream(None)
+    be.synchronize()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("toks, lens, drafted", SHARES[:2] + SHARES[3:4])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_no_number_is_its_own_affair(be, kind, toks, lens, drafted, bad):
+    w = World(44, kind, toks, lens, 16, 2, 64, 32, tree=trees(np.random.default_rng(3), toks) if drafted else None)
+    q, clean, scale = w.attn(be)
+    for t, h in ((0, 3), (w.n - 1, 15)):
+        q[t, h, 17] = bad
+    _, out, _ = w.attn(be, q, scale)
+    for t, h in ((0, 3), (w.n - 1, 15)):
+        assert not out[t, h].isfinite().any()
+        out[t, h] = clean[t, h]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_sequences_may_share_pages(be, kind):
+    w = World(45, kind, [1, 40, 2], [200, 160, 170], 8, 2, 128, 16)
+    w.table[1:, :10] = w.table[0, :10]  # a prefix of 160 slots
+    w.d_table = torch.tensor(w.table).cuda()
+    w.describe()
+    q, out, scale = w.attn(be)
+    w.check_attn(q, out, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads, kv_heads, toks, lens", [(256, 1, [3], [200]), (1024, 1, [1, 2], [77, 0]), (256, 256, [2, 17], [33, 0]), (1, 1, [150], [9])])
+def test_head_layouts_at_their_ends(be, kind, heads, kv_heads, toks, lens):
+    w = World(46, kind, toks, lens, heads, kv_heads, 64, 16)
+    q, out, scale = w.attn(be)
+    w.check_attn(q, out, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [0.0, -1.5])
+def test_scales_of_prompt_pieces(be, kind, scale):
+    w = World(47, kind, [70], [100], 8, 2, 64, 16)
+    q = torch.randn(70, 8, 64, device="cuda") * torch.logspace(-20, 1, 70, device="cuda")[:, None, None]
+    _, out, _ = w.attn(be, q, scale)
+    w.check_attn(q, out, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_page_may_be_a_whole_cache(be, kind):
+    w = World(48, kind, [1, 20], [1000, 3], 8, 2, 64, 65536, spare_pages=0)
+    q, out, scale = w.attn(be)
+    w.check_attn(q, out, scale)
+
+
 # ---- refusals and steps that are wrong ----
 
 

@@ -414,6 +414,8 @@ bool aligned16(const void *p)
 	return ((uintptr_t)p & 15) == 0;
 }
 
+constexpr long long MAX_STEP_ROWS = 0x7fff0000;  // head rows of a step: they are counted in 32 bits (more would be 500 GB of fp32)
+
 // What the host can see of a cache and a step.  *idle: a step without rows.
 int kv_views(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, unsigned flags, KvView &kv, StepView &st, bool &idle)
 {
@@ -433,7 +435,7 @@ int kv_views(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_
 	if (((long long)cache->n_pages * cache->n_head_kv) * cache->page_size > 0x7fffffff)
 		return TIE_CUDA_ENOTSUP;  // (rows are numbered in 32 bits where boxes of them are asked for)
 	if (step->n_seq < 1 || step->n_seq > KV_MAX_SEQ || step->n_tokens < 0 || !step->tok_start || !step->kv_len || !step->page_table ||
-	    step->max_pages < 1 || (long long)step->max_pages * cache->page_size > 1 << 30 ||
+	    step->max_pages < 1 || (long long)step->max_pages * cache->page_size > 1 << 30 || (long long)step->n_tokens * cache->n_head_kv > MAX_STEP_ROWS ||
 	    ((uintptr_t)step->tok_start | (uintptr_t)step->kv_len | (uintptr_t)step->page_table | (uintptr_t)step->pos) & 3 ||
 	    (uintptr_t)step->tree & 7 || !c)
 		return TIE_CUDA_EINVAL;
@@ -1685,9 +1687,9 @@ int tie_cuda_moe_block_inplace_ep(tie_cuda_ctx *c, int layer, float *hidden_dev,
 
 // ---- attention over a paged cache ----
 
-static int attn_heads(const tie_cuda_kv_cache *cache, int n_head)
+static int attn_heads(const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, int n_head)
 {
-	return n_head >= 1 && n_head <= 1024 && n_head % cache->n_head_kv == 0 ? TIE_CUDA_OK : TIE_CUDA_EINVAL;
+	return n_head >= 1 && n_head <= 1024 && n_head % cache->n_head_kv == 0 && (long long)step->n_tokens * n_head <= MAX_STEP_ROWS ? TIE_CUDA_OK : TIE_CUDA_EINVAL;
 }
 
 int tie_cuda_qk_norm_rope(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const tie_cuda_attn_qkv *in,
@@ -1699,7 +1701,7 @@ int tie_cuda_qk_norm_rope(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const
 	TRY(kv_views(c, cache, step, flags, kv, st, idle));
 	if (!in)
 		return TIE_CUDA_EINVAL;
-	TRY(attn_heads(cache, in->n_head));
+	TRY(attn_heads(cache, step, in->n_head));
 	if (idle)
 		return TIE_CUDA_OK;
 	const int64_t d = cache->head_dim;
@@ -1750,7 +1752,7 @@ int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cud
 	StepView st;
 	bool idle;
 	TRY(kv_views(c, cache, step, flags, kv, st, idle));
-	TRY(attn_heads(cache, n_head));
+	TRY(attn_heads(cache, step, n_head));
 	if (!(fabsf(scale) <= FLT_MAX))
 		return TIE_CUDA_EINVAL;
 	if (idle)
@@ -1789,7 +1791,7 @@ int tie_cuda_attn_block_inplace(tie_cuda_ctx *c, const tie_cuda_attn_weights *w,
 	if (!w || !w->wq || !w->wk || !w->wv || !w->wo || !aligned16(w->norm_w) || ((uintptr_t)w->q_norm_w | (uintptr_t)w->k_norm_w) & 3 ||
 	    !(w->rope_base >= 0.0f) || w->rope_base > FLT_MAX || !(fabsf(w->scale) <= FLT_MAX))
 		return TIE_CUDA_EINVAL;
-	TRY(attn_heads(cache, w->n_head));
+	TRY(attn_heads(cache, step, w->n_head));
 	const int T = step->n_tokens, H = c->cfg.hidden, d = cache->head_dim, qw = w->n_head * d, kw = cache->n_head_kv * d;
 	const DevTensor *wq, *wk, *wv, *wo;
 	TRY(dense_tensor(c, w->wq, H, qw, &wq));

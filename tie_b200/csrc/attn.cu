@@ -259,9 +259,11 @@ struct Warp {
 							q[nb][p][j][h] = (__byte_perm(n[0], n[1], s) & 0xffffu | __byte_perm(n[2], n[3], s) << 16) ^ 0x80808080u;
 						}
 					}
-				odd = odd || __shfl_xor_sync(0xffffffffu, (int)odd, 1);
-				odd = odd || __shfl_xor_sync(0xffffffffu, (int)odd, 2);
-				up = odd ? __int_as_float(0x7fc00000) : up;  // a row with an infinity or NaN has no scores
+				// (by all lanes, whatever their own: a || would leave the shuffle out where it is true, and the others waiting)
+				int any = odd;
+				any |= __shfl_xor_sync(0xffffffffu, any, 1);
+				any |= __shfl_xor_sync(0xffffffffu, any, 2);
+				up = any ? __int_as_float(0x7fc00000) : up;  // a row with an infinity or NaN has no scores
 			} else {
 				float2 v[KS][2];
 #pragma unroll

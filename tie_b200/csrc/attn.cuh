@@ -130,11 +130,6 @@ __device__ __forceinline__ float exp2_ftz(float x)
 	return r;
 }
 
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool there)
-{
-	const int n = there ? 16 : 0;
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exponent)
 {
 	return (w & exponent) == exponent || (w >> 16 & exponent) == exponent;

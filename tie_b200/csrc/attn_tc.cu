@@ -1,5 +1,5 @@
 // Attention over the paged cache for sequences with many query rows per key/value head (trees of drafted tokens, prompt
-// pieces): tiles of 128 rows x 128 keys on tcgen05.
+// pieces): tiles of 128 rows x 128 or 64 keys on tcgen05.
 //
 //   S = Q K^T, P = exp2(S - max), O = P V      rows (token, head of the group) on the 128 lanes of tensor memory
 //
@@ -9,16 +9,20 @@
 // tensor cores cut every sum off, which over a long cache would add up.
 //
 // One CTA per SM, 640 threads:
-//   * two warpgroups of softmax threads, a thread per row, take key tiles in turn, each with a running maximum and sum of its own,
-//     so that one's exponentials run under the other's MMAs; a third adds the tiles' products up, a thread per row, with the
-//     row in registers (where the softmax threads did that too, they waited for half of the time for products);
+//   * two warpgroups of softmax threads, a thread per row and half of a tile's keys; a third adds the tiles' products up, a
+//     thread per row, with the row in registers (where the softmax threads did that too, they waited for half of the time
+//     for products);
 //   * a warp requests keys, another values, by TMA straight into the swizzled operand layout, a box per page (as one
 //     cp.async per 16 bytes the address arithmetic alone took 5000 cycles a tile from two warps);
 //   * two warps each make operands of what came in where it is not one yet: Q8's bytes become fp16 in place, values behind
 //     the last key and values that are no numbers become zeros;
-//   * one thread finds the CTA's pieces of work, one issues the MMAs.  Q and P are operands in tensor memory (a step of
-//     shared memory then feeds only the keys or dims of the other operand: half of what the memory delivers); P's parts
-//     of 16 keys take the columns of these keys' scores.
+//   * one thread finds the CTA's pieces of work, one issues the MMAs (one for the scores and one for the products: 49.0 ->
+//     53.1 us below).  Q and P are operands in tensor memory (a step of shared memory then feeds only the keys or dims of the
+//     other operand: half of what the memory delivers); P's parts of 16 keys take the columns of these keys' scores.
+// What it takes (a piece of 512 tokens over 1500 keys, F16, 32 heads of 128 with 4 of keys: 49.0 us, 300 TFLOP/s, 600 of MMAs):
+// a tile of 128 keys takes about 3400 cycles where its MMAs take 2050 and its exponentials 1024: the scores of a tile wait
+// for the products of the last but one, and the issuing thread's four waits a tile cost 150 to 400 cycles each, complete or
+// not; 16000 cycles pass before the first scores and 5000 behind the last products.
 // Every wait is bounded, as in tensor.cu; after a time-out no wait waits any more and all roles run to their ends.
 #include <float.h>
 
@@ -208,9 +212,10 @@ template <int KIND, int D>
 struct Tile {
 	static constexpr bool SCALED = KIND == TIE_CUDA_KV_Q8;
 	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	 // of a value of Q and of P
-	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  More than two let a warpgroup work on one
-	// tile while the products of its last and the scores of its next are made (with two tiles of 128 keys it waited for half of
-	// the time).
+	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  Heads of 128, two parts: two tiles of
+	// 128 keys take 73.7 us for 8 trees of 64 tokens over 3500 keys (Q8) and 49.0 for a piece of 512 over 1500 (F16), four
+	// of 64 took 10 and 2 us more, since the waits are those of a tile.  Three parts, heads of 64: a third tile of 64
+	// keys brought 4096 tokens from 290 to 266 us.
 	static constexpr int TK = PARTS == 3 ? 64 : 128;
 	static constexpr int SLOTS = D == 128 ? 2 : 3;
 	static constexpr int STAGES = TK * D == 128 * 128 || (SCALED && D == 64) ? 2 : 4;
@@ -653,8 +658,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				top = fmaxf(sh->q_max[0][r], sh->q_max[1][r]);
 				// the row is brought to 1 .. 2 by a power of two (any fp32 row then keeps its 22 bits); it also takes the scale's sign
 				const int e = top > 0.0f ? min(max((int)(__float_as_uint(top) >> 23), 1), 253) : 127;
-				const float down = copysignf(__uint_as_float((uint32_t)(254 - e) << 23), a.scale_log2e);
+				float down = copysignf(__uint_as_float((uint32_t)(254 - e) << 23), a.scale_log2e);
 				row_scale = fabsf(a.scale_log2e) * __uint_as_float((uint32_t)e << 23);
+				if (row_scale == 0.0f) {  // the queries are zeros then, so that the -infinity of a key that is not seen stays one
+					down = 0.0f;
+					row_scale = 1.0f;
+				}
 #pragma unroll 1
 				for (int c = 0; c < HALF / 16; c++) {
 					uint32_t out[T::PARTS][8];
