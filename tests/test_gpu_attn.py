@@ -34,14 +34,15 @@ def be():
 class World:
     """A cache and a step, on the device for the library and in 64 bits on the host for the check."""
 
-    def __init__(self, seed, kind, toks, lens, heads=8, kv_heads=2, dim=128, page=16, pad=0, tree=None, pos=None, spare_pages=2):
+    def __init__(self, seed, kind, toks, lens, heads=8, kv_heads=2, dim=128, page=16, pad=0, tree=None, pos=None, spare_pages=2, far=False):
         from tie_b200 import moe
         self.kind, self.toks, self.lens, self.heads, self.kv_heads, self.dim, self.page = kind, toks, lens, heads, kv_heads, dim, page
         self.rng = np.random.default_rng(seed)
         self.n = sum(toks)
         self.rows = self.n + pad
         need = [-(-(a + t) // page) for a, t in zip(lens, toks)]
-        max_pages = max(1, max(need))
+        # (far: room for more slots than the kernels for few rows are chosen with)
+        max_pages = max(1, max(need)) + (32768 // page if far else 0)
         n_pages = sum(need) + spare_pages
         order = self.rng.permutation(n_pages)
         table, at = np.full((len(toks), max_pages), order[-1], np.int32), 0
@@ -287,35 +288,38 @@ def test_read_back(be, kind, out, toks, dim, kv_heads):
 # ---- attention ----
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim, heads, kv_heads, page", [(128, 32, 4, 16), (64, 24, 8, 64), (128, 4, 4, 128), (64, 10, 2, 32), (128, 32, 1, 16)])
 @pytest.mark.parametrize("toks, lens", [
     ([1], [0]), ([1], [1]), ([1], [127]), ([1], [640]), ([1, 1, 1], [5, 0, 300]), ([3, 0, 1], [12, 7, 129]), ([20], [0]), ([9, 30], [200, 15]),
 ])
-def test_attention_of_tokens_that_see_what_is_in_front(be, kind, dim, heads, kv_heads, page, toks, lens):
-    w = World(11, kind, toks, lens, heads, kv_heads, dim, page, pad=2)
+def test_attention_of_tokens_that_see_what_is_in_front(be, far, kind, dim, heads, kv_heads, page, toks, lens):
+    w = World(11, kind, toks, lens, heads, kv_heads, dim, page, pad=2, far=far)
     q, out, scale = w.attn(be)
     w.check_attn(q, out, scale)
     assert (out[w.n:] == 7.25).all()
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim, heads, kv_heads", [(128, 32, 4), (64, 6, 2)])
 @pytest.mark.parametrize("toks, lens, empty", [
     ([2], [40], False), ([13], [255], False), ([64], [100], False), ([64, 1, 33], [0, 500, 31], False), ([7, 64], [0, 0], True), ([40], [33], True),
 ])
-def test_attention_of_trees(be, kind, dim, heads, kv_heads, toks, lens, empty):
+def test_attention_of_trees(be, far, kind, dim, heads, kv_heads, toks, lens, empty):
     tree = trees(np.random.default_rng(8), toks, empty)
-    w = World(12, kind, toks, lens, heads, kv_heads, dim, 16, tree=tree, pad=1)
+    w = World(12, kind, toks, lens, heads, kv_heads, dim, 16, tree=tree, pad=1, far=far)
     q, out, scale = w.attn(be)
     w.check_attn(q, out, scale)
     assert (out[w.n:] == 7.25).all()
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("toks, lens", [([200], [0]), ([130], [77]), ([65, 300], [40, 0])])
-def test_attention_of_prompt_pieces(be, kind, toks, lens):
-    w = World(13, kind, toks, lens, 16, 2, 128, 32)
+def test_attention_of_prompt_pieces(be, far, kind, toks, lens):
+    w = World(13, kind, toks, lens, 16, 2, 128, 32, far=far)
     q, out, scale = w.attn(be)
     w.check_attn(q, out, scale)
 
@@ -344,10 +348,11 @@ def test_long_caches_and_many_rows(be, kind, dim, heads, kv_heads, toks, lens, d
         row += t
 
 
-def test_many_sequences_of_all_lengths(be):
+@pytest.mark.parametrize("far", [False, True])
+def test_many_sequences_of_all_lengths(be, far):
     rng = np.random.default_rng(1)
     toks = rng.integers(0, 3, 333).tolist()
-    w = World(14, "f16", toks, rng.integers(0, 200, 333).tolist(), 4, 2, 64, 16)
+    w = World(14, "f16", toks, rng.integers(0, 200, 333).tolist(), 4, 2, 64, 16, far=far)
     q, out, scale = w.attn(be)
     w.check_attn(q, out, scale)
 
@@ -364,14 +369,15 @@ def test_long_cache_is_split_and_joined_the_same_every_time(be, kind):
         assert torch.equal(first, out)
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("heads", [8, 32])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_what_a_token_does_not_see_is_nothing_to_it(be, kind, bad, heads):
+def test_what_a_token_does_not_see_is_nothing_to_it(be, far, kind, bad, heads):
     """Stale slots behind the last token and drafted tokens on other branches hold anything."""
     toks, lens = [12, 5], [37, 3]
     tree = trees(np.random.default_rng(2), toks)
-    w = World(16, kind, toks, lens, heads, 2, 128, 16, tree=tree)
+    w = World(16, kind, toks, lens, heads, 2, 128, 16, tree=tree, far=far)
     q, clean, scale = w.attn(be)
     used = np.zeros(w.k.shape[0] * 16, bool)
     for s in range(2):
@@ -399,10 +405,11 @@ def test_what_a_token_does_not_see_is_nothing_to_it(be, kind, bad, heads):
         row += toks[s]
 
 
-def test_q8_factors_that_are_no_numbers_stay_where_they_are_seen(be):
+@pytest.mark.parametrize("far", [False, True])
+def test_q8_factors_that_are_no_numbers_stay_where_they_are_seen(be, far):
     toks, lens = [6], [20]
     tree = [1, 3, 5, 9, 17, 33]
-    w = World(17, "q8", toks, lens, 8, 2, 64, 16, tree=tree)
+    w = World(17, "q8", toks, lens, 8, 2, 64, 16, tree=tree, far=far)
     q, clean, scale = w.attn(be)
     for j, bad in ((2, float("nan")), (4, float("inf"))):
         pg, pl = w.slots(0, 20 + j, 21 + j)
@@ -541,10 +548,11 @@ def test_empty_steps_launch_nothing(be):
 SHARES = [([1, 2], [700, 9001], None), ([90, 40], [300, 2000], None), ([700, 300], [64, 900], None), ([64, 3], [1000, 8], True), ([2200], [50], None)]
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("toks, lens, drafted", SHARES)
-def test_out_may_be_q(be, kind, toks, lens, drafted):
-    w = World(40, kind, toks, lens, 32, 4, 128, 32, pad=3, tree=trees(np.random.default_rng(3), toks) if drafted else None)
+def test_out_may_be_q(be, far, kind, toks, lens, drafted):
+    w = World(40, kind, toks, lens, 32, 4, 128, 32, pad=3, tree=trees(np.random.default_rng(3), toks) if drafted else None, far=far)
     q, out, scale = w.attn(be)
     both = q.clone()
     w.attn(be, both, scale, out=both)
@@ -573,11 +581,12 @@ def test_two_contexts_at_once(kind):
             b.close()
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
-def test_a_captured_prompt_step_follows_its_arrays(be, kind):
+def test_a_captured_prompt_step_follows_its_arrays(be, far, kind):
     """One graph for steps of up to 600 rows: few rows and many, rows in front of the first sequence and behind the last, none at all."""
     from tie_b200 import moe
-    w = World(43, kind, [300, 300], [400, 400], 16, 2, 64, 32)
+    w = World(43, kind, [300, 300], [400, 400], 16, 2, 64, 32, far=far)
     q, _, scale = w.attn(be)
     out = torch.empty_like(q)
     side = torch.cuda.Stream()
@@ -604,11 +613,12 @@ def test_a_captured_prompt_step_follows_its_arrays(be, kind):
     be.synchronize()
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("toks, lens, drafted", SHARES[:2] + SHARES[3:4])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_a_query_that_is_no_number_is_its_own_affair(be, kind, toks, lens, drafted, bad):
-    w = World(44, kind, toks, lens, 16, 2, 64, 32, tree=trees(np.random.default_rng(3), toks) if drafted else None)
+def test_a_query_that_is_no_number_is_its_own_affair(be, far, kind, toks, lens, drafted, bad):
+    w = World(44, kind, toks, lens, 16, 2, 64, 32, tree=trees(np.random.default_rng(3), toks) if drafted else None, far=far)
     q, clean, scale = w.attn(be)
     for t, h in ((0, 3), (w.n - 1, 15)):
         q[t, h, 17] = bad
@@ -619,9 +629,10 @@ def test_a_query_that_is_no_number_is_its_own_affair(be, kind, toks, lens, draft
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
-def test_sequences_may_share_pages(be, kind):
-    w = World(45, kind, [1, 40, 2], [200, 160, 170], 8, 2, 128, 16)
+def test_sequences_may_share_pages(be, far, kind):
+    w = World(45, kind, [1, 40, 2], [200, 160, 170], 8, 2, 128, 16, far=far)
     w.table[1:, :10] = w.table[0, :10]  # a prefix of 160 slots
     w.d_table = torch.tensor(w.table).cuda()
     w.describe()
@@ -629,18 +640,20 @@ def test_sequences_may_share_pages(be, kind):
     w.check_attn(q, out, scale)
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads, kv_heads, toks, lens", [(256, 1, [3], [200]), (1024, 1, [1, 2], [77, 0]), (256, 256, [2, 17], [33, 0]), (1, 1, [150], [9])])
-def test_head_layouts_at_their_ends(be, kind, heads, kv_heads, toks, lens):
-    w = World(46, kind, toks, lens, heads, kv_heads, 64, 16)
+def test_head_layouts_at_their_ends(be, far, kind, heads, kv_heads, toks, lens):
+    w = World(46, kind, toks, lens, heads, kv_heads, 64, 16, far=far)
     q, out, scale = w.attn(be)
     w.check_attn(q, out, scale)
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("scale", [0.0, -1.5])
-def test_scales_of_prompt_pieces(be, kind, scale):
-    w = World(47, kind, [70], [100], 8, 2, 64, 16)
+def test_scales_of_prompt_pieces(be, far, kind, scale):
+    w = World(47, kind, [70], [100], 8, 2, 64, 16, far=far)
     q = torch.randn(70, 8, 64, device="cuda") * torch.logspace(-20, 1, 70, device="cuda")[:, None, None]
     _, out, _ = w.attn(be, q, scale)
     w.check_attn(q, out, scale)
@@ -680,12 +693,13 @@ def test_refusals(be):
     refused(moe.EINVAL, be.qk_norm_rope_ptr, w.cache, w.step, odd[:, :256], kv, kv, q, 4)
 
 
+@pytest.mark.parametrize("far", [False, True])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("how", ["page", "page_high", "len", "len_far", "rows", "start", "tree"])
-def test_wrong_steps_are_reported_and_the_rest_is_right(be, kind, how):
+def test_wrong_steps_are_reported_and_the_rest_is_right(be, far, kind, how):
     from tie_b200 import moe
-    toks, lens = [2, 3], [70, 33]
-    w = World(24, kind, toks, lens, 8, 2, 64, 16)
+    toks, lens, heads = [2, 3], [70, 33], 32 if far else 8
+    w = World(24, kind, toks, lens, heads, 2, 64, 16, far=far)
     q, clean, scale = w.attn(be)
     if how == "page":
         w.d_table[1, 0] = -1
@@ -700,7 +714,7 @@ def test_wrong_steps_are_reported_and_the_rest_is_right(be, kind, how):
     elif how == "start":
         w.tok_start[0] = -3
     else:
-        w = World(24, kind, [70, 3], lens, 8, 2, 64, 16, tree=[1] * 73)
+        w = World(24, kind, [70, 3], lens, heads, 2, 64, 16, tree=[1] * 73, far=far)
         q, clean, scale = None, None, 0.125
     for call in ("attn", "write", "read"):
         if how in ("tree", "page") and call != "attn":  # (slots 33 .. 35 lie in the third page)
@@ -717,7 +731,7 @@ def test_wrong_steps_are_reported_and_the_rest_is_right(be, kind, how):
         assert e.value.code == moe.EKERNEL
         assert "page" in str(e.value) or "step" in str(e.value)
     # the context goes on
-    w = World(24, kind, toks, lens, 8, 2, 64, 16)
+    w = World(24, kind, toks, lens, heads, 2, 64, 16, far=far)
     if q is not None:
         _, out, _ = w.attn(be, q, scale)
         assert torch.equal(out, clean)

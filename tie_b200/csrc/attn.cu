@@ -482,17 +482,28 @@ struct Warp {
 			}
 		}
 		if constexpr (!C::Q8) {
-			// 0 * infinity is not nothing: where a group that not every row sees holds a value that is no number (or that nobody
-			// has written), its products are made one by one
-			bool odd = false;
+			// 0 * infinity is not nothing: where a group that not every row sees holds values that are no numbers, nobody's (stale
+			// slots) become zeros, and the products of the others are made one by one
+			bool odd = false, cleared = false;
 			if (masked) {
 				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
 				for (int i = lane; i < C::GROUP * C::ROW / 4; i += 32) {
+					const int k = (4 * i & (C::PANEL - 1)) >> 7;
 					uint32_t w;
 					asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vs + 4 * i) : "memory");
-					odd = odd || nonfinite16(w, EXPONENT);
+					if (!nonfinite16(w, EXPONENT))
+						continue;
+					if (key0 + k < key_end && (there >> (k >> 4) & 1)) {
+						odd = true;
+					} else {
+						asm volatile("st.shared.u32 [%0], %1;" ::"r"(vs + 4 * i), "r"(0u) : "memory");
+						cleared = true;
+					}
 				}
+				if (cleared)
+					ptx::fence_proxy_async_smem();	// (the next values come in over these stores)
 				odd = __any_sync(0xffffffffu, odd);
+				__syncwarp();
 			}
 			if (odd) {
 				one_by_one(vs, s, alpha, lane);
@@ -897,10 +908,17 @@ int attn_setup(tie_cuda_ctx *c)
 int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind, int head_dim, const float *q, float *out, int n_head, float scale)
 {
 	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * ATTN_LOG2E, c->s.attn_part, c->s.attn_count, c->s.attn_join};
-	// rows of a sequence and key/value head, on average: up to 8 and up to 16 in tiles of that, more in tiles of 128
+	// Rows of a sequence and key/value head, on average: up to 8 and up to 16 in tiles of that.  More go in tiles of 128, which
+	// read the cache once for all of them but take 18 us for the least: where the page table has no room for more slots than
+	// leave a tile of 16 rows and 128 keys to each SM, those are done sooner (12 tokens of 8 heads, F16: 11.7 us where tiles of
+	// 128 take 20.2 with 100 slots in front, 16.1 and 20.2 with 500; with 2000, 3 of these units to an SM, 27.2 and 21.6).
 	const long long rows = ((long long)st.n_tokens * a.group + st.n_seq - 1) / st.n_seq;
-	if (rows > 16)
-		return launch_attn_tc(c, kv, st, kind, head_dim, a);
+	if (rows > 16) {
+		const long long tiles = ((long long)st.n_tokens * a.group + 15) / 16 + st.n_seq - 1;
+		const long long units = (((long long)st.max_pages << kv.page_shift) + ATTN_UNIT - 1) / ATTN_UNIT;
+		if (tiles * kv.n_head_kv * units > c->sm_count)
+			return launch_attn_tc(c, kv, st, kind, head_dim, a);
+	}
 	const bool two = rows > 8;
 	if (kind == TIE_CUDA_KV_F16)
 		return go_kind<TIE_CUDA_KV_F16>(c, kv, st, head_dim, two, a);
