@@ -256,7 +256,8 @@ int tie_cuda_moe_block_inplace_ep(tie_cuda_ctx *c, int layer, float *hidden_dev,
  * writing and for attention.
  *
  * The cache is the caller's: two arrays of device memory, [n_pages][n_head_kv][page_size][head_dim] elements each, 16-byte
- * aligned, and for TIE_CUDA_KV_Q8 two of fp32 factors, [n_pages][n_head_kv][page_size], aligned the same (2^31 - 1 rows at most).  An element of Q8 is a whole number
+ * aligned, and for TIE_CUDA_KV_Q8 two of fp32 factors, [n_pages][n_head_kv][page_size], aligned the same (2^31 - 1 rows at
+ * most, else TIE_CUDA_ENOTSUP).  An element of Q8 is a whole number
  * of -127 .. 127 that stands for itself times its row's factor; rows are written as rint(x / s), s = max|x| / 127 (IEEE
  * divisions).  A row with an infinity or NaN in it reads back as NaN throughout, one whose s would be below 2^-126 as
  * zeros.  F16 rounds to nearest and holds infinities beyond +-65504. */
@@ -283,7 +284,7 @@ typedef struct {
  * TIE_CUDA_NO_SYNC: the next synchronising one) return TIE_CUDA_EKERNEL.  No slot may belong to two rows of one step. */
 typedef struct {
 	int n_seq;		/* 1 .. 1024 */
-	int n_tokens;		/* rows of the step's arrays, 0 included */
+	int n_tokens;		/* rows of the step's arrays, 0 included (times heads: below 2^31 - 2^16) */
 	const int *tok_start;	/* [n_seq + 1], ascending */
 	const int *kv_len;	/* [n_seq] slots in front of this step's tokens */
 	const int *page_table;	/* [n_seq][max_pages] */
@@ -324,7 +325,9 @@ int tie_cuda_kv_read(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_
  * as it is (the step's own tokens must have been written); q, out [n_tokens][n_head][head_dim], n_head a multiple of the
  * cache's n_head_kv, query head h with key/value head h / (n_head / n_head_kv).  A token that sees nothing gets zeros; what
  * stands in slots that a token does not see, NaN included, is nothing to it.  fp32 results: queries and probabilities
- * meet the cache's elements in parts that keep 22 bits (BF16: 24).  out may be q. */
+ * meet the cache's elements in parts that keep 22 bits (BF16: 24; queries against a Q8 cache, where there are few, as whole
+ * numbers of 24 bits relative to their row's largest).  A row that sees a value or a factor that is no number, or is no number
+ * itself, gets infinities or NaN in the dims that depend on it.  out may be q. */
 int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const float *q, int n_head,
 		  float scale, float *out, unsigned flags);
 

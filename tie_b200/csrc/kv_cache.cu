@@ -122,7 +122,8 @@ __device__ __forceinline__ void store_cache_row(uint8_t *rows, float *scales, lo
 	}
 }
 
-// One CTA: one token; a warp takes two or four head rows at a time, the next ones requested before those in hand are worked on,
+// One CTA: one token (4096 tokens with 32 heads of q and 4 each of k and v, BF16: 31.3 us, 5.1 TB/s; one token: 11.4 us, launch and
+// call); a warp takes two or four head rows at a time, the next ones requested before those in hand are worked on,
 // the first before anything is known of the token; blockIdx.y shares the rows of a token out where tokens alone would leave
 // SMs idle.  Two warps find the token's place for all and form its angles, in 64 bits and in turns, so that only the
 // fraction of a turn is rounded to 32: at position 100,000 a 32-bit angle would be off by up to 0.004.
@@ -261,7 +262,7 @@ __device__ __forceinline__ void store_values(O *p, const float (&x)[N])
 }
 
 // One CTA: READ_TOKENS tokens of one head, keys (blockIdx.z 0) or values.  A warp takes a row at a time, so that its stores are
-// whole rows (8 values a thread, two stores of 16 bytes 32 apart: 134 us for 120000 slots of Q8 to fp32), READ_U of them in flight.
+// whole rows (8 values a thread, two stores of 16 bytes 32 apart: 134 us for 120000 slots of Q8 to fp32, now 109, 5.6 TB/s), READ_U of them in flight.
 constexpr int READ_TOKENS = 64, READ_U = READ_TOKENS / WARPS;
 template <int KIND, int D, typename O>
 __global__ void __launch_bounds__(THREADS) kv_read_rows(const KvView kv, const StepView st, O *k_out, O *v_out)
