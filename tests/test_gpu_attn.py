@@ -358,6 +358,18 @@ def test_many_sequences_of_all_lengths(be, far):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_as_many_sequences_as_a_step_has(be, kind):
+    """1024 of them, some empty, more query rows on average than the kernel for few rows takes."""
+    rng = np.random.default_rng(5)
+    toks = rng.integers(0, 6, 1024).tolist()
+    w = World(49, kind, toks, rng.integers(0, 60, 1024).tolist(), 8, 1, 64, 16, far=True)
+    k, v = w.held("k"), w.held("v")
+    w.held = {"k": k, "v": v}.__getitem__
+    q, out, scale = w.attn(be)
+    w.check_attn(q, out, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_long_cache_is_split_and_joined_the_same_every_time(be, kind):
     w = World(15, kind, [1, 2], [20011, 9000], 8, 1, 128, 64)
     q, out, scale = w.attn(be)
