@@ -1023,21 +1023,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	}
 }
 
-// The parts that CTAs left of the items they shared, joined: CTA (c, i) takes 32 rows x 32 dims of the item that began in CTA c
-// and went on behind it, if there is one; its warps take the parts in turn, a lane a row, and are joined in their order.  A
-// launch of its own: an item of a few tiles of keys a CTA has tens of parts of 66 KB, and one CTA, the last at the item,
-// took 130 us to add them up (tree of 13 tokens over 9001 slots: 172 us).
-constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
+// The parts that CTAs left of the items they shared, joined: a CTA takes 32 rows x 32 dims of an item at a time, its warps the
+// parts in turn, a lane a row; they are joined in their order.  A launch of its own: an item of a few tiles of keys a CTA has
+// tens of parts of 66 KB, and one CTA, the last at the item, took 130 us to add them up (tree of 13 tokens over 9001 slots:
+// 172 us).  Every CTA finds the shared items for itself, so that no more of them are launched than run at once (16 for each CTA
+// of the launch before, most with nothing to do: 73.8 us instead of 71.8 for 8 trees of 64 tokens over 3500 keys).
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_CTAS = 4;  // CTAs per SM
 template <int D>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_join(const AttnArgs a)
+__device__ __forceinline__ void join_block(const AttnArgs &a, int c0, int block, float (&s_m)[JOIN_WARPS][32], float (&s_l)[JOIN_WARPS][32], float4 (&s_acc)[JOIN_WARPS][8][32],
+					   int lane, int warp)
 {
-	__shared__ float s_m[JOIN_WARPS][32], s_l[JOIN_WARPS][32];
-	__shared__ float4 s_acc[JOIN_WARPS][8][32];
-	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
-	pdl_wait();
 	const AttnJoin it = a.join[c0];
-	const int n = it.n, first = (blockIdx.y & 3) * 32, r = first + lane, d40 = (blockIdx.y >> 2) * 8;
-	if (it.row0 + first >= it.n_rows)  // (none: no rows)
+	const int n = it.n, first = (block & 3) * 32, r = first + lane, d40 = (block >> 2) * 8;
+	if (it.row0 + first >= it.n_rows)
 		return;
 	constexpr size_t PART = attn_part_floats(ROWS);
 	float top = -INFINITY, sum = 0.0f;
@@ -1060,6 +1058,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_join(const AttnArgs a)
 		for (int j = 0; j < 8; j++)
 			acc[j] = make_float4(fmaf(v[j].x, f, acc[j].x * g), fmaf(v[j].y, f, acc[j].y * g), fmaf(v[j].z, f, acc[j].z * g), fmaf(v[j].w, f, acc[j].w * g));
 	}
+	__syncthreads();  // (the block before has been read)
 	s_m[warp][lane] = top;
 	s_l[warp][lane] = sum;
 #pragma unroll
@@ -1088,6 +1087,26 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_join(const AttnArgs a)
 	reinterpret_cast<float4 *>(dst)[d40 + warp] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
+template <int D>
+__global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) attn_join(const AttnArgs a, int n_cta)
+{
+	constexpr int BLOCKS = ROWS / 32 * (D / 32);
+	__shared__ float s_m[JOIN_WARPS][32], s_l[JOIN_WARPS][32];
+	__shared__ float4 s_acc[JOIN_WARPS][8][32];
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	pdl_wait();
+	int unit = blockIdx.x;	// of the shared items that follow; each has BLOCKS
+	for (int base = 0; base < n_cta; base += 32) {
+		// (all warps find the same)
+		uint32_t shared = __ballot_sync(0xffffffffu, base + lane < n_cta && a.join[min(base + lane, n_cta - 1)].n_rows > 0);
+		for (; shared; shared &= shared - 1) {
+			for (; unit < BLOCKS; unit += gridDim.x)
+				join_block<D>(a, base + __ffs(shared) - 1, unit, s_m, s_l, s_acc, lane, warp);
+			unit -= BLOCKS;
+		}
+	}
+}
+
 template <int KIND, int D>
 int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 {
@@ -1098,7 +1117,7 @@ int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 		return rc;
 	attn_tiles<KIND, D><<<c->sm_count, THREADS, T::SMEM, c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
-	return launch_kernel(c, true, 1, attn_join<D>, dim3(c->sm_count, ROWS / 32 * (D / 32)), JOIN_THREADS, 0, a);
+	return launch_kernel(c, true, 1, attn_join<D>, dim3(JOIN_CTAS * c->sm_count), JOIN_THREADS, 0, a, c->sm_count);
 }
 template <int KIND>
 int allow_smem(tie_cuda_ctx *c)
