@@ -16,10 +16,10 @@
 //     cp.async per 16 bytes the address arithmetic alone took 5000 cycles a tile from two warps);
 //   * two warps each make operands of what came in where it is not one yet: Q8's bytes become fp16 in place, values behind
 //     the last key and values that are no numbers become zeros;
-//   * one thread finds the CTA's pieces of work, one issues the MMAs (one for the scores and one for the products: 49.0 ->
-//     53.1 us below).  Q and P are operands in tensor memory (a step of shared memory then feeds only the keys or dims of the
+//   * one thread finds the CTA's pieces of work, one issues the MMAs (one for the scores and one for the products: 49.0 us
+//     of the piece below became 53.1).  Q and P are operands in tensor memory (a step of shared memory then feeds only the keys or dims of the
 //     other operand: half of what the memory delivers); P's parts of 16 keys take the columns of these keys' scores.
-// What it takes (a piece of 512 tokens over 1500 keys, F16, 32 heads of 128 with 4 of keys: 49.0 us, 300 TFLOP/s, 600 of MMAs):
+// What it takes (a piece of 512 tokens over 1500 keys, F16, 32 heads of 128 with 4 of keys: 47.7 us, 310 TFLOP/s, 620 of MMAs):
 // a tile of 128 keys takes about 3400 cycles where its MMAs take 2050 and its exponentials 1024: the scores of a tile wait
 // for the products of the last but one, and the issuing thread's four waits a tile cost 150 to 400 cycles each, complete or
 // not; 16000 cycles pass before the first scores and 5000 behind the last products.
@@ -59,7 +59,7 @@ struct Shared {
 	Piece piece[PIECES];	// made by a warp of its own: they cost several divisions each
 	uint64_t k_raw[MAX_STAGES], k_full[MAX_STAGES], k_free[MAX_STAGES];  // keys have come in; are the operand; have been used
 	uint64_t v_raw[MAX_STAGES], v_full[MAX_STAGES], v_free[MAX_STAGES];
-	uint64_t s_full[MAX_SLOTS], p_full[MAX_SLOTS], o_full, o_free, q_come, q_full, ml_full[2], fin;
+	uint64_t s_full[MAX_SLOTS], p_full[MAX_SLOTS], o_full, o_free, q_come, q_full, l_full[PIECES], fin;
 	// What the softmax threads need to know of a tile's keys outlives its operand slot, which is free once the scores are
 	// made: tile n + FACTS is requested after the scores of tile n + SLOTS at the least, these after the products of n.
 	uint64_t f_full[MAX_FACTS];
@@ -73,7 +73,9 @@ struct Shared {
 	// what the products of a tile have to be added up with: maximum of a row, factor; whether values are no numbers, bad pages
 	float t_top[TILE_FACTS][ROWS], t_unit[TILE_FACTS];
 	uint32_t t_odd[TILE_FACTS], t_bad[TILE_FACTS];
-	float2 ml[2][2][ROWS];	// per piece in turn and warpgroup: maximum and sum of a row
+	// per piece in turn and warpgroup: sum of a row's p, relative to its maximum in the end.  (Of PIECES, since a piece without
+	// tiles makes nobody wait for the warpgroup that takes them.)
+	float l[PIECES][2][ROWS];
 	uint32_t tmem_base, abort;
 };
 
@@ -579,9 +581,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			ptx::mbar_init(ptx::smem_u32(&sh->v_full[i]), MAKE_THREADS);
 			ptx::mbar_init(ptx::smem_u32(&sh->v_free[i]), 1);
 		}
-		for (int i = 0; i < 2; i++) {
-			ptx::mbar_init(ptx::smem_u32(&sh->ml_full[i]), SOFT_THREADS);
-		}
 		for (int i = 0; i < T::SLOTS; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->s_full[i]), 1);
 			ptx::mbar_init(ptx::smem_u32(&sh->p_full[i]), SOFT_THREADS);
@@ -590,6 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 			ptx::mbar_init(ptx::smem_u32(&sh->f_full[i]), T::SCALED ? MAKE_THREADS : 1);
 		for (int i = 0; i < PIECES; i++) {
 			ptx::mbar_init(ptx::smem_u32(&sh->piece_full[i]), 1);
+			ptx::mbar_init(ptx::smem_u32(&sh->l_full[i]), SOFT_THREADS);
 			ptx::mbar_init(ptx::smem_u32(&sh->piece_free[i]), SOFT_THREADS / 32 + FOLD_THREADS / 32 + 1 + 2 + (T::SCALED ? 4 : 2));  // softmax, fold, MMA, ask, make
 		}
 		ptx::mbar_init(ptx::smem_u32(&sh->o_full), 1);
@@ -804,8 +804,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[score]));
 				l = fmaf(l, alpha, sum.x + sum.y);
 			}
-			sh->ml[n & 1u][wg][r] = make_float2(m, l);
-			ptx::mbar_arrive(ptx::smem_u32(&sh->ml_full[n & 1u]));
+			sh->l[n % PIECES][wg][r] = l;
+			ptx::mbar_arrive(ptx::smem_u32(&sh->l_full[n % PIECES]));
 		}
 	} else if (warp < W_KEYS) {
 		// ================= fold: a thread per row adds the tiles' products up =================
@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				}
 				ptx::tc_fence_before();
 				if (i == p.n_tiles - 1)	 // (what the piece is finished with is read before the piece after the next can be)
-					wait(sh->ml_full[n & 1u], n >> 1 & 1u);
+					wait(sh->l_full[n % PIECES], n / PIECES & 1u);
 				if (odd) {  // infinities and NaN among values that not every row sees: p > 0 times them is what they are
 					const int key0 = p.unit0 * ATTN_UNIT + i * TK;
 #pragma unroll 1
@@ -874,12 +874,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
 			}
 			if (p.n_tiles == 0)
-				wait(sh->ml_full[n & 1u], n >> 1 & 1u);
-			const float2 m0 = sh->ml[n & 1u][0][r], m1 = sh->ml[n & 1u][1][r];
+				wait(sh->l_full[n % PIECES], n / PIECES & 1u);
+			const float sum = sh->l[n % PIECES][0][r] + sh->l[n % PIECES][1][r];  // (relative to the largest maximum, as the products)
 			if (p.n_tiles > 0)
 				ptx::mbar_arrive(ptx::smem_u32(&sh->o_free));
-			// the sums of p, as the products relative to the largest maximum
-			const float sum = (m0.x == -INFINITY ? 0.0f : m0.y * exp2_ftz(m0.x - top)) + (m1.x == -INFINITY ? 0.0f : m1.y * exp2_ftz(m1.x - top));
 			if (!p.whole) {
 				float *part = a.part + (2 * blockIdx.x + (p.first ? 1 : 0)) * attn_part_floats(ROWS);
 				part[ROWS * 128 + r] = top;
