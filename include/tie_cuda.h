@@ -257,10 +257,10 @@ int tie_cuda_moe_block_inplace_ep(tie_cuda_ctx *c, int layer, float *hidden_dev,
  *
  * The cache is the caller's: two arrays of device memory, [n_pages][n_head_kv][page_size][head_dim] elements each, 16-byte
  * aligned, and for TIE_CUDA_KV_Q8 two of fp32 factors, [n_pages][n_head_kv][page_size], aligned the same (2^31 - 1 rows at
- * most, else TIE_CUDA_ENOTSUP).  An element of Q8 is a whole number
- * of -127 .. 127 that stands for itself times its row's factor; rows are written as rint(x / s), s = max|x| / 127 (IEEE
- * divisions).  A row with an infinity or NaN in it reads back as NaN throughout, one whose s would be below 2^-126 as
- * zeros.  F16 rounds to nearest and holds infinities beyond +-65504. */
+ * most, else TIE_CUDA_ENOTSUP).  An element of Q8 is a whole number of -127 .. 127 that stands for itself times its row's
+ * factor; rows are written as rint(x / s), s = max|x| / 127 (IEEE divisions).  A row with an infinity or NaN in it reads
+ * back as NaN throughout, one whose s would be below 2^-126 as zeros.  F16 rounds to nearest and holds infinities beyond
+ * +-65504. */
 #define TIE_CUDA_KV_F32 0 /* rows that tie_cuda_kv_read puts out; no cache has this type */
 #define TIE_CUDA_KV_F16 1
 #define TIE_CUDA_KV_BF16 2 /* KV_CACHE_TYPE, config.h */
