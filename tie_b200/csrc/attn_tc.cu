@@ -214,10 +214,10 @@ template <int KIND, int D>
 struct Tile {
 	static constexpr bool SCALED = KIND == TIE_CUDA_KV_Q8;
 	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	 // of a value of Q and of P
-	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  Heads of 128, two parts: two tiles of
-	// 128 keys take 73.7 us for 8 trees of 64 tokens over 3500 keys (Q8) and 49.0 for a piece of 512 over 1500 (F16), four
-	// of 64 took 10 and 2 us more, since the waits are those of a tile.  Three parts, heads of 64: a third tile of 64
-	// keys brought 4096 tokens from 290 to 266 us.
+	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  Heads of 128, two parts: with two tiles of
+	// 128 keys 8 trees of 64 tokens over 3500 keys (Q8) took 77.9 us and a piece of 512 over 1500 (F16) 53.4, with four of 64
+	// keys 84.5 and 55.1, since each tile has its waits (71.8 and 47.7 now).  Three parts, heads of 64: a third tile of 64 keys
+	// brought 4096 tokens from 290 to 266 us (254 now).
 	static constexpr int TK = PARTS == 3 ? 64 : 128;
 	static constexpr int SLOTS = D == 128 ? 2 : 3;
 	static constexpr int STAGES = TK * D == 128 * 128 || (SCALED && D == 64) ? 2 : 4;
