@@ -206,9 +206,10 @@ struct Warp {
 	static constexpr int KS = D / C::Q_STEP, MB = D / 16, H = C::HALVES;
 	uint32_t q[NB][C::Q_PARTS][KS][2];
 	float row_scale[NB][2];	 // scale * log2 e, and what the row's parts were divided by
-	float acc[NB][MB][4];	 // Q8: in units of v_unit
+	float acc[NB][MB][4];	 // Q8: in units of v_unit, apart: over the row's multiple of p (`more`)
 	float m[NB][2], l[NB][2];  // running maximum (of the whole column), sum (of this lane's keys)
-	float v_unit;		 // Q8: a power of two, of the largest value factor so far
+	float v_unit;		 // Q8: of the largest value factor so far (attn_unit_of)
+	bool apart;		 // Q8: rows have units of their own
 
 	__device__ __forceinline__ void begin(const AttnArgs &a, const SeqView &seq, int head_kv, int row0, int lane)
 	{
@@ -308,13 +309,14 @@ struct Warp {
 				for (int i = 0; i < 4; i++)
 					acc[nb][mb][i] = 0.0f;
 		}
-		v_unit = 0.0f;
+		v_unit = ATTN_LEAST_UNIT;
+		apart = false;
 	}
 
 	// The group of keys from key0 on, in shared memory at `stage`; keys at or behind key_end, and 16 of them whose bit of `there`
-	// is not set, are nobody's.
+	// is not set, are nobody's.  more[..].w, while the rows have units of their own: what a row's p are multiplied by, v_unit over its unit.
 	__device__ __forceinline__ void group(const AttnArgs &a, const StepView &st, const SeqView &seq, uint32_t stage, uint32_t factors, int key0, int key_end, unsigned there, int row0,
-					      int lane)
+					      float4 *more, int lane)
 	{
 		const int g = lane >> 2, c = lane & 3;
 		const uint32_t ks = stage, vs = stage + C::GROUP * C::ROW;
@@ -377,9 +379,10 @@ struct Warp {
 					}
 			}
 		}
-		float v_rel[H][2], unit_change = 1.0f;
+		const bool masked = there != (1u << H) - 1u || key0 + C::GROUP > min(seq.kv_len, key_end);
+		float f[H][2], unit_change = 1.0f;  // Q8: factors of the values, in units of v_unit
 		if constexpr (C::Q8) {
-			float f[H][2], top = 0.0f;
+			float top = 0.0f;
 #pragma unroll
 			for (int h = 0; h < H; h++)
 #pragma unroll
@@ -399,21 +402,18 @@ struct Warp {
 					f[h][i] = fabsf(f[h][i]) <= FLT_MAX ? f[h][i] : __int_as_float(0x7fc00000);
 					top = fmaxf(top, fabsf(f[h][i]));
 				}
-			// the unit: a power of two that no factor so far has reached the double of
-			const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(top)) & 0x7f800000u;
-			const float unit = __uint_as_float(min(max(e, 0x00800000u), 253u << 23));
+			const float unit = attn_unit_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
 			if (unit > v_unit) {
-				unit_change = v_unit * __uint_as_float((254u << 23) - __float_as_uint(unit));
+				unit_change = v_unit * attn_unit_inverse(unit);
 				v_unit = unit;
 			}
-			const float inv = __uint_as_float((254u << 23) - __float_as_uint(v_unit));
+			const float inv = attn_unit_inverse(v_unit);
 #pragma unroll
 			for (int h = 0; h < H; h++)
 #pragma unroll
 				for (int i = 0; i < 2; i++)
-					v_rel[h][i] = f[h][i] * inv;
+					f[h][i] *= inv;
 		}
-		const bool masked = there != (1u << H) - 1u || key0 + C::GROUP > min(seq.kv_len, key_end);
 		if (masked) {
 #pragma unroll
 			for (int nb = 0; nb < NB; nb++)
@@ -434,6 +434,20 @@ struct Warp {
 								s[h][nb][2 * k + i] = -INFINITY;
 						}
 				}
+			if constexpr (C::Q8) {
+				bool far = false;
+#pragma unroll
+				for (int h = 0; h < H; h++)
+#pragma unroll
+					for (int i = 0; i < 2; i++)
+						far = far || !(fabsf(f[h][i]) * ATTN_WIDE >= 1.0f || f[h][i] == 0.0f);  // (or no number)
+				if (!apart && __any_sync(0xffffffffu, far)) {
+					apart = true;
+					if (lane < 8 * NB)
+						more[lane].w = 1.0f;
+					__syncwarp();
+				}
+			}
 		}
 		uint32_t b[NB][H][C::PARTS][2];  // P^T as the second operand
 		float alpha[NB][2];
@@ -453,7 +467,6 @@ struct Warp {
 				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2_ftz(m[nb][i] - top);
 				m[nb][i] = top;
 				l[nb][i] *= alpha[nb][i];
-				alpha[nb][i] *= unit_change;
 			}
 #pragma unroll
 			for (int h = 0; h < H; h++) {
@@ -463,14 +476,45 @@ struct Warp {
 #pragma unroll
 				for (int i = 0; i < 2; i++)
 					l[nb][i] += s[h][nb][i] + s[h][nb][2 + i];
-				if constexpr (C::Q8) {
+			}
+			if constexpr (C::Q8) {
+				if (__builtin_expect(apart, 0)) {
 #pragma unroll
-					for (int i = 0; i < 4; i++) {
-						const float z = s[h][nb][i] * v_rel[h][i >> 1];
-						// (where a row does not see every key, a factor that is no number is nothing to it)
-						s[h][nb][i] = masked && s[h][nb][i] == 0.0f ? 0.0f : z;
+					for (int i = 0; i < 2; i++) {
+						float most = 0.0f;
+#pragma unroll
+						for (int h = 0; h < H; h++)
+#pragma unroll
+							for (int k = 0; k < 2; k++)
+								most = fmaxf(most, s[h][nb][2 * k + i] == 0.0f ? 0.0f : fabsf(f[h][k]));
+						most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+						most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+						most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+						const float was = unit_change * attn_unit_inverse(more[nb * 8 + 2 * c + i].w);  // the row's unit, as a share of v_unit
+						const float m = attn_unit_inverse(fmaxf(was, attn_unit_of(most)));
+						alpha[nb][i] *= was * m;
+						__syncwarp();
+						if (lane < 4)
+							more[nb * 8 + 2 * lane + i].w = m;
+						// (a factor that is no number is nothing to a row that does not see it)
+#pragma unroll
+						for (int h = 0; h < H; h++)
+#pragma unroll
+							for (int k = 0; k < 2; k++)
+								s[h][nb][2 * k + i] = s[h][nb][2 * k + i] == 0.0f ? 0.0f : s[h][nb][2 * k + i] * (f[h][k] * m);
 					}
+				} else {
+					alpha[nb][0] *= unit_change;
+					alpha[nb][1] *= unit_change;
+#pragma unroll
+					for (int h = 0; h < H; h++)
+#pragma unroll
+						for (int i = 0; i < 4; i++)
+							s[h][nb][i] *= f[h][i >> 1];
 				}
+			}
+#pragma unroll
+			for (int h = 0; h < H; h++)
 #pragma unroll
 				for (int k = 0; k < 2; k++) {
 					uint32_t part[C::PARTS];
@@ -479,7 +523,6 @@ struct Warp {
 					for (int p = 0; p < C::PARTS; p++)
 						b[nb][h][p][k] = transpose8x8(part[p]);
 				}
-			}
 		}
 		if constexpr (!C::Q8) {
 			// 0 * infinity is not nothing: where a group that not every row sees holds values that are no numbers, nobody's (stale
@@ -523,10 +566,10 @@ struct Warp {
 						r[i] ^= 0x80808080u;
 #pragma unroll
 					for (int k = 0; k < 2; k++) {
-						f[k][h][0] = int8_pair<0x4240>(r[2 * k]);
-						f[k][h][1] = int8_pair<0x4341>(r[2 * k]);
-						f[k][h][2] = int8_pair<0x4240>(r[2 * k + 1]);
-						f[k][h][3] = int8_pair<0x4341>(r[2 * k + 1]);
+						f[k][h][0] = int8_pair_low<0x4240>(r[2 * k]);
+						f[k][h][1] = int8_pair_low<0x4341>(r[2 * k]);
+						f[k][h][2] = int8_pair_low<0x4240>(r[2 * k + 1]);
+						f[k][h][3] = int8_pair_low<0x4341>(r[2 * k + 1]);
 					}
 				} else {
 					ldsm4_trans(f[0][h], vs + C::place(16 * h + (lane & 7) + 8 * (lane >> 4), 2 * mb + (lane >> 3 & 1)));
@@ -617,7 +660,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ AttnWork work;
 	__shared__ Ring<KIND, D> ring;
-	__shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS], s_w[ROWS][WARPS], s_top[ROWS], s_sum[ROWS], s_unit[WARPS];
+	__shared__ float4 s_row[WARPS][ROWS];  // each warp's: maximum of a row, sum of p, unit of the sums; `more` of Warp::group
+	__shared__ float2 s_all[ROWS];	       // maximum and sum of p of all
+	__shared__ float s_w[ROWS][WARPS];		      // what a warp's sums count for
 	const uint32_t stages = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u, factors = stages + WARPS * C::STAGES * C::STAGE;
 	// [half of the warps][8 rows][D]: sums on their way together
 	float *sums = reinterpret_cast<float *>(smem_raw + (factors - ptx::smem_u32(smem_raw)) + WARPS * C::STAGES * C::FACTORS);
@@ -654,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 		for (int g = p.unit0 * UNIT_GROUPS + warp; g < g_end; g += WARPS, taken++) {
 			const uint32_t slot = taken % C::STAGES, at = warp * C::STAGES + slot;
 			dec_wait(ptx::smem_u32(&ring.full[warp][slot]), st.status, taken / C::STAGES & 1u);
-			w.group(a, st, seq, stages + at * C::STAGE, factors + at * C::FACTORS, g * C::GROUP, p.key_end, ring.there[warp][slot], p.row0, lane);
+			w.group(a, st, seq, stages + at * C::STAGE, factors + at * C::FACTORS, g * C::GROUP, p.key_end, ring.there[warp][slot], p.row0, s_row[warp], lane);
 			__syncwarp();
 			if (lane == 0)
 				ptx::mbar_arrive(ptx::smem_u32(&ring.empty[warp][slot]));
@@ -670,28 +715,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 				sum += __shfl_xor_sync(0xffffffffu, sum, 8);
 				sum += __shfl_xor_sync(0xffffffffu, sum, 16);
 				if (lane < 4) {
-					s_m[warp][nb * 8 + 2 * lane + i] = w.m[nb][i];
-					s_l[warp][nb * 8 + 2 * lane + i] = sum;
+					float4 &to = s_row[warp][nb * 8 + 2 * lane + i];
+					to = make_float4(w.m[nb][i], sum, !C::Q8 ? 1.0f : ATTN_Q8_DOWN * (w.apart ? w.v_unit * attn_unit_inverse(to.w) : w.v_unit), 0.0f);
 				}
 			}
-		if (lane == 0)
-			s_unit[warp] = C::Q8 ? w.v_unit : 1.0f;
-		workers_sync();
-		if (threadIdx.x < ROWS) {
-			const int r = threadIdx.x;
+		auto weigh = [&](int r) {
 			float top = -INFINITY, sum = 0.0f;
 #pragma unroll
 			for (int i = 0; i < WARPS; i++)
-				top = fmaxf(top, s_m[i][r]);
+				top = fmaxf(top, s_row[i][r].x);
 #pragma unroll
 			for (int i = 0; i < WARPS; i++) {
-				const float f = s_m[i][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[i][r] - top);
-				s_w[r][i] = f * s_unit[i];
-				sum = fmaf(s_l[i][r], f, sum);
+				const float4 v = s_row[i][r];
+				const float f = v.x == -INFINITY ? 0.0f : exp2_ftz(v.x - top);
+				s_w[r][i] = C::Q8 ? f * v.z : f;
+				sum = fmaf(v.y, f, sum);
 			}
-			s_top[r] = top;
-			s_sum[r] = sum;
-		}
+			s_all[r] = make_float2(top, sum);
+		};
+		workers_sync();
+		if (threadIdx.x < ROWS)
+			weigh(threadIdx.x);
 		workers_sync();
 		const bool whole = p.unit0 == 0 && p.unit1 == p.item_units;
 		const int n_rows = seq.n_tok * a.group;
@@ -699,6 +743,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 		auto out_row = [&](int r) {
 			const int tok = r / a.group;
 			return a.out + ((long long)(seq.tok0 + tok) * a.n_head + p.head * a.group + (r - tok * a.group)) * D;
+		};
+		auto finished = [](float4 y, float sum) {
+			const float inv = sum == 0.0f ? 0.0f : (C::Q8 ? ATTN_Q8_UP : 1.0f) / sum;
+			return make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 		};
 		// 8 rows: the later warps' sums to the earlier ones, and these by all threads (4 dims of a row each)
 		auto together = [&](auto give, auto take) {
@@ -743,15 +791,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 					if (!whole) {
 						*reinterpret_cast<float4 *>(part + r * D + col) = y;
 					} else if (p.row0 + r < n_rows) {
-						const float inv = s_sum[r] == 0.0f ? 0.0f : 1.0f / s_sum[r];
-						*reinterpret_cast<float4 *>(out_row(p.row0 + r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+						*reinterpret_cast<float4 *>(out_row(p.row0 + r) + col) = finished(y, s_all[r].y);
 					}
 				});
 		if (!whole) {
-			if (threadIdx.x < ROWS) {
-				part[MAX_ROWS * 128 + threadIdx.x] = s_top[threadIdx.x];
-				part[MAX_ROWS * 128 + MAX_ROWS + threadIdx.x] = s_sum[threadIdx.x];
-			}
+			if (threadIdx.x < ROWS)
+				reinterpret_cast<float2 *>(part + MAX_ROWS * 128)[threadIdx.x] = s_all[threadIdx.x];
 			// the CTAs of the item: those of its first and last unit, and all between
 			const int c0 = attn_cta_of(p.first_unit, total, n_cta), c1 = attn_cta_of(p.first_unit + p.item_units - 1, total, n_cta), n = c1 - c0 + 1;
 			__threadfence();
@@ -777,20 +822,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 					for (int i = warp; i < n; i += WARPS) {
 						const float *src = at(i);
 						float4 v[STEPS];
-						float pm[STEPS], pl[STEPS];
+						float2 of[STEPS];
 #pragma unroll
 						for (int k = 0; k < STEPS; k++) {
 							const int r = nb * 8 + k * PER + lane / D4;
 							v[k] = __ldcg(reinterpret_cast<const float4 *>(src + r * D) + lane % D4);
-							pm[k] = __ldcg(src + MAX_ROWS * 128 + r);
-							pl[k] = __ldcg(src + MAX_ROWS * 128 + MAX_ROWS + r);
+							of[k] = __ldcg(reinterpret_cast<const float2 *>(src + MAX_ROWS * 128) + r);
 						}
 #pragma unroll
 						for (int k = 0; k < STEPS; k++) {
-							const float next = fmaxf(top[k], pm[k]);
-							const float f = pm[k] == -INFINITY ? 0.0f : exp2_ftz(pm[k] - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
+							const float next = fmaxf(top[k], of[k].x);
+							const float f = of[k].x == -INFINITY ? 0.0f : exp2_ftz(of[k].x - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
 							top[k] = next;
-							l[k] = fmaf(pl[k], f, l[k] * o);
+							l[k] = fmaf(of[k].y, f, l[k] * o);
 							if (f != 0.0f)
 								sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
 										     fmaf(v[k].w, f, sum[k].w * o));
@@ -798,25 +842,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 					}
 #pragma unroll
 					for (int k = 0; k < STEPS; k++)
-						if (lane % D4 == 0) {
-							s_m[warp][k * PER + lane / D4] = top[k];
-							s_l[warp][k * PER + lane / D4] = l[k];
-						}
+						if (lane % D4 == 0)
+							s_row[warp][k * PER + lane / D4] = make_float4(top[k], l[k], 1.0f, 0.0f);
 					workers_sync();
-					if (threadIdx.x < 8) {
-						const int r = threadIdx.x;
-						float t = -INFINITY, all = 0.0f;
-#pragma unroll
-						for (int k = 0; k < WARPS; k++)
-							t = fmaxf(t, s_m[k][r]);
-#pragma unroll
-						for (int k = 0; k < WARPS; k++) {
-							const float f = s_m[k][r] == -INFINITY ? 0.0f : exp2_ftz(s_m[k][r] - t);
-							s_w[r][k] = f;
-							all = fmaf(s_l[k][r], f, all);
-						}
-						s_sum[r] = all;
-					}
+					if (threadIdx.x < 8)
+						weigh(threadIdx.x);
 					workers_sync();
 					together(
 						[&](float *to, bool add) {
@@ -833,8 +863,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 							const int r = p.row0 + nb * 8 + r8;
 							if (r >= n_rows)
 								return;
-							const float inv = s_sum[r8] == 0.0f ? 0.0f : 1.0f / s_sum[r8];
-							*reinterpret_cast<float4 *>(out_row(r) + col) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+							*reinterpret_cast<float4 *>(out_row(r) + col) = finished(y, s_all[r8].y);
 						});
 				}
 				if (threadIdx.x == 0)

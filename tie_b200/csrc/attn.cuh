@@ -25,10 +25,28 @@ struct AttnArgs {
 	AttnJoin *join;
 };
 
-// What a CTA leaves for a shared item of ROWS rows: [row][D] sums, then [row] maxima, then [row] sums of p.
+// What a CTA leaves for a shared item of ROWS rows: its sums ([row][D] in attn.cu, [D / 4][row][4] in attn_tc.cu), then the maxima, the
+// sums of p.
 __host__ __device__ constexpr size_t attn_part_floats(int rows)
 {
 	return (size_t)rows * (128 + 2);
+}
+
+// Q8's value factors meet p in 16-bit parts, as shares of a unit: a power of two, of the largest factor.  The parts reach down to
+// 2^-38 of it, so that a row must not share the unit of a factor that it does not see: in tiles that not every row sees in full, and
+// whose factors lie further apart than ATTN_WIDE (up to there p of 1 keeps 2^-31 in its parts), each row has a unit of its own.
+constexpr float ATTN_LEAST_UNIT = 0x1p-126f, ATTN_WIDE = 0x1p8f;
+// Sums of Q8's products, not yet divided by the sum of p, are held 2^34 times smaller, so that 2^20 keys with factors of 2^120 do not
+// pass fp32's range: 2^14 lie in the values' operand (int8_pair_low), 2^20 in the unit, which leaves factors of 2^-106 and more all bits.
+constexpr float ATTN_Q8_DOWN = 0x1p-20f, ATTN_Q8_UP = 0x1p34f;
+__device__ __forceinline__ float attn_unit_of(float top)
+{
+	return __uint_as_float(min(max(__float_as_uint(top) & 0x7f800000u, 0x00800000u), 253u << 23));
+}
+// of a unit, or of the inverse of one
+__device__ __forceinline__ float attn_unit_inverse(float unit)
+{
+	return __uint_as_float((254u << 23) - __float_as_uint(unit));
 }
 
 // The work of a launch: items = (sequence, key/value head, tile of query rows), each of as many units as its keys take;
@@ -141,6 +159,15 @@ __device__ __forceinline__ uint32_t int8_pair(uint32_t x_biased)
 {
 	const uint32_t h = __byte_perm(x_biased, 0x64646464u, SEL);
 	const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&h), __half2half2(__ushort_as_half(0x6480)));  // 1152
+	return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// The same, times 2^-14 (fp16's least normal number, so that 1 stays one).
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t int8_pair_low(uint32_t x_biased)
+{
+	const uint32_t h = __byte_perm(x_biased, 0x64646464u, SEL);
+	const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&h), __half2half2(__ushort_as_half(0x0400)), __half2half2(__ushort_as_half(0xac80)));  // -1152 * 2^-14
 	return *reinterpret_cast<const uint32_t *>(&v);
 }
 

@@ -65,24 +65,32 @@ struct Shared {
 	uint64_t f_full[MAX_FACTS];
 	uint32_t bad[MAX_FACTS], bad_values[MAX_STAGES];  // groups of 16 keys of a tile whose page does not exist
 	alignas(16) float k_scale[640];	 // [FACTS][TK]
-	alignas(16) float v_got[256], v_scale[256];  // [STAGES][TK]: factors as they came, and relative to the tile's largest
-	float v_top[MAX_STAGES], make_max[MAX_STAGES][2];
+	alignas(16) float v_got[256], v_scale[256];  // [STAGES][TK]: factors as they came, and as shares of the tile's unit
+	float v_unit[MAX_STAGES], make_max[MAX_STAGES][2];
 	uint32_t odd[MAX_STAGES][2];  // a masked tile's values hold one that is no number (per warp)
-	float q_max[2][ROWS];
+	// of a row, per warpgroup: the largest query of a piece; in tiles of Q8 whose factors lie far apart, the largest share that the row
+	// sees (by then q_full has come in from all who read the other)
+	float row_max[2][ROWS];
 	float half_top[2][2][ROWS];	 // per tile in turn and warpgroup: the largest score of a row
-	// what the products of a tile have to be added up with: maximum of a row, factor; whether values are no numbers, bad pages
+	// what the products of a tile have to be added up with: maximum of a row, unit (below 0: each row's own, by its exponent);
+	// whether values are no numbers, bad pages
 	float t_top[TILE_FACTS][ROWS], t_unit[TILE_FACTS];
 	uint32_t t_odd[TILE_FACTS], t_bad[TILE_FACTS];
 	// per piece in turn and warpgroup: sum of a row's p, relative to its maximum in the end.  (Of PIECES, since a piece without
 	// tiles makes nobody wait for the warpgroup that takes them.)
 	float l[PIECES][2][ROWS];
 	uint32_t tmem_base, abort;
+	uint8_t t_row_unit[TILE_FACTS][ROWS];
 };
 
 // How a launch's work is shared out.  WHOLE: items, several to a CTA.  EVEN: each CTA the same number of units, whatever items
 // they belong to (a CTA then mostly has the end of one and the beginning of another).  PARTS: no more items than CTAs,
 // each cut into as many equal parts as leave one part to a CTA.
 enum Share : int { WHOLE, EVEN, PARTS };
+// Where Q8's factors lie far apart in a tile that not every row sees in full (ATTN_WIDE), a row's p are raised by as much as the largest
+// factor that it sees is below the tile's, so that their products with the shares fill the 16-bit parts again.  Shares are held
+// times 2^WIDE_UP there and p are raised by that much less, for shares down to 2^-200.
+constexpr int WIDE_UP = 100, WIDE_MOST = 104;
 // What a piece costs besides its tiles (set-up, first loads, joins), in units.
 constexpr int PIECE_UNITS = 8;
 struct Walk {
@@ -253,6 +261,18 @@ __device__ __forceinline__ void bar_sync()
 	asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
 
+// The same, and whether any thread brings a true one.
+template <int ID, int N>
+__device__ __forceinline__ bool bar_any(bool mine)
+{
+	uint32_t any;
+	asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+		     : "=r"(any)
+		     : "r"((uint32_t)mine), "n"(ID), "n"(N)
+		     : "memory");
+	return any != 0;
+}
+
 // Bounded; true once the barrier's phase is complete.
 struct Waiter {
 	volatile uint32_t *abort;
@@ -386,6 +406,18 @@ __device__ __forceinline__ RowView row_view(const StepView &st, const Piece &p, 
 	return v;
 }
 
+// Of a tile's keys from `first` on the largest share of a factor that a row sees (out of line: the loops it is called from fill the
+// instruction caches as they are).
+__device__ __noinline__ float largest_share(const float *share, int first, int n, int key0, uint32_t bad, RowView view)
+{
+	float most = 0.0f;
+#pragma unroll 1
+	for (int k = first; k < first + n; k++)
+		if (view.keys(key0 + k, bad >> (k >> 4) & 1u) & 1u)
+			most = fmaxf(most, fabsf(share[k]));
+	return most;
+}
+
 // Requests the tiles of keys (VALUES false) or values: a warp, a lane per page of a tile.
 template <int KIND, int D, bool VALUES>
 __device__ __forceinline__ void ask(const KvView &kv, const StepView &st, Shared *sh, const CUtensorMap *map, uint32_t ring, uint32_t raw, const Waiter &wait,
@@ -489,11 +521,19 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 						if (masked && !there(r))
 							v[j] = make_uint4(0, 0, 0, 0);
 						const uint32_t b[4] = {v[j].x ^ 0x80808080u, v[j].y ^ 0x80808080u, v[j].z ^ 0x80808080u, v[j].w ^ 0x80808080u};
-						sts128(at + T::place(r, 2 * ch), make_uint4(int8_pair<0x4140>(b[0]), int8_pair<0x4342>(b[0]), int8_pair<0x4140>(b[1]), int8_pair<0x4342>(b[1])));
-						sts128(at + T::place(r, 2 * ch + 1), make_uint4(int8_pair<0x4140>(b[2]), int8_pair<0x4342>(b[2]), int8_pair<0x4140>(b[3]), int8_pair<0x4342>(b[3])));
+						uint4 lo, hi;
+						if constexpr (VALUES) {
+							lo = make_uint4(int8_pair_low<0x4140>(b[0]), int8_pair_low<0x4342>(b[0]), int8_pair_low<0x4140>(b[1]), int8_pair_low<0x4342>(b[1]));
+							hi = make_uint4(int8_pair_low<0x4140>(b[2]), int8_pair_low<0x4342>(b[2]), int8_pair_low<0x4140>(b[3]), int8_pair_low<0x4342>(b[3]));
+						} else {
+							lo = make_uint4(int8_pair<0x4140>(b[0]), int8_pair<0x4342>(b[0]), int8_pair<0x4140>(b[1]), int8_pair<0x4342>(b[1]));
+							hi = make_uint4(int8_pair<0x4140>(b[2]), int8_pair<0x4342>(b[2]), int8_pair<0x4140>(b[3]), int8_pair<0x4342>(b[3]));
+						}
+						sts128(at + T::place(r, 2 * ch), lo);
+						sts128(at + T::place(r, 2 * ch + 1), hi);
 					}
 				}
-				if constexpr (VALUES) {	 // factors relative to the tile's largest, which multiplies the tile's sums
+				if constexpr (VALUES) {	 // factors as shares of a unit, which multiplies the tile's sums
 					constexpr int EACH = T::TK / MAKE_THREADS;
 					float f[EACH];
 					float top = 0.0f;
@@ -504,19 +544,16 @@ __device__ __forceinline__ void make(Shared *sh, uint32_t ring, uint32_t raw, co
 						f[j] = fabsf(f[j]) <= FLT_MAX ? f[j] : __int_as_float(0x7fc00000);
 						top = fmaxf(top, fabsf(f[j]));
 					}
-#pragma unroll
-					for (int o = 16; o; o >>= 1)
-						top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+					top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // (as the number that its bits are)
 					if (lane == 0)
 						sh->make_max[slot][t >> 5] = top;
 					bar_sync<2, MAKE_THREADS>();
-					top = fmaxf(sh->make_max[slot][0], sh->make_max[slot][1]);
-					top = top > 0.0f ? top : 1.0f;
+					const float unit = attn_unit_of(fmaxf(sh->make_max[slot][0], sh->make_max[slot][1]));
 					if (t == 0)
-						sh->v_top[slot] = top;
+						sh->v_unit[slot] = unit;
 #pragma unroll
 					for (int j = 0; j < EACH; j++)
-						sh->v_scale[slot * T::TK + t + MAKE_THREADS * j] = f[j] / top;
+						sh->v_scale[slot * T::TK + t + MAKE_THREADS * j] = f[j] * attn_unit_inverse(unit);
 				}
 			} else if (masked) {
 				constexpr uint32_t EXPONENT = KIND == TIE_CUDA_KV_F16 ? 0x7c00u : 0x7f80u;
@@ -566,6 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 	extern __shared__ uint8_t smem_raw[];
 	__shared__ Shared shared;
 	__shared__ AttnWork work;
+	static_assert(T::SMEM + sizeof(Shared) + sizeof(AttnWork) <= 227 * 1024, "shared memory of a CTA");
 	Shared *sh = &shared;
 	const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
 	constexpr int TK = T::TK;
@@ -653,9 +691,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 					top = fmaxf(fmaxf(fmaxf(top, fabsf(__uint_as_float(x.x))), fmaxf(fabsf(__uint_as_float(x.y)), fabsf(__uint_as_float(x.z)))),
 						    fabsf(__uint_as_float(x.w)));
 				}
-				sh->q_max[wg][r] = top;
+				sh->row_max[wg][r] = top;
 				bar_sync<1, SOFT_THREADS>();
-				top = fmaxf(sh->q_max[0][r], sh->q_max[1][r]);
+				top = fmaxf(sh->row_max[0][r], sh->row_max[1][r]);
 				// the row is brought to 1 .. 2 by a power of two (any fp32 row then keeps its 22 bits); it also takes the scale's sign
 				const int e = top > 0.0f ? min(max((int)(__float_as_uint(top) >> 23), 1), 253) : 127;
 				float down = copysignf(__uint_as_float((uint32_t)(254 - e) << 23), a.scale_log2e);
@@ -751,19 +789,38 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				sh->half_top[i & 1][wg][r] = top;
 				bar_sync<1, SOFT_THREADS>();
 				top = fmaxf(m, fmaxf(top, sh->half_top[i & 1][wg ^ 1][r]) * row_scale);
-				const float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
+				float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
 				const float alpha = m == -INFINITY ? 0.0f : exp2_ftz(m - top);
 				m = top;
 				// the values' factors, and whether all of them are numbers; read before P is handed over: when its products are
 				// made the slot is another tile's
 				if (T::SCALED || masked)
 					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
+				bool wide = false;
+				int up = 0;  // p are larger by 2^up
+				if (T::SCALED && masked) {
+					const float share = fabsf(sh->v_scale[slot * TK + r]);
+					wide = bar_any<1, SOFT_THREADS>(share * ATTN_WIDE < 1.0f && share != 0.0f);
+				}
+				if (wide) {
+					if (wg == 0)
+						sh->v_scale[slot * TK + r] *= __uint_as_float((127u + WIDE_UP) << 23);
+					bar_sync<1, SOFT_THREADS>();
+					sh->row_max[wg][r] = largest_share(&sh->v_scale[slot * TK], wg * CHUNKS * 32, CHUNKS * 32, key0, bad, view);
+					bar_sync<1, SOFT_THREADS>();
+					const int e = __float_as_uint(sh->v_unit[slot]) >> 23;
+					const int share = (int)(__float_as_uint(attn_unit_of(fmaxf(sh->row_max[0][r], sh->row_max[1][r]))) >> 23) - 127;
+					up = min(max(-share, -WIDE_UP), min(WIDE_MOST, e - WIDE_UP - 1));
+					base += (float)up;
+					if (wg == 0)
+						sh->t_row_unit[tiles % TILE_FACTS][r] = (uint8_t)(e - up - WIDE_UP);
+				}
 				if (wg == 0)
 					sh->t_top[tiles % TILE_FACTS][r] = top;
 				if (threadIdx.x == 0) {
 					sh->t_odd[tiles % TILE_FACTS] = masked ? sh->odd[slot][0] | sh->odd[slot][1] : 0u;
 					sh->t_bad[tiles % TILE_FACTS] = bad;
-					sh->t_unit[tiles % TILE_FACTS] = T::SCALED ? sh->v_top[slot] : 1.0f;
+					sh->t_unit[tiles % TILE_FACTS] = !T::SCALED ? 1.0f : wide ? -1.0f : sh->v_unit[slot] * ATTN_Q8_DOWN;
 				}
 				float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
@@ -802,7 +859,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
 				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[score]));
-				l = fmaf(l, alpha, sum.x + sum.y);
+				l = fmaf(l, alpha, T::SCALED ? (sum.x + sum.y) * __uint_as_float((uint32_t)(127 - up) << 23) : sum.x + sum.y);
 			}
 			sh->l[n % PIECES][wg][r] = l;
 			ptx::mbar_arrive(ptx::smem_u32(&sh->l_full[n % PIECES]));
@@ -831,7 +888,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tc_fence_after();
 				// relative to the largest maximum so far (the tiles' are those of the two warpgroups)
 				const float t_top = sh->t_top[at][r], next = fmaxf(top, t_top);
-				const float f = t_top == -INFINITY ? 0.0f : exp2_ftz(t_top - next) * sh->t_unit[at], g = top == -INFINITY ? 0.0f : exp2_ftz(top - next);
+				float unit = sh->t_unit[at];
+				if (T::SCALED && unit < 0.0f)
+					unit = __uint_as_float((uint32_t)sh->t_row_unit[at][r] << 23) * ATTN_Q8_DOWN;
+				const float f = t_top == -INFINITY ? 0.0f : exp2_ftz(t_top - next) * unit, g = top == -INFINITY ? 0.0f : exp2_ftz(top - next);
 				const bool odd = KIND != TIE_CUDA_KV_Q8 && sh->t_odd[at];
 				const uint32_t bad = sh->t_bad[at];
 				top = next;
@@ -888,7 +948,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				continue;
 			}
 			// whole rows go out by 16 dims through shared memory, each warp its 32: 4 lanes then store 64 bytes of a row
-			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+			const float inv = sum == 0.0f ? 0.0f : (T::SCALED ? ATTN_Q8_UP : 1.0f) / sum;
 			long long at[4];
 #pragma unroll
 			for (int i = 0; i < 4; i++) {
@@ -1027,7 +1087,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 // 172 us).  Every CTA finds the shared items for itself, so that no more of them are launched than run at once (16 for each CTA
 // of the launch before, most with nothing to do: 73.8 us instead of 71.8 for 8 trees of 64 tokens over 3500 keys).
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32, JOIN_CTAS = 4;  // CTAs per SM
-template <int D>
+template <int D, bool SCALED>
 __device__ __forceinline__ void join_block(const AttnArgs &a, int c0, int block, float (&s_m)[JOIN_WARPS][32], float (&s_l)[JOIN_WARPS][32], float4 (&s_acc)[JOIN_WARPS][8][32],
 					   int lane, int warp)
 {
@@ -1079,13 +1139,13 @@ __device__ __forceinline__ void join_block(const AttnArgs &a, int c0, int block,
 	}
 	if (it.row0 + r >= it.n_rows)
 		return;
-	const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+	const float inv = sum == 0.0f ? 0.0f : (SCALED ? ATTN_Q8_UP : 1.0f) / sum;
 	const int t = (it.row0 + r) / a.group;
 	float *dst = a.out + ((long long)(it.tok0 + t) * a.n_head + it.head * a.group + (it.row0 + r - t * a.group)) * D;
 	reinterpret_cast<float4 *>(dst)[d40 + warp] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
-template <int D>
+template <int D, bool SCALED>
 __global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) attn_join(const AttnArgs a, int n_cta)
 {
 	constexpr int BLOCKS = ROWS / 32 * (D / 32);
@@ -1099,7 +1159,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) attn_join(const AttnA
 		uint32_t shared = __ballot_sync(0xffffffffu, base + lane < n_cta && a.join[min(base + lane, n_cta - 1)].n_rows > 0);
 		for (; shared; shared &= shared - 1) {
 			for (; unit < BLOCKS; unit += gridDim.x)
-				join_block<D>(a, base + __ffs(shared) - 1, unit, s_m, s_l, s_acc, lane, warp);
+				join_block<D, SCALED>(a, base + __ffs(shared) - 1, unit, s_m, s_l, s_acc, lane, warp);
 			unit -= BLOCKS;
 		}
 	}
@@ -1115,7 +1175,7 @@ int go(tie_cuda_ctx *c, const KvView &kv, const StepView &st, const AttnArgs &a)
 		return rc;
 	attn_tiles<KIND, D><<<c->sm_count, THREADS, T::SMEM, c->stream>>>(kv, st, a, map[0], map[1]);
 	TIE_CUDA_LAUNCHED(c);
-	return launch_kernel(c, true, 1, attn_join<D>, dim3(JOIN_CTAS * c->sm_count), JOIN_THREADS, 0, a, c->sm_count);
+	return launch_kernel(c, true, 1, attn_join<D, T::SCALED>, dim3(JOIN_CTAS * c->sm_count), JOIN_THREADS, 0, a, c->sm_count);
 }
 template <int KIND>
 int allow_smem(tie_cuda_ctx *c)
