@@ -327,7 +327,8 @@ int tie_cuda_kv_read(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_
  * stands in slots that a token does not see, NaN included, is nothing to it.  fp32 results: queries and probabilities
  * meet the cache's elements in parts that keep 22 bits (BF16: 24; queries against a Q8 cache, where there are few, as whole
  * numbers of 24 bits relative to their row's largest; Q8: a probability times a value's factor, down to 2^-31 of the largest factor
- * that the row sees).  A row that sees a value or a factor that is no number, or is no number
+ * that the row sees).  Values may be as large as their type has them: sum_j p_j v_j, the largest p 1, may be 2^20 times what Q8's largest
+ * factors and 2^15 times what BF16's largest values make.  A row that sees a value or a factor that is no number, or is no number
  * itself, gets infinities or NaN in the dims that depend on it.  out may be q. */
 int tie_cuda_attn(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step, const float *q, int n_head,
 		  float scale, float *out, unsigned flags);

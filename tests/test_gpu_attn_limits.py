@@ -61,3 +61,16 @@ def test_q8_values_of_any_size(be, far, power, toks, lens, drafted):
     q, out, scale = w.attn(be)
     assert out.isfinite().all()
     w.check_attn(q, out, scale)
+
+
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("power", [124, -80])
+@pytest.mark.parametrize("toks, lens, drafted", [([1], [300], False), ([1, 2], [5000, 40], False), ([20, 3], [700, 9], True), ([600], [64], False)])
+def test_bf16_values_of_any_size(be, far, power, toks, lens, drafted):
+    w = World(63, "bf16", toks, lens, 16, 2, 64, 32, tree=trees(np.random.default_rng(3), toks) if drafted else None, far=far)
+    w.v = (w.v.float() * 2.0 ** power).bfloat16()
+    assert w.v.isfinite().all()
+    w.describe()
+    q, out, scale = w.attn(be)
+    assert out.isfinite().all()
+    w.check_attn(q, out, scale)

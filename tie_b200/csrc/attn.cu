@@ -463,7 +463,7 @@ struct Warp {
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
 				top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-				base[i] = (top == -INFINITY ? 0.0f : top) - ATTN_P_SHIFT;
+				base[i] = (top == -INFINITY ? 0.0f : top) - ATTN_P_SHIFT<KIND>;
 				alpha[nb][i] = m[nb][i] == -INFINITY ? 0.0f : exp2_ftz(m[nb][i] - top);
 				m[nb][i] = top;
 				l[nb][i] *= alpha[nb][i];

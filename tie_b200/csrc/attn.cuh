@@ -5,7 +5,10 @@
 
 namespace tie {
 
-constexpr float ATTN_P_SHIFT = 14.0f;  // p is held as p * 2^14: fp16 parts of it reach down to 2^-38 of the largest
+// p is held times a power of two.  2^14 where its parts are fp16, which then reach down to 2^-38 of the largest; 2^-15 where they are bf16,
+// whose values may be as large as fp32's: 2^15 keys with the largest p and the largest values still have a sum.
+template <int KIND>
+constexpr float ATTN_P_SHIFT = KIND == TIE_CUDA_KV_BF16 ? -15.0f : 14.0f;
 constexpr float ATTN_LOG2E = 1.4426950408889634f;
 constexpr int ATTN_UNIT = 128;	       // keys: what an item's work is counted in
 constexpr int ATTN_MAX_ROWS = 128;     // query rows of a tile, at most

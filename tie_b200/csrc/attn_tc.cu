@@ -789,7 +789,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				sh->half_top[i & 1][wg][r] = top;
 				bar_sync<1, SOFT_THREADS>();
 				top = fmaxf(m, fmaxf(top, sh->half_top[i & 1][wg ^ 1][r]) * row_scale);
-				float base = ATTN_P_SHIFT - (top == -INFINITY ? 0.0f : top);
+				float base = ATTN_P_SHIFT<KIND> - (top == -INFINITY ? 0.0f : top);
 				const float alpha = m == -INFINITY ? 0.0f : exp2_ftz(m - top);
 				m = top;
 				// the values' factors, and whether all of them are numbers; read before P is handed over: when its products are
