@@ -74,3 +74,39 @@ def test_bf16_values_of_any_size(be, far, power, toks, lens, drafted):
     q, out, scale = w.attn(be)
     assert out.isfinite().all()
     w.check_attn(q, out, scale)
+
+
+# A key with a value that is no number, of a score so low that its p is 0: in front of the step (another warp's or CTA's keys than those that
+# count), among the step's own tokens (of which not every row sees all).
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("toks, lens, drafted, slot", [
+    ([1], [300], False, 7), ([1], [5000], False, 4800), ([30], [100], False, 110), ([30], [100], False, 3), ([30], [40], True, 45), ([64], [2000], True, 1000), ([200], [900], False, 1000),
+])
+def test_a_value_that_is_no_number_is_seen_where_its_probability_is_nothing(be, far, kind, bad, toks, lens, drafted, slot):
+    w = World(64, kind, toks, lens, 8, 1, 64, 16, tree=trees(np.random.default_rng(4), toks) if drafted else None, far=far)
+    q = torch.tensor(w.rng.standard_normal((w.rows, 8, 64)), dtype=torch.float32).cuda() + 1.0
+    # every query is about 1 in each dim: this key's scores are about -64 * 4 * scale below the others'
+    pg, pl = (int(x[0]) for x in w.slots(0, slot, slot + 1))
+    w.k[pg, :, pl] = -120 if kind == "q8" else -40
+    if kind == "q8":
+        w.k_scale[pg, :, pl] = 1.0 / 3
+    _, clean, scale = w.attn(be, q, 1.0)
+    sees = torch.tensor(w.sees(0, 0)[:, slot]).cuda()
+    assert sees.any() and clean.isfinite().all()
+    if kind == "q8":
+        w.v_scale[pg, :, pl] = bad
+    else:
+        w.v[pg, :, pl, 5] = bad
+    _, out, _ = w.attn(be, q, 1.0)
+    hit = out[sees] if kind == "q8" else out[sees][..., 5:6]
+    assert not hit.isfinite().any()
+    rest = out.clone()
+    if kind == "q8":
+        rest[sees] = clean[sees]
+    else:
+        rest[sees, :, 5] = clean[sees, :, 5]
+    # the others' products may be made one by one: another order of the same sums
+    assert (rest - clean).abs().max() <= 2.0 ** -17 * w.v_scale[w.v_scale.isfinite()].abs().max() * 127 if kind == "q8" else \
+        (rest - clean).abs().max() <= 2.0 ** -17 * 8

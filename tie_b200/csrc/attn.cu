@@ -441,11 +441,19 @@ struct Warp {
 #pragma unroll
 					for (int i = 0; i < 2; i++)
 						far = far || !(fabsf(f[h][i]) * ATTN_WIDE >= 1.0f || f[h][i] == 0.0f);  // (or no number)
-				if (!apart && __any_sync(0xffffffffu, far)) {
-					apart = true;
-					if (lane < 8 * NB)
+				if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
+					if (!apart && lane < 8 * NB)
 						more[lane].w = 1.0f;
 					__syncwarp();
+					apart = true;
+					// (in the products below 0 times what is no number is 0, for the rows that do not see it)
+#pragma unroll
+					for (int h = 0; h < H; h++)
+#pragma unroll
+						for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+							for (int i = 0; i < 4; i++)
+								l[nb][i & 1] = s[h][nb][i] != -INFINITY && f[h][i >> 1] != f[h][i >> 1] ? f[h][i >> 1] : l[nb][i & 1];
 				}
 			}
 		}
@@ -549,7 +557,7 @@ struct Warp {
 				__syncwarp();
 			}
 			if (odd) {
-				one_by_one(vs, s, alpha, lane);
+				one_by_one(a, st, seq, vs, s, alpha, key0, key_end, there, row0, lane);
 				return;
 			}
 		}
@@ -599,8 +607,18 @@ struct Warp {
 		return C::Q8 ? 16 * mb + 2 * (lane >> 2) + (i >> 1) : 16 * mb + (lane >> 2) + 8 * (i >> 1);
 	}
 
-	__device__ __forceinline__ void one_by_one(uint32_t vs, const float (&p)[H][NB][4], const float (&alpha)[NB][2], int lane)
+	__device__ __forceinline__ void one_by_one(const AttnArgs &a, const StepView &st, const SeqView &seq, uint32_t vs, const float (&p)[H][NB][4],
+						   const float (&alpha)[NB][2], int key0, int key_end, unsigned there, int row0, int lane)
 	{
+		int tok[NB][2];
+		unsigned long long bits[NB][2];
+#pragma unroll
+		for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+			for (int i = 0; i < 2; i++) {
+				tok[nb][i] = min((row0 + nb * 8 + 2 * (lane & 3) + i) / a.group, seq.n_tok - 1);
+				bits[nb][i] = st.tree ? st.tree[seq.tok0 + tok[nb][i]] : 0;
+			}
 #pragma unroll
 		for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -609,8 +627,12 @@ struct Warp {
 				for (int i = 0; i < 4; i++)
 					acc[nb][mb][i] *= alpha[nb][i & 1];
 #pragma unroll 1
-		for (int k = 0; k < C::GROUP; k++) {
+		for (int k = 0; k < C::GROUP && key0 + k < key_end; k++) {
+			if (!(there >> (k >> 4) & 1))
+				continue;
+			const int j = key0 + k - seq.kv_len;
 			float pk[NB][2];
+			bool sees[NB][2];
 #pragma unroll
 			for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -619,6 +641,7 @@ struct Warp {
 					if (H == 2 && k >= 16)
 						mine = k & 8 ? p[H - 1][nb][2 + i] : p[H - 1][nb][i];
 					pk[nb][i] = __shfl_sync(0xffffffffu, mine, (k & 7) * 4 + (lane & 3));
+					sees[nb][i] = j < 0 || (st.tree ? j < KV_MAX_TREE && (bits[nb][i] >> j & 1) : j <= tok[nb][i]);
 				}
 #pragma unroll
 			for (int mb = 0; mb < MB; mb++)
@@ -632,7 +655,7 @@ struct Warp {
 					for (int nb = 0; nb < NB; nb++)
 #pragma unroll
 						for (int i = 0; i < 2; i++)
-							if (pk[nb][i] != 0.0f)
+							if (sees[nb][i])
 								acc[nb][mb][2 * h + i] = fmaf(pk[nb][i], v, acc[nb][mb][2 * h + i]);
 				}
 		}
@@ -780,8 +803,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 #pragma unroll
 							for (int h = 0; h < 2; h++) {
 								float &d = to[r * D + w.dim(mb, 2 * h, lane)];
-								// (a warp whose keys the row does not see has nothing to give)
-								const float v = f == 0.0f ? 0.0f : w.acc[nb][mb][2 * h + i] * f;
+								const float v = w.acc[nb][mb][2 * h + i] * f;
 								d = add ? d + v : v;
 							}
 					}
@@ -835,9 +857,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const S
 							const float f = of[k].x == -INFINITY ? 0.0f : exp2_ftz(of[k].x - next), o = top[k] == -INFINITY ? 0.0f : exp2_ftz(top[k] - next);
 							top[k] = next;
 							l[k] = fmaf(of[k].y, f, l[k] * o);
-							if (f != 0.0f)
-								sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
-										     fmaf(v[k].w, f, sum[k].w * o));
+							sum[k] = make_float4(fmaf(v[k].x, f, sum[k].x * o), fmaf(v[k].y, f, sum[k].y * o), fmaf(v[k].z, f, sum[k].z * o),
+									     fmaf(v[k].w, f, sum[k].w * o));
 						}
 					}
 #pragma unroll

@@ -89,8 +89,8 @@ struct Shared {
 enum Share : int { WHOLE, EVEN, PARTS };
 // Where Q8's factors lie far apart in a tile that not every row sees in full (ATTN_WIDE), a row's p are raised by as much as the largest
 // factor that it sees is below the tile's, so that their products with the shares fill the 16-bit parts again.  Shares are held
-// times 2^WIDE_UP there and p are raised by that much less, for shares down to 2^-200.
-constexpr int WIDE_UP = 100, WIDE_MOST = 104;
+// times 2^WIDE_UP there and p are raised by that much less, or p of 1 would pass fp32's range for shares of 2^-114.
+constexpr int WIDE_UP = 100;
 // What a piece costs besides its tiles (set-up, first loads, joins), in units.
 constexpr int PIECE_UNITS = 8;
 struct Walk {
@@ -406,15 +406,15 @@ __device__ __forceinline__ RowView row_view(const StepView &st, const Piece &p, 
 	return v;
 }
 
-// Of a tile's keys from `first` on the largest share of a factor that a row sees (out of line: the loops it is called from fill the
-// instruction caches as they are).
+// Of a tile's keys from `first` on the largest share of a factor that a row sees, NaN where one is no number (out of line: the loops it is
+// called from fill the instruction caches as they are).
 __device__ __noinline__ float largest_share(const float *share, int first, int n, int key0, uint32_t bad, RowView view)
 {
 	float most = 0.0f;
 #pragma unroll 1
 	for (int k = first; k < first + n; k++)
 		if (view.keys(key0 + k, bad >> (k >> 4) & 1u) & 1u)
-			most = fmaxf(most, fabsf(share[k]));
+			most = most == most && share[k] == share[k] ? fmaxf(most, fabsf(share[k])) : __int_as_float(0x7fc00000);
 	return most;
 }
 
@@ -796,21 +796,30 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				// made the slot is another tile's
 				if (T::SCALED || masked)
 					wait(sh->v_full[slot], tiles / T::STAGES & 1u);
-				bool wide = false;
+				bool special = false, wide = false;
 				int up = 0;  // p are larger by 2^up
+				float lost = 0.0f;
 				if (T::SCALED && masked) {
 					const float share = fabsf(sh->v_scale[slot * TK + r]);
-					wide = bar_any<1, SOFT_THREADS>(share * ATTN_WIDE < 1.0f && share != 0.0f);
+					const bool far = share * ATTN_WIDE < 1.0f && share != 0.0f;
+					special = bar_any<1, SOFT_THREADS>(far || share != share);
+					if (special)
+						wide = bar_any<1, SOFT_THREADS>(far);
+				}
+				if (special) {
+					// (in the products below 0 times what is no number is 0, for the rows that do not see it)
+					const float most = largest_share(&sh->v_scale[slot * TK], wg * CHUNKS * 32, CHUNKS * 32, key0, bad, view);
+					lost = most == most ? 0.0f : most;
+					sh->row_max[wg][r] = most;
 				}
 				if (wide) {
+					bar_sync<1, SOFT_THREADS>();
 					if (wg == 0)
 						sh->v_scale[slot * TK + r] *= __uint_as_float((127u + WIDE_UP) << 23);
 					bar_sync<1, SOFT_THREADS>();
-					sh->row_max[wg][r] = largest_share(&sh->v_scale[slot * TK], wg * CHUNKS * 32, CHUNKS * 32, key0, bad, view);
-					bar_sync<1, SOFT_THREADS>();
 					const int e = __float_as_uint(sh->v_unit[slot]) >> 23;
-					const int share = (int)(__float_as_uint(attn_unit_of(fmaxf(sh->row_max[0][r], sh->row_max[1][r]))) >> 23) - 127;
-					up = min(max(-share, -WIDE_UP), min(WIDE_MOST, e - WIDE_UP - 1));
+					const int share = (int)(__float_as_uint(attn_unit_of(fmaxf(sh->row_max[0][r], sh->row_max[1][r]))) >> 23) - 127 + WIDE_UP;
+					up = min(max(-share, -WIDE_UP), e - WIDE_UP - 1);
 					base += (float)up;
 					if (wg == 0)
 						sh->t_row_unit[tiles % TILE_FACTS][r] = (uint8_t)(e - up - WIDE_UP);
@@ -859,7 +868,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles(const KvView kv, const 
 				ptx::tmem_st_wait();
 				ptx::tc_fence_before();
 				ptx::mbar_arrive(ptx::smem_u32(&sh->p_full[score]));
-				l = fmaf(l, alpha, T::SCALED ? (sum.x + sum.y) * __uint_as_float((uint32_t)(127 - up) << 23) : sum.x + sum.y);
+				l = fmaf(l, alpha, T::SCALED ? (sum.x + sum.y) * __uint_as_float((uint32_t)(127 - up) << 23) + lost : sum.x + sum.y);
 			}
 			sh->l[n % PIECES][wg][r] = l;
 			ptx::mbar_arrive(ptx::smem_u32(&sh->l_full[n % PIECES]));
