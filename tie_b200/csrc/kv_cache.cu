@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) qk_norm_rope_rows(const KvView 
 	using R = Row<D>;
 	constexpr int HALF = D / 2;
 	__shared__ float2 s_turn[HALF];	 // cos, sin
-	__shared__ int s_place[3];	 // is a sequence's; slot (-1: has none); page
+	__shared__ int s_place[2];	 // slot (-1: has none), page
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x, l = lane % R::LANES;
 	const int rows = a.n_head + 2 * kv.n_head_kv, step = WRITE_WARPS * gridDim.y * R::AT_ONCE;
 	int r = (blockIdx.y * WRITE_WARPS + warp) * R::AT_ONCE + lane / R::LANES;
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(WRITE_THREADS) qk_norm_rope_rows(const KvView 
 				slot = seq.kv_len + i;
 				page = st.page_table[(long long)s * st.max_pages + (slot >> kv.page_shift)];
 			}
-			if (a.rotate && threadIdx.x < HALF) {
-				const int pos = st.pos ? st.pos[t] : max(slot, 0);
+			if (a.rotate && slot >= 0 && threadIdx.x < HALF) {
+				const int pos = st.pos ? st.pos[t] : slot;
 				const double turns = pos * rope.turns[threadIdx.x], part = turns - rint(turns);
 				float2 cs;
 				sincospif((float)(2.0 * part), &cs.y, &cs.x);
@@ -168,15 +168,15 @@ __global__ void __launch_bounds__(WRITE_THREADS) qk_norm_rope_rows(const KvView 
 			}
 		}
 		if (threadIdx.x == 0) {
-			s_place[0] = s >= 0;
-			s_place[1] = slot;
-			s_place[2] = page;
+			s_place[0] = slot;
+			s_place[1] = page;
 		}
 	}
 	__syncthreads();
-	if (!s_place[0])
-		return;	 // a row behind the last sequence
-	const int slot = s_place[1], page = s_place[2], in_page = slot & ((1 << kv.page_shift) - 1);
+	const int slot = s_place[0], page = s_place[1];
+	if (slot < 0)
+		return;	 // a row that no sequence has, or has no slot for
+	const int in_page = slot & ((1 << kv.page_shift) - 1);
 	float2 turn[4];
 	if (a.rotate)
 #pragma unroll
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) qk_norm_rope_rows(const KvView 
 		if (r_warp + R::AT_ONCE <= a.n_head)
 			continue;  // (of these rows none is the cache's)
 		const int head = is_v ? r - a.n_head - kv.n_head_kv : r - a.n_head;
-		const long long page_row = !is_q && r < rows && slot >= 0 ? kv_page_row(kv, st, page, head) : -1;
+		const long long page_row = !is_q && r < rows ? kv_page_row(kv, st, page, head) : -1;
 		store_cache_row<KIND, D>(is_v ? kv.v : kv.k, is_v ? kv.v_scale : kv.k_scale, page_row < 0 ? -1 : page_row + in_page, x.v, l);
 	}
 }
