@@ -278,7 +278,8 @@ typedef struct {
 /* The tokens of a step.  Sequence s has rows tok_start[s] .. tok_start[s+1] - 1 of the step's arrays (none, if they are
  * equal); its row i belongs to its slot kv_len[s] + i, and slot j lies in page page_table[s][j / page_size] at place
  * j % page_size.  For rows that no sequence has (a padded batch: n_tokens above tok_start[n_seq]) nothing is written, and what
- * stands in them is nothing to the others; they are there all the same: every array has n_tokens rows, which may be read.
+ * stands in them is nothing to the others; they are there all the same: q, k, v and their outputs have n_tokens rows, which may be
+ * read.
  * The arrays are device memory, read by the kernels: a captured step follows them when it is replayed.
  * What does not fit - a page number outside the cache, rows outside [0, n_tokens), negative lengths, slots behind the row
  * of the page table, more than 64 tokens of a sequence with a tree - is left out by the kernels and makes the call (with

@@ -132,3 +132,43 @@ def test_a_tree_of_too_many_tokens_is_its_own_affair(be, far, kind):
     refused(w.attn, be, q, 0.125, out=out)
     for s in (0, 2):
         check_sequence(w, s, q, out, 0.125)
+
+
+def test_a_fused_array_may_be_handed_over_whole(be):
+    """q's rows are the first values of the rows of a contiguous array that holds k and v behind them."""
+    w = World(72, "f16", [2, 5], [3, 30], 8, 2, 64, 16)
+    both = torch.tensor(w.rng.standard_normal((7, 12 * 64)), dtype=torch.float32).cuda()
+    k, v = both[:, 8 * 64:10 * 64], both[:, 10 * 64:]
+    outs = []
+    for q in (both[:, :8 * 64].contiguous(), both[:, :8 * 64], both, both.view(7, 12, 64)):
+        outs.append(torch.empty(7, 8, 64, device="cuda"))
+        torch.cuda.synchronize()
+        be.qk_norm_rope_ptr(w.cache, w.step, q, k, v, outs[-1], 8)
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
+def test_arrays_that_do_not_fit_are_refused_before_a_kernel_sees_them(be):
+    from tie_b200 import moe
+    w = World(73, "f16", [2, 5], [3, 30], 8, 2, 64, 16)
+    q, kv = torch.zeros(7, 8, 64, device="cuda"), torch.zeros(7, 2, 64, device="cuda")
+    before = be.launch_count
+
+    def no(call, *a, **k):
+        with pytest.raises(moe.TieCudaError) as e:
+            call(*a, **k)
+        assert e.value.code == moe.EINVAL
+
+    no(be.attn_ptr, w.cache, w.step, q[:6], q, 8, 0.1)
+    no(be.attn_ptr, w.cache, w.step, q, q.half(), 8, 0.1)
+    no(be.attn_ptr, w.cache, w.step, q.cpu(), q, 8, 0.1)
+    no(be.qk_norm_rope_ptr, w.cache, w.step, q[:, :4].contiguous(), kv, kv, q, 8)
+    no(be.qk_norm_rope_ptr, w.cache, w.step, q, kv[:6], kv, q, 8)
+    no(be.qk_norm_rope_ptr, w.cache, w.step, q, kv, kv.cpu(), q, 8)
+    no(be.qk_norm_rope_ptr, w.cache, w.step, q, kv, kv, q[:6], 8)
+    no(be.qk_norm_rope_ptr, w.cache, w.step, q, kv, kv, q, 8, q_norm_w=torch.ones(32, device="cuda"))
+    no(be.kv_read_ptr, w.cache, w.step, kv, kv[:6].clone())
+    no(be.kv_read_ptr, w.cache, w.step, kv, kv, moe.KV_F16)
+    no(be.kv_read_ptr, w.cache, w.step, kv.half(), kv.bfloat16(), moe.KV_F16)
+    no(moe.KvStep, w.tok_start.long(), w.kv_len, w.d_table, 7)
+    no(moe.KvCache, moe.KV_BF16, w.k, w.v)
+    assert be.launch_count == before

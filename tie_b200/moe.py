@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -42,6 +43,7 @@ EXPORTS = [
 EP_HANDLE_BYTES = 64
 EP_PEER_POINTERS, EP_PEER_IPC_HANDLES = 0, 1
 KV_F32, KV_F16, KV_BF16, KV_Q8 = 0, 1, 2, 3  # types of a cache (F32: of rows read back only)
+_ELEMENTS = {KV_F32: ("float32",), KV_F16: ("float16", "int16", "uint16"), KV_BF16: ("bfloat16", "int16", "uint16"), KV_Q8: ("int8", "uint8")}
 PHASES = ["router", "sort", "split", "gate_up", "swiglu", "down", "combine"]  # swiglu: 0, gate_up makes it (tie_cuda_get_profile)
 
 
@@ -159,13 +161,14 @@ def load_library() -> ctypes.CDLL:
     L.tie_cuda_mat_mat.restype = i32
     L.tie_cuda_mat_mat.argtypes = [vp, vp, vp, vp, i32, i32, i32, u32]
     L.tie_cuda_qk_norm_rope.restype = i32
-    L.tie_cuda_qk_norm_rope.argtypes = [vp, vp, vp, vp, u32]
+    kv_cache, kv_step = ctypes.POINTER(KvCache), ctypes.POINTER(KvStep)  # (take the structures themselves: no byref() a call)
+    L.tie_cuda_qk_norm_rope.argtypes = [vp, kv_cache, kv_step, vp, u32]
     L.tie_cuda_kv_read.restype = i32
-    L.tie_cuda_kv_read.argtypes = [vp, vp, vp, vp, vp, i32, u32]
+    L.tie_cuda_kv_read.argtypes = [vp, kv_cache, kv_step, vp, vp, i32, u32]
     L.tie_cuda_attn_block_inplace.restype = i32
-    L.tie_cuda_attn_block_inplace.argtypes = [vp, vp, vp, vp, vp, u32]
+    L.tie_cuda_attn_block_inplace.argtypes = [vp, vp, kv_cache, kv_step, vp, u32]
     L.tie_cuda_attn.restype = i32
-    L.tie_cuda_attn.argtypes = [vp, vp, vp, vp, i32, f32, vp, u32]
+    L.tie_cuda_attn.argtypes = [vp, kv_cache, kv_step, vp, i32, f32, vp, u32]
     _lib = L
     return L
 
@@ -191,9 +194,29 @@ def _ptr(a):
     raise TypeError(type(a))
 
 
+def _refuse(what: str, why: str):
+    raise TieCudaError(EINVAL, what, why)
+
+
+_type_names = {}  # of dtypes, without their module
+
+
+def _type_name(a) -> str:
+    return _type_names.get(a.dtype) or _type_names.setdefault(a.dtype, str(a.dtype).split(".")[-1])
+
+
+def _check_array(a, what: str, name: str, types):
+    """A tensor that kernels read: of one of `types`, on the device (or pinned)."""
+    t = _type_name(a)
+    if t not in types:
+        _refuse(what, f"{name} is {t}, not {' or '.join(types)}")
+    if not (getattr(a, "is_cuda", False) or (hasattr(a, "is_pinned") and a.is_pinned())):
+        _refuse(what, f"{name} is not on the device")
+
+
 class KvCache(ctypes.Structure):
     """tie_cuda_kv_cache over the caller's tensors: k, v [n_pages][n_head_kv][page_size][head_dim] of the type that `kind`
-    names (KV_Q8: int8, with fp32 k_scale, v_scale [n_pages][n_head_kv][page_size])."""
+    names, or 16- or 8-bit whole numbers with its bits (KV_Q8: int8, with fp32 k_scale, v_scale [n_pages][n_head_kv][page_size])."""
     _fields_ = [
         ("type", ctypes.c_int), ("n_head_kv", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
         ("n_pages", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
@@ -205,6 +228,13 @@ class KvCache(ctypes.Structure):
         assert tuple(v.shape) == tuple(k.shape)
         for x in (k_scale, v_scale):
             assert x is None or tuple(x.shape) == tuple(k.shape[:3])
+        types = _ELEMENTS.get(kind)
+        for name, x in (("k", k), ("v", v)):
+            if types:  # (a kind that no cache has is the library's to refuse)
+                _check_array(x, "KvCache", name, types)
+        for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if x is not None:
+                _check_array(x, "KvCache", name, ("float32",))
         super().__init__(kind, n_head_kv, head_dim, page_size, n_pages, _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale))
         self.keep = (k, v, k_scale, v_scale)
 
@@ -220,6 +250,11 @@ class KvStep(ctypes.Structure):
     def __init__(self, tok_start, kv_len, page_table, n_tokens: int, tree=None, pos=None):
         n_seq, max_pages = page_table.shape
         assert tok_start.shape[0] == n_seq + 1 and kv_len.shape[0] == n_seq
+        for name, x in (("tok_start", tok_start), ("kv_len", kv_len), ("page_table", page_table), ("pos", pos)):
+            if x is not None and not isinstance(x, int):
+                _check_array(x, "KvStep", name, ("int32",))
+        if tree is not None and not isinstance(tree, int):
+            _check_array(tree, "KvStep", "tree", ("int64", "uint64"))
         super().__init__(n_seq, n_tokens, _ptr(tok_start), _ptr(kv_len), _ptr(page_table), max_pages, _ptr(tree), _ptr(pos))
         self.keep = (tok_start, kv_len, page_table, tree, pos)
 
@@ -231,6 +266,9 @@ class AttnQkv(ctypes.Structure):
         ("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p), ("norm_eps", ctypes.c_float),
         ("rope_base", ctypes.c_float), ("rope_interleaved", ctypes.c_int), ("q_out", ctypes.c_void_p),
     ]
+
+
+_QKV = struct.Struct("<i4xQQQqqqQQffi4xQ")
 
 
 class AttnWeights(ctypes.Structure):
@@ -248,17 +286,59 @@ class AttnWeights(ctypes.Structure):
         self.keep = (wq, wk, wv, wo, norm_w, q_norm_w, k_norm_w)
 
 
-def _rows_ptr(a, width: int):
-    """Address and row stride (in elements) of a tensor of rows, each `width` contiguous elements; an int address has them one behind the other."""
+_dtypes = [None] * 4  # of the values of KV_F32 .. KV_Q8: torch's own, once a tensor of it has come in (torch is not imported here)
+
+
+def _is_of(a, kind: int) -> bool:
+    if not hasattr(a, "data_ptr") or _type_name(a) not in _ELEMENTS[kind]:
+        return False
+    if _type_name(a) == _ELEMENTS[kind][0]:
+        _dtypes[kind] = a.dtype
+    return True
+
+
+# (The two below run for every array of every call: as many questions as it takes, each of which is a tenth of a microsecond.)
+def _values_ptr(a, count: int, device: int, what: str, name: str, kind: int = 0):
+    """Address of a contiguous tensor of `kind` (KV_F32) with `count` values or more; an int or None is taken as it is."""
+    if a is None or isinstance(a, int):
+        return a
+    if (a.dtype is not _dtypes[kind] and not _is_of(a, kind)) or a.numel() < count or not a.is_contiguous():
+        _refuse(what, f"{name} is not {count} or more contiguous values of {_ELEMENTS[kind][0]}")
+    if a.get_device() != device and not a.is_pinned():
+        _refuse(what, f"{name} is not on the context's device")
+    return a.data_ptr()
+
+
+def _rows_ptr(a, width: int, n_rows: int, device: int, what: str, name: str):
+    """Address and row stride (in elements) of n_rows rows of `width` contiguous fp32 values in a tensor: row i is a[i], or its first
+    values where that is longer; a contiguous tensor with other leading dimensions has the rows one behind the other, and so has
+    an int address."""
     if isinstance(a, int):
         return a, width
-    if a.is_contiguous():
+    if (a.dtype is not _dtypes[KV_F32] and not _is_of(a, KV_F32)) or (a.get_device() != device and not a.is_pinned()):
+        _refuse(what, f"{name} is not of fp32 on the context's device")
+    numel, whole = a.numel(), a.is_contiguous()
+    if whole and numel == n_rows * width:  # (the usual call)
         return a.data_ptr(), width
-    want = 1
-    for n, s in zip(reversed(a.shape[1:]), reversed(a.stride()[1:])):
-        assert n == 1 or s == want, "the values of a token's row must be contiguous"
-        want *= n
-    return a.data_ptr(), a.stride(0) if a.shape[0] > 1 else max(width, a.stride(0))
+    shape, stride = a.shape, a.stride()
+    if not whole:
+        row = 1
+        for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
+            assert n == 1 or s == row, "the values of a token's row must be contiguous"
+            row *= n
+        if row < width or shape[0] < n_rows:
+            _refuse(what, f"{name} has {shape[0]} rows of {row} values, not {n_rows} of {width}")
+        return a.data_ptr(), stride[0] if shape[0] > 1 else max(width, stride[0])
+    if len(shape) > 1 and shape[0] >= n_rows and shape[0] * width <= numel:
+        return a.data_ptr(), numel // shape[0] if numel else width
+    # rows one behind the other: their ends are ends of a's, or within its first dimension
+    row, i = 1, len(shape) - 1
+    while i > 0 and row * shape[i] <= width:
+        row *= shape[i]
+        i -= 1
+    if numel < n_rows * width or (row != width and (i > 0 or width % max(row, 1))):
+        _refuse(what, f"{name} of shape {tuple(shape)} has not {n_rows} rows of {width} values")
+    return a.data_ptr(), width
 
 
 class MoeBackend:
@@ -279,7 +359,7 @@ class MoeBackend:
         self.hidden, self.n_expert, self.top_k, self.ffn_dim = hidden, n_expert, top_k, ffn_dim
         self.n_layers, self.max_tokens = n_layers, max_tokens
         self.ep_rank, self.ep_size = ep_rank, ep_size
-        self._host_keep = {}
+        self._host_keep, self.device = {}, device
 
     # -- lifetime --
     def close(self):
@@ -465,23 +545,47 @@ class MoeBackend:
     def qk_norm_rope_ptr(self, cache: KvCache, step: KvStep, q, k, v, q_out, n_head: int, q_norm_w=None, k_norm_w=None,
                          norm_eps: float = 1e-6, rope_base: float = 1e6, rope_interleaved: bool = False, flags: int = DEVICE):
         """q, k, v: [n_tokens][..] rows, which may be slices of one array (the row stride is taken from the tensor)."""
-        kv_width = cache.n_head_kv * cache.head_dim
-        (qp, qs), (kp, ks), (vp, vs) = _rows_ptr(q, n_head * cache.head_dim), _rows_ptr(k, kv_width), _rows_ptr(v, kv_width)
-        qkv = AttnQkv(n_head, qp, kp, vp, qs, ks, vs, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, rope_base, int(rope_interleaved), _ptr(q_out))
-        rc = self.L.tie_cuda_qk_norm_rope(self.h, ctypes.byref(cache), ctypes.byref(step), ctypes.byref(qkv), flags)
-        self._check(rc, "tie_cuda_qk_norm_rope")
+        dim = cache.head_dim
+        kv_width = cache.n_head_kv * dim
+        what, n, dev = "tie_cuda_qk_norm_rope", step.n_tokens, self.device
+        qp, qs = _rows_ptr(q, n_head * dim, n, dev, what, "q")
+        kp, ks = _rows_ptr(k, kv_width, n, dev, what, "k")
+        vp, vs = _rows_ptr(v, kv_width, n, dev, what, "v")
+        # (AttnQkv's bytes: to fill a ctypes structure takes four times as long)
+        qw, kw = _values_ptr(q_norm_w, dim, dev, what, "q_norm_w") or 0, _values_ptr(k_norm_w, dim, dev, what, "k_norm_w") or 0
+        op = _values_ptr(q_out, n * n_head * dim, dev, what, "q_out") or 0
+        try:
+            qkv = _QKV.pack(n_head, qp, kp, vp, qs, ks, vs, qw, kw, norm_eps, rope_base, 1 if rope_interleaved else 0, op)
+        except (struct.error, OverflowError) as e:
+            _refuse(what, str(e))
+        rc = self.L.tie_cuda_qk_norm_rope(self.h, cache, step, qkv, flags)
+        if rc:
+            self._check(rc, what)
 
     def kv_read_ptr(self, cache: KvCache, step: KvStep, k_out, v_out, out_type: int = KV_F32, flags: int = DEVICE):
-        rc = self.L.tie_cuda_kv_read(self.h, ctypes.byref(cache), ctypes.byref(step), _ptr(k_out), _ptr(v_out), out_type, flags)
-        self._check(rc, "tie_cuda_kv_read")
+        what, count, dev = "tie_cuda_kv_read", step.n_tokens * cache.n_head_kv * cache.head_dim, self.device
+        if 0 <= out_type < KV_Q8:
+            k_out, v_out = _values_ptr(k_out, count, dev, what, "k_out", out_type), _values_ptr(v_out, count, dev, what, "v_out", out_type)
+        else:  # (the library's to refuse)
+            k_out, v_out = _ptr(k_out), _ptr(v_out)
+        rc = self.L.tie_cuda_kv_read(self.h, cache, step, k_out, v_out, out_type, flags)
+        if rc:
+            self._check(rc, what)
 
     def attn_ptr(self, cache: KvCache, step: KvStep, q, out, n_head: int, scale: float, flags: int = DEVICE):
-        rc = self.L.tie_cuda_attn(self.h, ctypes.byref(cache), ctypes.byref(step), _ptr(q), n_head, scale, _ptr(out), flags)
-        self._check(rc, "tie_cuda_attn")
+        what, count, dev = "tie_cuda_attn", step.n_tokens * n_head * cache.head_dim, self.device
+        rc = self.L.tie_cuda_attn(self.h, cache, step, _values_ptr(q, count, dev, what, "q"), n_head, scale,
+                                  _values_ptr(out, count, dev, what, "out"), flags)
+        if rc:
+            self._check(rc, what)
 
     def attn_block_inplace_ptr(self, weights: AttnWeights, cache: KvCache, step: KvStep, hidden, flags: int = DEVICE):
-        rc = self.L.tie_cuda_attn_block_inplace(self.h, ctypes.byref(weights), ctypes.byref(cache), ctypes.byref(step), _ptr(hidden), flags)
-        self._check(rc, "tie_cuda_attn_block_inplace")
+        what, dev = "tie_cuda_attn_block_inplace", self.device
+        for name, a, count in zip(("norm_w", "q_norm_w", "k_norm_w"), getattr(weights, "keep", ())[4:], (self.hidden, cache.head_dim, cache.head_dim)):
+            _values_ptr(a, count, dev, what, name)
+        rc = self.L.tie_cuda_attn_block_inplace(self.h, ctypes.byref(weights), cache, step,
+                                                _values_ptr(hidden, step.n_tokens * self.hidden, dev, what, "hidden"), flags)
+        self._check(rc, what)
 
     # -- math_dispatch rows --
     def make_current(self):
