@@ -172,3 +172,19 @@ def test_arrays_that_do_not_fit_are_refused_before_a_kernel_sees_them(be):
     no(moe.KvStep, w.tok_start.long(), w.kv_len, w.d_table, 7)
     no(moe.KvCache, moe.KV_BF16, w.k, w.v)
     assert be.launch_count == before
+
+
+def test_a_factor_that_is_no_number_behind_a_bad_page(be):
+    """Keys that all rows see, a warp's second ones behind a group with a page missing and factors far apart: a factor that is no number
+    is seen although its key's probability is nothing."""
+    w = World(74, "q8", [1] * 40, [2000] * 40, 8, 1, 64, 16)
+    q = torch.tensor(w.rng.standard_normal((40, 8, 64)), dtype=torch.float32).cuda() + 1.0
+    for s in range(40):
+        pg, pl = (int(x[0]) for x in w.slots(s, 50, 51))
+        w.v_scale[pg, :, pl] *= 1e6
+        pg, pl = (int(x[0]) for x in w.slots(s, 300, 301))
+        w.k[pg, :, pl], w.k_scale[pg, :, pl], w.v_scale[pg, :, pl] = -120, 1.0 / 3, float("nan")
+    w.d_table[:, 2] = -1
+    out = torch.zeros_like(q)
+    refused(w.attn, be, q, 1.0, out=out)
+    assert out.isnan().all()

@@ -434,7 +434,9 @@ struct Warp {
 								s[h][nb][2 * k + i] = -INFINITY;
 						}
 				}
-			if constexpr (C::Q8) {
+		}
+		if constexpr (C::Q8) {
+			if (masked || apart) {
 				bool far = false;
 #pragma unroll
 				for (int h = 0; h < H; h++)
