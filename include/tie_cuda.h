@@ -316,7 +316,8 @@ typedef struct {
 /* q_out = rotate(norm(q)); the cache's slots of the step's tokens = rotate(norm(k)), v (model_qwen3.c:312-380: the norms of
  * queries and keys for each head, the rotation and the store into the cache).  norm(x) = x * w / sqrt(mean(x^2) + eps) over
  * a head.  Angles are formed in 64 bits.  The entry points from here to tie_cuda_attn take device pointers (TIE_CUDA_DEVICE, with or
- * without TIE_CUDA_NO_SYNC), arrays of floats and of rows 16-byte aligned (else TIE_CUDA_EINVAL), and allocate nothing: a
+ * without TIE_CUDA_NO_SYNC), arrays of floats and of rows 16-byte aligned (q_norm_w and k_norm_w 4; else TIE_CUDA_EINVAL), and
+ * allocate nothing: a
  * caller may capture them into a graph of its own (TIE_CUDA_GRAPH is ignored).  Calls of one
  * context share its scratch and follow one another on its stream; so have replays of graphs that were captured from it. */
 int tie_cuda_qk_norm_rope(tie_cuda_ctx *c, const tie_cuda_kv_cache *cache, const tie_cuda_kv_step *step,

@@ -673,9 +673,9 @@ constexpr size_t smem_bytes()
 
 // One CTA per SM, each an equal share of the launch's units of 128 keys; a worker warp takes every eighth group of 16 or 32 keys
 // through a ring of its own, so that no warp waits for another until the sums are joined.  Bound by HBM where there is much
-// to read (48 tokens over 20,000 slots each, F16: 313 us, 6.3 TB/s; over 5000: 73 us, 5.2 TB/s; one token over 100,003, Q8: 32
-// us, 3.3 TB/s: 4 us until the first keys are there, 8 from the last ones to the joined row) and by one chain of latencies
-// where there is little (one token over 500: 9.6 us, launch included).
+// to read (48 tokens over 20,000 slots each, F16: 313 us, 6.3 TB/s; over 5000: 73 us, 5.2 TB/s; one token over 100,003, Q8: 31
+// us, 3.4 TB/s: 4 us until the first keys are there, 8 from the last ones to the joined row) and by one chain of latencies
+// where there is little (one token over 500: 11.0 us, launch and call included).
 template <int KIND, int D, int NB>
 __global__ void __launch_bounds__(THREADS, 1) attn_rows(const KvView kv, const StepView st, const AttnArgs a, const __grid_constant__ CUtensorMap k_map,
 							const __grid_constant__ CUtensorMap v_map)
@@ -966,9 +966,13 @@ int launch_attn(tie_cuda_ctx *c, const KvView &kv, const StepView &st, int kind,
 {
 	AttnArgs a = {q, out, n_head, n_head / kv.n_head_kv, scale * ATTN_LOG2E, c->s.attn_part, c->s.attn_count, c->s.attn_join};
 	// Rows of a sequence and key/value head, on average: up to 8 and up to 16 in tiles of that.  More go in tiles of 128, which
-	// read the cache once for all of them but take 18 us for the least: where the page table has no room for more slots than
-	// leave a tile of 16 rows and 128 keys to each SM, those are done sooner (12 tokens of 8 heads, F16: 11.7 us where tiles of
-	// 128 take 20.2 with 100 slots in front, 16.1 and 20.2 with 500; with 2000, 3 of these units to an SM, 27.2 and 21.6).
+	// read the cache once for all of them but take 22 us for the least: where the page table has no room for more slots than
+	// leave a tile of 16 rows and 128 keys to each SM, those are done sooner (12 tokens of 8 heads, F16: 12.9 us where tiles of
+	// 128 take 27.8 with 100 slots in front, 17.9 and 23.3 with 500, 30.8 and 23.6 with 1000, 29.3 and 24.4 with 2000).  What the host
+	// does not see decides neither: a table of 4096 slots over 100 used ones takes the 27.8.
+	// A step of both kinds goes one way as a whole.  A piece of 512 beside single tokens, F16 / Q8, over the sum of both by
+	// themselves: 47 over 4000 slots 171 us of 172 / 224 of 170; 250 over 1000 (tiles) 187 of 156 / 212 of 142; 700 over 1000 (few rows)
+	// 751 of 306 / 624 of 270.
 	const long long rows = ((long long)st.n_tokens * a.group + st.n_seq - 1) / st.n_seq;
 	if (rows > 16) {
 		const long long tiles = ((long long)st.n_tokens * a.group + 15) / 16 + st.n_seq - 1;

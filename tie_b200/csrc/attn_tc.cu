@@ -19,7 +19,7 @@
 //   * one thread finds the CTA's pieces of work, one issues the MMAs (one for the scores and one for the products: 49.0 us
 //     of the piece below became 53.1).  Q and P are operands in tensor memory (a step of shared memory then feeds only the keys or dims of the
 //     other operand: half of what the memory delivers); P's parts of 16 keys take the columns of these keys' scores.
-// What it takes (a piece of 512 tokens over 1500 keys, F16, 32 heads of 128 with 4 of keys: 47.7 us, 310 TFLOP/s, 620 of MMAs):
+// What it takes (a piece of 512 tokens over 1500 keys, F16, 32 heads of 128 with 4 of keys: 47.3 us, 312 TFLOP/s, 620 of MMAs):
 // a tile of 128 keys takes about 3400 cycles where its MMAs take 2050 and its exponentials 1024: the scores of a tile wait
 // for the products of the last but one, and the issuing thread's four waits a tile cost 150 to 400 cycles each, complete or
 // not; 16000 cycles pass before the first scores and 5000 behind the last products.
@@ -224,8 +224,8 @@ struct Tile {
 	static constexpr int PARTS = KIND == TIE_CUDA_KV_BF16 ? 3 : 2;	 // of a value of Q and of P
 	// Keys of a tile, and score tiles: as many as tensor memory holds beside Q and O.  Heads of 128, two parts: with two tiles of
 	// 128 keys 8 trees of 64 tokens over 3500 keys (Q8) took 77.9 us and a piece of 512 over 1500 (F16) 53.4, with four of 64
-	// keys 84.5 and 55.1, since each tile has its waits (71.8 and 47.7 now).  Three parts, heads of 64: a third tile of 64 keys
-	// brought 4096 tokens from 290 to 266 us (254 now).
+	// keys 84.5 and 55.1, since each tile has its waits (71.6 and 47.3 now).  Three parts, heads of 64: a third tile of 64 keys
+	// brought 4096 tokens from 290 to 266 us (257 now).
 	static constexpr int TK = PARTS == 3 ? 64 : 128;
 	static constexpr int SLOTS = D == 128 ? 2 : 3;
 	static constexpr int STAGES = TK * D == 128 * 128 || (SCALED && D == 64) ? 2 : 4;

@@ -122,7 +122,7 @@ __device__ __forceinline__ void store_cache_row(uint8_t *rows, float *scales, lo
 	}
 }
 
-// One CTA: one token (4096 tokens with 32 heads of q and 4 each of k and v, BF16: 31.3 us, 5.1 TB/s; one token: 11.4 us, launch and
+// One CTA: one token (4096 tokens with 32 heads of q and 4 each of k and v, BF16: 30.7 us, 5.2 TB/s; one token: 11.8 us, launch and
 // call); a warp takes two or four head rows at a time, the next ones requested before those in hand are worked on,
 // the first before anything is known of the token; blockIdx.y shares the rows of a token out where tokens alone would leave
 // SMs idle.  Two warps find the token's place for all and form its angles, in 64 bits and in turns, so that only the
